@@ -10,7 +10,7 @@ from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libaegist_mixer.so"
 
-F32, BF16, I8 = 0, 1, 2
+F32, BF16, I8, Q4 = 0, 1, 2, 3
 
 P = C.c_void_p
 I = C.c_int
@@ -91,6 +91,16 @@ SIGNATURES: dict[str, tuple] = {
     "aegist_moe_experts": (I, [P, P, P, P, P, I, I, I, I, I, P, P, P, SZ, P]),
     "aegist_shared_gate_add": (I, [P, P, P, P, I, I, P]),
     "aegist_silu_mul": (I, [P, P, P, LL, P]),
+    "aegist_q4_bytes": (SZ, [I, I, I]),
+    "aegist_q4_quantize": (I, [P, I, LL, P, I, I, I, P]),
+    "aegist_q4_pack": (I, [P, P, P, P, I, I, I, P]),
+    "aegist_q4_dequantize": (I, [P, P, I, I, I, P]),
+    "aegist_linear_q4": (I, [P, I, LL, P, P, LL, I, I, I, I, I, P, SZ, P]),
+    "aegist_linear_q4_workspace_bytes": (SZ, [I, I, I, I, I]),
+    "aegist_token_logprobs": (I, [P, I, LL, P, P, P, P, P, I, I, I, P, SZ, P]),
+    "aegist_token_logprobs_workspace_bytes": (SZ, [I, I, I]),
+    "aegist_head_logprobs": (I, [P, I, LL, P, I, P, P, P, P, P, P, I, I, I, I, I, P, SZ, P]),
+    "aegist_head_logprobs_workspace_bytes": (SZ, [I, I, I, I, I, I, I]),
 }
 
 

@@ -10,9 +10,11 @@ provider here: no op computes anything in torch.
 """
 from __future__ import annotations
 
+from typing import NamedTuple
+
 import torch
 
-from ._lib import BF16, F32, I8, AegistError, call, lib
+from ._lib import BF16, F32, I8, Q4, AegistError, call, lib
 
 _DT = {torch.float32: F32, torch.bfloat16: BF16}
 
@@ -422,6 +424,209 @@ def gemv_bf16(x, weight, y=None):
         y = torch.empty(N, dtype=torch.float32, device=x.device)
     call("aegist_gemv_bf16", _p(x), _p(weight), _p(y), N, K, _stream())
     return y
+
+
+# --- projections with 4-bit weights, and what an output head answers ----------------------------
+
+def _call_on(device, name: str, *args):
+    """call() on the current stream of `device`, which need not be the current device."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        call(name, *args, _stream(device))
+    else:
+        with torch.cuda.device(device):
+            call(name, *args, _stream(device))
+
+
+def _one_device(*ts):
+    """The device that all the given tensors are on."""
+    dev = ts[0].device
+    for t in ts[1:]:
+        if t is not None and t.device != dev:
+            raise AegistError("device", -1, f"tensors on {dev} and {t.device}: one device expected")
+    return dev
+
+
+def _scratch(nbytes: int, device):
+    """Workspace of one call: (pointer, bytes, tensor). From torch's allocator, which orders its reuse on the
+    stream and gives a captured graph memory of its own."""
+    if nbytes == 0:
+        return None, 0, None
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return ws.data_ptr(), nbytes, ws
+
+
+def _rows(x, what: str):
+    """x [..., K] as [M, K] with contiguous, 16-byte aligned rows."""
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise AegistError("shape", -1, f"{what} needs a last dimension")
+    x2 = x.reshape(-1, x.shape[-1])
+    if x2.stride(1) != 1:
+        raise AegistError("layout", -1, f"{what} rows must be contiguous")
+    return x2, x2.stride(0) if x2.shape[0] > 1 else -(-x2.shape[1] // 8) * 8
+
+
+class Q4Weight:
+    """A weight matrix [N, K] in 4 bits, packed for linear_q4 (the q4 block of include/aegist_mixer.h):
+    w = code * scale + min per `group` consecutive inputs. Made by q4_quantize or q4_pack."""
+
+    __slots__ = ("data", "shape", "group")
+
+    def __init__(self, data, shape, group: int):
+        self.data, self.shape, self.group = data, tuple(shape), group
+
+    @property
+    def device(self):
+        return self.data.device
+
+
+def _q4_empty(N: int, K: int, group: int, device):
+    nbytes = lib().aegist_q4_bytes(N, K, group)
+    if nbytes == 0 and N > 0:
+        raise AegistError("q4", -1, f"no 4-bit form of [{N}, {K}] in groups of {group}: groups of 32, 64 or 128, "
+                                    "K a positive multiple of the group")
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
+def q4_quantize(weight, group: int = 64) -> Q4Weight:
+    """weight [N, K] (fp32 or bf16, rows contiguous) rounded to 4 bits: per group of `group` (32, 64, 128) inputs
+    min = fp16(smallest), scale = fp16((largest - min) / 15), code = rint((w - min) / scale) in 0..15, evaluated
+    in double. A group with a value that is not finite or beyond +-65504 dequantises to NaN."""
+    if weight.dim() != 2 or weight.stride(1) != 1:
+        raise AegistError("layout", -1, "weight must be [N, K] with contiguous rows")
+    N, K = weight.shape
+    p, dt = _p(weight), _dt(weight)
+    data = _q4_empty(N, K, group, weight.device)
+    _call_on(weight.device, "aegist_q4_quantize", p, dt, weight.stride(0) if N > 1 else K, data.data_ptr(), N, K, group)
+    return Q4Weight(data, (N, K), group)
+
+
+def q4_pack(codes, scale, mins=None) -> Q4Weight:
+    """Packs 4-bit weights of the engine's layout (q4_dequantize, hybrid.py:463-469): codes uint8 [N, K/2], two
+    to a byte with the even element in the low nibble; scale and mins fp16 [N, K/group]. Without mins the weights
+    are (code - 8) * scale."""
+    _need_contig(codes, scale, mins)
+    if codes.dtype != torch.uint8 or scale.dtype != torch.float16 or (mins is not None and mins.dtype != torch.float16):
+        raise AegistError("dtype", -3, "codes must be uint8, scale and mins fp16")
+    if codes.dim() != 2 or scale.dim() != 2 or scale.shape[0] != codes.shape[0] or scale.shape[1] == 0 or \
+            (mins is not None and mins.shape != scale.shape):
+        raise AegistError("shape", -1, "codes [N, K/2] with scale and mins [N, K/group] expected")
+    N, K = codes.shape[0], 2 * codes.shape[1]
+    group, rest = divmod(K, scale.shape[1])
+    if rest:
+        raise AegistError("shape", -1, f"{scale.shape[1]} groups do not divide K = {K}")
+    dev = _one_device(codes, scale, mins)
+    pc, ps, pm = _p(codes), _p(scale), _p(mins)
+    data = _q4_empty(N, K, group, dev)
+    _call_on(dev, "aegist_q4_pack", pc, ps, pm, data.data_ptr(), N, K, group)
+    return Q4Weight(data, (N, K), group)
+
+
+def q4_dequantize(weight: Q4Weight):
+    """The fp32 [N, K] matrix that a packed weight stands for."""
+    N, K = weight.shape
+    out = torch.empty(N, K, dtype=torch.float32, device=weight.device)
+    _call_on(weight.device, "aegist_q4_dequantize", _p(weight.data), _p(out), N, K, weight.group)
+    return out
+
+
+def linear_q4(x, weight: Q4Weight, out=None, accumulate: bool = False):
+    """out[..., n] (+)= sum_k x[..., k] weight[n, k] in fp32: linear() with a 4-bit weight.
+
+    x [..., K] fp32 or bf16 (rows contiguous, 16-byte aligned); out fp32 [..., N], contiguous (allocated if
+    None; with accumulate the product is added into it)."""
+    N, K = weight.shape
+    x2, ldx = _rows(x, "x")
+    if x2.shape[1] != K:
+        raise AegistError("shape", -1, f"weight [{N}, {K}] does not match x [..., {x2.shape[1]}]")
+    M = x2.shape[0]
+    if out is None:
+        if accumulate:
+            raise AegistError("shape", -1, "accumulate needs out")
+        out = torch.empty(*x.shape[:-1], N, dtype=torch.float32, device=x.device)
+    _need_contig(out)
+    if out.dtype != torch.float32 or out.numel() != M * N:
+        raise AegistError("shape", -1, "out must be fp32 [..., N]")
+    dev = _one_device(x2, weight.data, out)
+    px, pw, po, dt = _p(x2), _p(weight.data), _p(out), _dt(x2)
+    wp, wn, ws = _scratch(lib().aegist_linear_q4_workspace_bytes(dt, M, N, K, weight.group), dev)
+    _call_on(dev, "aegist_linear_q4", px, dt, ldx, pw, po, N, M, N, K, weight.group, int(accumulate), wp, wn)
+    return out
+
+
+class TokenLogprobs(NamedTuple):
+    """Per row: the log probability of its token, the entropy, and the most probable tokens with their log
+    probabilities (None where none were asked for)."""
+    logprob: torch.Tensor
+    entropy: torch.Tensor
+    top_ids: torch.Tensor | None
+    top_logprobs: torch.Tensor | None
+
+
+def _logprob_outputs(lead, tokens, top: int, device):
+    if tokens.dtype != torch.int32:
+        raise AegistError("dtype", -3, "tokens must be int32")
+    if tuple(tokens.shape) != tuple(lead):
+        raise AegistError("shape", -1, f"tokens {tuple(tokens.shape)} for rows {tuple(lead)}")
+    _need_contig(tokens)
+    both = torch.empty(2, *lead, dtype=torch.float32, device=device)
+    ids = torch.empty(*lead, top, dtype=torch.int32, device=device) if top > 0 else None
+    lps = torch.empty(*lead, top, dtype=torch.float32, device=device) if top > 0 else None
+    return TokenLogprobs(both[0], both[1], ids, lps)
+
+
+def token_logprobs(logits, tokens, top: int = 0) -> TokenLogprobs:
+    """Log probabilities of given tokens: logits [..., V] fp32 or bf16 (rows contiguous), tokens int32 [...].
+
+    Returns (logprob [...], entropy [...], top_ids [..., top] int32, top_logprobs [..., top]), fp32, the `top`
+    (0 to 64) most probable tokens in descending order, ties to the lower token. A negative token (padding)
+    has logprob 0, one past the vocabulary NaN. Logits of -inf have no probability; a row of nothing else has
+    logprob -inf and entropy 0, a row with NaN or +inf NaN."""
+    if logits.dim() < 1 or logits.shape[-1] == 0:
+        raise AegistError("shape", -1, "logits need a vocabulary")
+    V = logits.shape[-1]
+    x = logits.reshape(-1, V)
+    if V > 1 and x.stride(1) != 1:
+        raise AegistError("layout", -1, "logits rows must be contiguous")
+    T = x.shape[0]
+    dev = _one_device(x, tokens)
+    px, pt, dt = _p(x), _p(tokens), _dt(x)
+    r = _logprob_outputs(logits.shape[:-1], tokens, top, dev)
+    wp, wn, ws = _scratch(lib().aegist_token_logprobs_workspace_bytes(T, V, top), dev)
+    _call_on(dev, "aegist_token_logprobs", px, dt, x.stride(0) if T > 1 else V, pt, r.logprob.data_ptr(),
+             r.entropy.data_ptr(), _p(r.top_ids), _p(r.top_logprobs), T, V, top, wp, wn)
+    return r
+
+
+def head_logprobs(x, weight, tokens, top: int = 0, scale=None) -> TokenLogprobs:
+    """token_logprobs of the logits x weight^T of an output head, which are never whole in memory.
+
+    x [..., K] fp32 or bf16 (rows contiguous, 16-byte aligned); weight [V, K]: a Q4Weight, int8 with scale bf16
+    [V], or bf16 (scale None or bf16 [V]); tokens int32 [...]."""
+    V, K = weight.shape
+    q4 = isinstance(weight, Q4Weight)
+    x2, ldx = _rows(x, "x")
+    if x2.shape[1] != K:
+        raise AegistError("shape", -1, f"weight [{V}, {K}] does not match x [..., {x2.shape[1]}]")
+    w = weight.data if q4 else weight
+    if q4:
+        if scale is not None:
+            raise AegistError("shape", -1, "a 4-bit weight has its own scales")
+        wdt = Q4
+    else:
+        _need_contig(w, scale)
+        wdt = {torch.int8: I8, torch.bfloat16: BF16}.get(w.dtype)
+        if wdt is None:
+            raise AegistError("dtype", -3, "weight must be 4-bit, int8 or bf16")
+        if scale is not None and (scale.dtype != torch.bfloat16 or scale.numel() != V):
+            raise AegistError("shape", -1, "scale must be bf16 [V]")
+    T, group = x2.shape[0], weight.group if q4 else 0
+    dev = _one_device(x2, w, tokens, scale)
+    px, pw, pt, ps, dt = _p(x2), _p(w), _p(tokens), _p(scale), _dt(x2)
+    r = _logprob_outputs(x.shape[:-1], tokens, top, dev)
+    wp, wn, ws = _scratch(lib().aegist_head_logprobs_workspace_bytes(dt, wdt, T, V, K, group, top), dev)
+    _call_on(dev, "aegist_head_logprobs", px, dt, ldx, pw, wdt, ps, pt, r.logprob.data_ptr(), r.entropy.data_ptr(),
+             _p(r.top_ids), _p(r.top_logprobs), T, V, K, group, top, wp, wn)
+    return r
 
 
 # --- mixture of experts (MoE, aegist/hybrid.py:631-652; HybridEngine::moe, hybrid.rs:863-955) -----

@@ -1,0 +1,36 @@
+// Layout of a 4-bit weight matrix as the projections read it (Q4 weight), and the host-side launchers of
+// q4.hip that other files call.
+//
+// A weight [N, K] in groups of G = 32, 64 or 128 consecutive k: w[n, k] = code * scale[n, k / G] + min[n, k / G],
+// codes 0..15, scale and min in fp16. One block of memory with three sections:
+//   codes   [N / 16][K / 128][64 lanes][16 bytes]: 1 KB holds 16 rows x 128 k in the order of the matrix
+//           operand of v_mfma_f32_16x16x32_f16, so that a wave reads 1 KB in one contiguous piece and needs no
+//           exchange between lanes. Lane 16 q + r has row r; its dword j has the 8 codes k = 32 j + 8 q + e,
+//           element e at nibble e / 2 + 4 (e % 2): the two codes of a dword's halves, masked out in place, are
+//           two fp16 subnormals.
+//   scale   [N / 16][K / G / 8][16 rows][8 groups] fp16: 16 bytes are 8 consecutive groups of a row
+//   min     the same
+// Rows, k and groups past the matrix are zeros.
+#pragma once
+
+#include "common.h"
+
+namespace aegist {
+
+struct Q4Dims {
+    int N, K, G;
+    __host__ __device__ int tiles() const { return (N + 15) / 16; }
+    __host__ __device__ int chunks() const { return (K + 127) / 128; }
+    __host__ __device__ int blocks8() const { return (K / G + 7) / 8; }
+    __host__ __device__ size_t code_bytes() const { return (size_t)tiles() * chunks() * 1024; }
+    __host__ __device__ size_t scale_bytes() const { return (size_t)tiles() * blocks8() * 256; }
+    __host__ __device__ size_t bytes() const { return code_bytes() + 2 * scale_bytes(); }
+};
+
+// AEGIST_OK, or the error of sizes that no Q4 weight has.
+int check_q4(const char* who, int N, int K, int G);
+size_t linear_q4_workspace(int x_dtype, int M, int N, int K, int G);
+int launch_linear_q4(const void* X, int x_dtype, long long ldx, const void* W, float* Y, long long ldy, int M, int N,
+                     int K, int G, int accumulate, void* ws, size_t ws_bytes, hipStream_t st);
+
+}  // namespace aegist

@@ -1,0 +1,312 @@
+// Projections with 4-bit weights, and the making of those weights.
+//
+//   Y[m, n] (+)= sum_k X[m, k] (code[n, k] * scale[n, k / G] + min[n, k / G])
+#include "q4.h"
+
+#include <algorithm>
+
+using namespace aegist;
+
+namespace {
+
+typedef uint32_t u4v __attribute__((ext_vector_type(4)));
+
+// nibble of element e (0..7) in a dword of codes
+__host__ __device__ constexpr int q4_shift(int e) { return 4 * (e / 2 + 4 * (e % 2)); }
+
+struct Q4Ptr {
+    const unsigned char* codes;
+    const _Float16 *scale, *mins;
+};
+__host__ __device__ inline Q4Ptr q4_ptr(const void* w, const Q4Dims& d) {
+    const unsigned char* p = (const unsigned char*)w;
+    return {p, (const _Float16*)(p + d.code_bytes()), (const _Float16*)(p + d.code_bytes() + d.scale_bytes())};
+}
+// index of (row n, group g) in the scale and min sections
+__device__ __forceinline__ size_t q4_group(const Q4Dims& d, int n, int g) {
+    return ((size_t)(n / 16) * d.blocks8() + g / 8) * 128 + (n % 16) * 8 + g % 8;
+}
+
+// One wave per 16 rows x 128 k. Lane 16 q + r holds the runs k = 32 j + 8 q .. + 7 of row r, so a group's extremes
+// are its own values' and, over the four q, two exchanges'. The code is decided in doubles: w - min and its
+// quotient by the scale next to a half would round either way in fp32.
+template <typename TW>
+__global__ void __launch_bounds__(256) q4_quantize_kernel(const TW* __restrict__ W, long long ldw, unsigned char* out,
+                                                          const Q4Dims d) {
+    const int lane = threadIdx.x % WAVE, r = lane % 16, q = lane / 16;
+    const int c = blockIdx.x * 4 + threadIdx.x / WAVE, nt = blockIdx.y + blockIdx.z * 65535;
+    if (c >= d.chunks() || nt >= d.tiles()) return;
+    const int n = nt * 16 + r;
+    const bool row = n < d.N;
+    float w[4][8];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const int k = c * 128 + 32 * j + 8 * q;
+#pragma unroll
+        for (int e = 0; e < 8; e++) w[j][e] = row && k < d.K ? Act<TW>::ld(W, (size_t)n * ldw + k + e) : 0.f;
+    }
+    float lo[4], hi[4];
+    bool bad[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        lo[j] = hi[j] = w[j][0];
+        bad[j] = false;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            lo[j] = fminf(lo[j], w[j][e]);
+            hi[j] = fmaxf(hi[j], w[j][e]);
+            bad[j] |= !(fabsf(w[j][e]) <= 65504.f);
+        }
+    }
+    const int span = d.G / 32;  // runs of 32 k per group
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+#pragma unroll
+        for (int o = 16; o < 64; o *= 2) {
+            lo[j] = fminf(lo[j], __shfl_xor(lo[j], o, WAVE));
+            hi[j] = fmaxf(hi[j], __shfl_xor(hi[j], o, WAVE));
+            bad[j] |= __shfl_xor((int)bad[j], o, WAVE) != 0;
+        }
+    }
+#pragma unroll
+    for (int s = 1; s < 4; s *= 2)
+        if (s < span) {
+            float l2[4], h2[4];
+            bool b2[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                l2[j] = fminf(lo[j], lo[j ^ s]);
+                h2[j] = fmaxf(hi[j], hi[j ^ s]);
+                b2[j] = bad[j] | bad[j ^ s];
+            }
+#pragma unroll
+            for (int j = 0; j < 4; j++) lo[j] = l2[j], hi[j] = h2[j], bad[j] = b2[j];
+        }
+    u4v codes;
+    _Float16* scale = (_Float16*)(out + d.code_bytes());
+    _Float16* mins = (_Float16*)(out + d.code_bytes() + d.scale_bytes());
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const _Float16 mn = bad[j] ? (_Float16)__builtin_nanf("") : (_Float16)lo[j];
+        const double range = ((double)hi[j] - (double)mn) / 15.0;
+        const _Float16 sc = range > 0.0 ? (_Float16)range : (_Float16)0.f;
+        uint32_t p = 0;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const double v = sc > (_Float16)0.f ? rint(((double)w[j][e] - (double)mn) / (double)sc) : 0.0;
+            p |= (uint32_t)(int)fmin(fmax(v, 0.0), 15.0) << q4_shift(e);
+        }
+        const int k = c * 128 + 32 * j;
+        codes[j] = row && k < d.K ? p : 0;
+        if (q == 0 && row && k < d.K && k % d.G == 0) {
+            scale[q4_group(d, n, k / d.G)] = sc;
+            mins[q4_group(d, n, k / d.G)] = mn;
+        }
+    }
+    ((u4v*)out)[((size_t)nt * d.chunks() + c) * 64 + lane] = codes;
+}
+
+// Codes of the engine's layout (two to a byte, the even element low) into the operand's order, one wave per 16
+// rows x 128 k. min = -8 scale where none are given: (code - 8) * scale.
+__global__ void __launch_bounds__(256) q4_pack_kernel(const unsigned char* __restrict__ codes, unsigned char* out,
+                                                      const Q4Dims d) {
+    const int lane = threadIdx.x % WAVE, r = lane % 16, q = lane / 16;
+    const int c = blockIdx.x * 4 + threadIdx.x / WAVE, nt = blockIdx.y + blockIdx.z * 65535;
+    if (c >= d.chunks() || nt >= d.tiles()) return;
+    const int n = nt * 16 + r;
+    u4v v;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const int k = c * 128 + 32 * j + 8 * q;
+        uint32_t s = 0, p = 0;
+        if (n < d.N && k < d.K) s = *(const uint32_t*)(codes + ((size_t)n * d.K + k) / 2);
+#pragma unroll
+        for (int e = 0; e < 8; e++) p |= (s >> (4 * e) & 15) << q4_shift(e);
+        v[j] = p;
+    }
+    ((u4v*)out)[((size_t)nt * d.chunks() + c) * 64 + lane] = v;
+}
+
+// Scales and minima from rows [N, K / G], or (src null) zeros in the places that no group has.
+__global__ void __launch_bounds__(256) q4_pack_groups_kernel(const _Float16* __restrict__ scale,
+                                                             const _Float16* __restrict__ mins, unsigned char* out,
+                                                             const Q4Dims d, bool fill) {
+    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x, all = d.scale_bytes() / 2;
+    if (i >= all) return;
+    const int g = (int)(i / 128 % d.blocks8()) * 8 + i % 8, n = (int)(i / 128 / d.blocks8()) * 16 + i / 8 % 16;
+    const bool in = n < d.N && g < d.K / d.G;
+    if (!fill && in) return;
+    _Float16 s = 0, m = 0;
+    if (in) {
+        s = scale[(size_t)n * (d.K / d.G) + g];
+        m = mins ? mins[(size_t)n * (d.K / d.G) + g] : (_Float16)(-8.f * (float)s);
+    }
+    ((_Float16*)(out + d.code_bytes()))[i] = s;
+    ((_Float16*)(out + d.code_bytes() + d.scale_bytes()))[i] = m;
+}
+
+__global__ void __launch_bounds__(256) q4_dequantize_kernel(const unsigned char* __restrict__ W, float* __restrict__ out,
+                                                            const Q4Dims d) {
+    const int lane = threadIdx.x % WAVE, r = lane % 16, q = lane / 16;
+    const int c = blockIdx.x * 4 + threadIdx.x / WAVE, nt = blockIdx.y + blockIdx.z * 65535;
+    if (c >= d.chunks() || nt >= d.tiles()) return;
+    const int n = nt * 16 + r;
+    if (n >= d.N) return;
+    const Q4Ptr w = q4_ptr(W, d);
+    const u4v v = ((const u4v*)w.codes)[((size_t)nt * d.chunks() + c) * 64 + lane];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const int k = c * 128 + 32 * j + 8 * q;
+        if (k >= d.K) continue;
+        const size_t gi = q4_group(d, n, k / d.G);
+        const float s = (float)w.scale[gi], m = (float)w.mins[gi];
+        float f[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) f[e] = fmaf((float)(v[j] >> q4_shift(e) & 15), s, m);
+        float4* o = (float4*)(out + (size_t)n * d.K + k);
+        o[0] = float4{f[0], f[1], f[2], f[3]};
+        o[1] = float4{f[4], f[5], f[6], f[7]};
+    }
+}
+
+// 16 rows of W x 16 rows of X per workgroup, a product per thread.
+template <typename TX>
+__global__ void __launch_bounds__(256) linear_q4_kernel(const TX* __restrict__ X, long long ldx,
+                                                        const unsigned char* __restrict__ W, float* __restrict__ Y,
+                                                        long long ldy, int M, const Q4Dims d, int accumulate) {
+    const int r = threadIdx.x % 16, n = blockIdx.x * 16 + r;
+    const Q4Ptr w = q4_ptr(W, d);
+    for (int m = blockIdx.y * 16 + threadIdx.x / 16; m < M; m += gridDim.y * 16) {
+        if (n >= d.N) return;
+        const TX* x = X + (size_t)m * ldx;
+        float acc = 0.f;
+        for (int g = 0; g < d.K / d.G; g++) {
+            float p = 0.f, s = 0.f;
+            for (int k = g * d.G; k < (g + 1) * d.G; k += 8) {
+                const int lane = k % 32 / 8 * 16 + r;
+                const uint32_t v = ((const uint32_t*)w.codes)[(((size_t)blockIdx.x * d.chunks() + k / 128) * 64 + lane) * 4 +
+                                                              k % 128 / 32];
+                for (int e = 0; e < 8; e++) {
+                    const float f = Act<TX>::ld(x, k + e);
+                    p = fmaf((float)(v >> q4_shift(e) & 15), f, p);
+                    s += f;
+                }
+            }
+            const size_t gi = q4_group(d, n, g);
+            acc = fmaf(p, (float)w.scale[gi], fmaf(s, (float)w.mins[gi], acc));
+        }
+        float* y = Y + (size_t)m * ldy + n;
+        *y = accumulate ? *y + acc : acc;
+    }
+}
+
+// grid over (chunks / 4, tiles): tiles past 65535 go on along z
+dim3 q4_grid(const Q4Dims& d) {
+    return dim3((d.chunks() + 3) / 4, std::min(d.tiles(), 65535), (d.tiles() + 65534) / 65535);
+}
+
+}  // namespace
+
+namespace aegist {
+
+int check_q4(const char* who, int N, int K, int G) {
+    const std::string w(who);
+    if (G != 32 && G != 64 && G != 128) return fail(AEGIST_ERR_SHAPE, w + ": groups of 32, 64 or 128 values");
+    if (N < 0 || K <= 0 || K % G) return fail(AEGIST_ERR_SHAPE, w + ": K must be a positive multiple of the group");
+    return 0;
+}
+
+size_t linear_q4_workspace(int, int, int, int, int) { return 0; }
+
+int launch_linear_q4(const void* X, int x_dtype, long long ldx, const void* W, float* Y, long long ldy, int M, int N,
+                     int K, int G, int accumulate, void*, size_t, hipStream_t st) {
+    int rc = check_q4("linear_q4", N, K, G);
+    if (rc) return rc;
+    if (x_dtype != AEGIST_F32 && x_dtype != AEGIST_BF16)
+        return fail(AEGIST_ERR_DTYPE, "linear_q4: X must be AEGIST_F32 or AEGIST_BF16");
+    if (M < 0) return fail(AEGIST_ERR_SHAPE, "linear_q4: negative size");
+    if (M == 0 || N == 0) return 0;
+    if (!X || !W || !Y) return fail(AEGIST_ERR_SHAPE, "linear_q4: null operand");
+    const int xs = x_dtype == AEGIST_F32 ? 4 : 2;
+    if (ldx < K || (ldx * xs) % 16 || (uintptr_t)X % 16)
+        return fail(AEGIST_ERR_SHAPE, "linear_q4: X needs 16-byte aligned rows (ldx >= K)");
+    if (ldy < N) return fail(AEGIST_ERR_SHAPE, "linear_q4: ldy < N");
+    if ((uintptr_t)W % 16) return fail(AEGIST_ERR_SHAPE, "linear_q4: W must be 16-byte aligned");
+    const Q4Dims d{N, K, G};
+    const dim3 grid(d.tiles(), std::min((M + 15) / 16, 65535));
+    if (x_dtype == AEGIST_F32)
+        linear_q4_kernel<float><<<grid, 256, 0, st>>>((const float*)X, ldx, (const unsigned char*)W, Y, ldy, M, d, accumulate);
+    else
+        linear_q4_kernel<uint16_t><<<grid, 256, 0, st>>>((const uint16_t*)X, ldx, (const unsigned char*)W, Y, ldy, M, d, accumulate);
+    return after_launch("linear_q4");
+}
+
+}  // namespace aegist
+
+extern "C" size_t aegist_q4_bytes(int N, int K, int group) {
+    if (check_q4("q4_bytes", N, K, group)) return 0;
+    return Q4Dims{N, K, group}.bytes();
+}
+
+extern "C" int aegist_q4_quantize(const void* W, int w_dtype, long long ldw, void* q4, int N, int K, int group,
+                                  void* stream) {
+    int rc = check_q4("q4_quantize", N, K, group);
+    if (rc) return rc;
+    if (w_dtype != AEGIST_F32 && w_dtype != AEGIST_BF16)
+        return fail(AEGIST_ERR_DTYPE, "q4_quantize: W must be AEGIST_F32 or AEGIST_BF16");
+    if (N == 0) return 0;
+    if (!W || !q4 || (uintptr_t)q4 % 16) return fail(AEGIST_ERR_SHAPE, "q4_quantize: null operand, or q4 not 16-byte aligned");
+    const int es = w_dtype == AEGIST_F32 ? 4 : 2;
+    if (ldw < K || (ldw * es) % 16 || (uintptr_t)W % 16)
+        return fail(AEGIST_ERR_SHAPE, "q4_quantize: W needs 16-byte aligned rows (ldw >= K)");
+    const Q4Dims d{N, K, group};
+    const hipStream_t st = AEG_STREAM(stream);
+    if (N % 16 || K / group % 8) {
+        q4_pack_groups_kernel<<<(unsigned)((d.scale_bytes() / 2 + 255) / 256), 256, 0, st>>>(nullptr, nullptr,
+                                                                                             (unsigned char*)q4, d, false);
+        if ((rc = after_launch("q4_quantize"))) return rc;
+    }
+    if (w_dtype == AEGIST_F32)
+        q4_quantize_kernel<float><<<q4_grid(d), 256, 0, st>>>((const float*)W, ldw, (unsigned char*)q4, d);
+    else
+        q4_quantize_kernel<uint16_t><<<q4_grid(d), 256, 0, st>>>((const uint16_t*)W, ldw, (unsigned char*)q4, d);
+    return after_launch("q4_quantize");
+}
+
+extern "C" int aegist_q4_pack(const void* codes, const uint16_t* scale, const uint16_t* mins, void* q4, int N, int K,
+                              int group, void* stream) {
+    int rc = check_q4("q4_pack", N, K, group);
+    if (rc) return rc;
+    if (N == 0) return 0;
+    if (!codes || !scale || !q4 || (uintptr_t)q4 % 16 || (uintptr_t)codes % 4)
+        return fail(AEGIST_ERR_SHAPE, "q4_pack: null operand, q4 not 16-byte or codes not 4-byte aligned");
+    const Q4Dims d{N, K, group};
+    const hipStream_t st = AEG_STREAM(stream);
+    q4_pack_kernel<<<q4_grid(d), 256, 0, st>>>((const unsigned char*)codes, (unsigned char*)q4, d);
+    if ((rc = after_launch("q4_pack"))) return rc;
+    q4_pack_groups_kernel<<<(unsigned)((d.scale_bytes() / 2 + 255) / 256), 256, 0, st>>>(
+        (const _Float16*)scale, (const _Float16*)mins, (unsigned char*)q4, d, true);
+    return after_launch("q4_pack");
+}
+
+extern "C" int aegist_q4_dequantize(const void* q4, float* out, int N, int K, int group, void* stream) {
+    int rc = check_q4("q4_dequantize", N, K, group);
+    if (rc) return rc;
+    if (N == 0) return 0;
+    if (!q4 || !out || (uintptr_t)q4 % 16 || (uintptr_t)out % 16)
+        return fail(AEGIST_ERR_SHAPE, "q4_dequantize: null operand, or one not 16-byte aligned");
+    const Q4Dims d{N, K, group};
+    q4_dequantize_kernel<<<q4_grid(d), 256, 0, AEG_STREAM(stream)>>>((const unsigned char*)q4, out, d);
+    return after_launch("q4_dequantize");
+}
+
+extern "C" size_t aegist_linear_q4_workspace_bytes(int x_dtype, int M, int N, int K, int group) {
+    if (M < 0 || check_q4("linear_q4_workspace", N, K, group)) return 0;
+    return linear_q4_workspace(x_dtype, M, N, K, group);
+}
+
+extern "C" int aegist_linear_q4(const void* X, int x_dtype, long long ldx, const void* q4, float* Y, long long ldy,
+                                int M, int N, int K, int group, int accumulate, void* ws, size_t ws_bytes,
+                                void* stream) {
+    return launch_linear_q4(X, x_dtype, ldx, q4, Y, ldy, M, N, K, group, accumulate, ws, ws_bytes, AEG_STREAM(stream));
+}

@@ -40,7 +40,7 @@
 extern "C" {
 #endif
 
-enum { AEGIST_F32 = 0, AEGIST_BF16 = 1, AEGIST_I8 = 2 /* weights only */ };
+enum { AEGIST_F32 = 0, AEGIST_BF16 = 1, AEGIST_I8 = 2 /* weights only */, AEGIST_Q4 = 3 /* packed weights only */ };
 
 enum {
     AEGIST_OK = 0,
@@ -406,6 +406,62 @@ int aegist_moe_experts(const float* h, const unsigned long long* eptr, const int
 int aegist_shared_gate_add(float* x, const float* y, const float* h, const uint16_t* wg, int T, int D, void* stream);
 /* silu_mul, aegist.cu:174-178: out = silu(g) * u over n elements (the shared expert's SwiGLU) */
 int aegist_silu_mul(const float* g, const float* u, float* out, long long n, void* stream);
+
+/* -------------------------------------------------------------------------------------
+ * Projections with 4-bit weights. A weight matrix [N, K] in groups of `group` (32, 64 or 128)
+ * consecutive k, w = code * scale + min, codes 0..15, scale and min fp16: the format of the
+ * experts above, packed into one block of device memory ("q4", 16-byte aligned,
+ * aegist_q4_bytes(N, K, group) bytes) in the order in which the matrix cores take it. K is a
+ * positive multiple of the group. No counterpart in the reference, whose projections are int8.
+ * ------------------------------------------------------------------------------------- */
+/* Bytes of a packed weight; 0 for sizes that none has. */
+size_t aegist_q4_bytes(int N, int K, int group);
+/* Rounds W [N, K] (AEGIST_F32 | AEGIST_BF16, row stride ldw elements, rows 16-byte aligned) to
+ * 4 bits: per group min = fp16(smallest), scale = fp16((largest - min) / 15) (0 if negative),
+ * code = (w - min) / scale rounded to the nearest, ties to even, kept in 0..15 (0 where the scale is
+ * 0), all evaluated in double. A group with a value that is not finite or beyond +-65504 gets
+ * a NaN minimum. */
+int aegist_q4_quantize(const void* W, int w_dtype, long long ldw, void* q4, int N, int K, int group, void* stream);
+/* Packs codes [N, K / 2] (two to a byte, the even element in the low nibble; 4-byte aligned) with
+ * scale and mins [N, K / group] fp16, as the sections of an expert row hold them. mins NULL: the
+ * symmetric form (code - 8) * scale, |8 scale| <= 65504. */
+int aegist_q4_pack(const void* codes, const uint16_t* scale, const uint16_t* mins, void* q4, int N, int K, int group,
+                   void* stream);
+/* out [N, K] fp32 (16-byte aligned) = code * scale + min. */
+int aegist_q4_dequantize(const void* q4, float* out, int N, int K, int group, void* stream);
+/* Y[m, n] (+)= sum_k X[m, k] w[n, k], Y fp32 with row stride ldy; X AEGIST_F32 | AEGIST_BF16 with row
+ * stride ldx elements, rows 16-byte aligned. Deterministic. Every value of X counts with 22 bits
+ * below the largest of its row; a row of X with an infinity or NaN has no finite output. Needs
+ * aegist_linear_q4_workspace_bytes(x_dtype, M, N, K, group) bytes (256-byte aligned; 0 at few
+ * rows). */
+size_t aegist_linear_q4_workspace_bytes(int x_dtype, int M, int N, int K, int group);
+int aegist_linear_q4(const void* X, int x_dtype, long long ldx, const void* q4, float* Y, long long ldy, int M, int N,
+                     int K, int group, int accumulate, void* ws, size_t ws_bytes, void* stream);
+
+/* -------------------------------------------------------------------------------------
+ * Log probabilities of given tokens under logits [T, V], with the entropy of each row and its
+ * `top` (0 to 64, at most V) most probable tokens. No counterpart in the reference, whose engine
+ * copies the logits to the host.
+ *   tokens       [T] int32. A negative one has logprob 0 (no token there), one past the vocabulary NaN
+ *   logprob      [T] fp32 = x[token] - ln sum e^x
+ *   entropy      [T] fp32 = - sum p ln p
+ *   top_ids      [T, top] int32, top_logprobs [T, top] fp32: descending, ties to the lower token
+ *                (both may be NULL if top is 0)
+ * Logits of -inf have no probability. A row of nothing else has logprob -inf for every token and
+ * entropy 0. A row with a NaN or +inf has NaN for all of them (top_ids: NaN first). Deterministic.
+ * ------------------------------------------------------------------------------------- */
+/* logits AEGIST_F32 | AEGIST_BF16, row stride ld elements, aligned to the element. */
+size_t aegist_token_logprobs_workspace_bytes(int T, int V, int top);
+int aegist_token_logprobs(const void* logits, int dtype, long long ld, const int* tokens, float* logprob,
+                          float* entropy, int* top_ids, float* top_logprobs, int T, int V, int top, void* ws,
+                          size_t ws_bytes, void* stream);
+/* The same for the logits X W^T of an output head W [V, K]: AEGIST_I8 with scale, AEGIST_BF16 (scale NULL
+ * or per row; group is ignored) as in aegist_linear, or AEGIST_Q4 (scale is ignored). The logits are made
+ * in parts in the workspace and are never whole. */
+size_t aegist_head_logprobs_workspace_bytes(int x_dtype, int w_dtype, int T, int V, int K, int group, int top);
+int aegist_head_logprobs(const void* X, int x_dtype, long long ldx, const void* W, int w_dtype, const uint16_t* scale,
+                         const int* tokens, float* logprob, float* entropy, int* top_ids, float* top_logprobs, int T,
+                         int V, int K, int group, int top, void* ws, size_t ws_bytes, void* stream);
 
 #ifdef __cplusplus
 }

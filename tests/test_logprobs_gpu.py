@@ -1,0 +1,221 @@
+"""Log probabilities of given tokens, entropy and alternatives: against log-softmax in 64 bits."""
+import math
+
+import pytest
+import torch
+
+from aegist_mixer import ops
+from oracle import mixer_ref as R
+
+pytestmark = pytest.mark.gpu
+INF = float("inf")
+
+
+def _ref(x, tokens, top):
+    """fp64 on the CPU; rows that nothing is left of by their rule."""
+    x = x.double().cpu()
+    m = x.amax(1, keepdim=True)
+    d = x - torch.where(torch.isinf(m), 0.0, m)  # (a sum of 3e38 and ln V is 3e38 in doubles too)
+    lse = torch.logsumexp(d, 1, keepdim=True)
+    lp = torch.where(torch.isinf(lse), -INF, d - lse)
+    ent = -(lp.exp() * lp).nan_to_num(nan=0.0).sum(1)
+    ent = torch.where(torch.isinf(lse[:, 0]), 0.0, ent)
+    ids = torch.sort(x, dim=1, descending=True, stable=True).indices[:, :top]
+    return lp.gather(1, tokens.long().cpu().unsqueeze(1))[:, 0], ent, ids, lp.gather(1, ids), x
+
+
+def _check(x, tokens, top, got):
+    """Tolerances: x - m is exact to 2^-24 |x - m|, e^(x - m) is within |x - m| 2^-24 and 2 units of itself, where terms
+    with |x - m| > 30 count for nothing; the sum of V terms in chains of at most 2^12 and a tree, each rounding
+    2^-24 of the sum: at worst (30 + 2 + 2^12) 2^-24, at random far less: 2^-16 stands for both. The
+    entropy's terms carry up to |x - m| <= 30 more."""
+    lp, ent, ids, lps, xd = _ref(x, tokens, top)
+    span = torch.where(torch.isfinite(lp), lp.abs(), 0.0) + 1
+    fin = torch.isfinite(lp)
+    a = got.logprob.cpu().double()
+    assert torch.equal(torch.isfinite(a), fin) and torch.equal(a[~fin], lp[~fin])
+    assert ((a - lp).abs()[fin] <= (2.0 ** -16 + span * 2.0 ** -22)[fin]).all()
+    assert ((got.entropy.cpu().double() - ent).abs() <= 30 * 2.0 ** -16).all()
+    if not top:
+        assert got.top_ids is None and got.top_logprobs is None
+        return
+    assert torch.equal(got.top_ids.cpu().long(), ids)
+    b = got.top_logprobs.cpu().double()
+    fin = torch.isfinite(lps)
+    assert torch.equal(b[~fin], lps[~fin])
+    assert ((b - lps).abs()[fin] <= (2.0 ** -16 + (lps.abs() + 1) * 2.0 ** -22)[fin]).all()
+
+
+def _case(T, V, dtype, seed=0, std=3.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(T, V, generator=g) * std).to(dtype), torch.randint(0, V, (T,), generator=g, dtype=torch.int32)
+
+
+@pytest.mark.parametrize("T", [1, 2, 3, 61, 300])
+@pytest.mark.parametrize("V", [1, 2, 63, 64, 65, 1000, 4099, 20000])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_token_logprobs(dev, T, V, dtype):
+    x, tok = _case(T, V, dtype, T + V)
+    for top in sorted({0, 1, min(5, V), min(64, V)}):
+        _check(x, tok, top, ops.token_logprobs(x.to(dev), tok.to(dev), top))
+
+
+@pytest.mark.parametrize("T,V,top", [(1, 131072, 20), (1, 262147, 64), (7, 100003, 5), (130, 100003, 3), (1, 1_000_003, 10)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_token_logprobs_large(dev, T, V, top, dtype):
+    x, tok = _case(T, V, dtype, T + V)
+    _check(x, tok, top, ops.token_logprobs(x.to(dev), tok.to(dev), top))
+
+
+@pytest.mark.parametrize("V", [5, 300, 9000, 70001])
+@pytest.mark.parametrize("T", [1, 9, 300])
+def test_ties_order_and_extremes(dev, T, V):
+    """Rows that selection finds hard: all alike, ascending, descending, few distinct values, one peak, -0 beside +0."""
+    g = torch.Generator().manual_seed(1)
+    top = min(V, 64)
+    rows = [torch.zeros(V), torch.arange(V) * 1e-3, -torch.arange(V) * 1e-3, torch.randint(0, 3, (V,), generator=g).float(),
+            torch.where(torch.arange(V) == V - 1, 50.0, 0.0), torch.where(torch.arange(V) % 2 == 0, -0.0, 0.0),
+            (torch.arange(V) % 256) * 0.01, (torch.arange(V) // 64) * -0.01, torch.full((V,), -3e38)]
+    x = torch.stack([rows[t % len(rows)] for t in range(T)]) if T > 1 else rows[3].unsqueeze(0)
+    tok = torch.randint(0, V, (T,), generator=g, dtype=torch.int32)
+    _check(x, tok, top, ops.token_logprobs(x.to(dev), tok.to(dev), top))
+    xb = x.bfloat16()
+    _check(xb, tok, top, ops.token_logprobs(xb.to(dev), tok.to(dev), top))
+
+
+@pytest.mark.parametrize("V", [7, 500, 40000])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_masked_rows(dev, V, dtype):
+    """-inf in most places, in all but one, in all; the token itself ruled out; masks of the type's lowest value."""
+    T, top = 12, min(V, 20)
+    x, tok = _case(T, V, dtype, V)
+    g = torch.Generator().manual_seed(2)
+    x[:6].masked_fill_(torch.rand(6, V, generator=g) < 0.95, -INF)
+    x[6], x[7] = -INF, -INF
+    x[7, V - 1] = 1.0
+    x[8, int(tok[8])] = -INF
+    x[9, : V - 2] = torch.finfo(dtype).min
+    x[10] = torch.finfo(dtype).min
+    x[11] = torch.finfo(dtype).max
+    _check(x, tok, top, ops.token_logprobs(x.to(dev), tok.to(dev), top))
+    r = ops.token_logprobs(x.to(dev), tok.to(dev), top)
+    assert r.logprob[6] == -INF and r.entropy[6] == 0 and r.top_ids[6].tolist() == list(range(top))
+    assert r.entropy[7] == 0 and r.top_logprobs[7, 0] == 0
+
+
+@pytest.mark.parametrize("V", [70, 30000])
+@pytest.mark.parametrize("T", [5, 400])
+def test_nan_infinity_and_other_tokens(dev, T, V):
+    x, tok = _case(T, V, torch.float32, 3)
+    x[0, 3], x[1, V - 1], x[2, 0] = float("nan"), INF, float("nan")
+    x[2, 1:] = -INF
+    tok[3], tok[4] = -1, V
+    r = ops.token_logprobs(x.to(dev), tok.to(dev), 4)
+    for t in range(3):
+        assert all(torch.isnan(v[t]).all() for v in (r.logprob, r.entropy, r.top_logprobs))
+    assert r.top_ids[0, 0] == 3 and r.top_ids[1, 0] == V - 1 and r.top_ids[2].tolist() == [0, 1, 2, 3]
+    assert r.logprob[3] == 0 and torch.isnan(r.logprob[4])
+    assert torch.isfinite(r.entropy[3:]).all() and torch.isfinite(r.top_logprobs[3:]).all()
+    keep = tok.clone()
+    keep[3:5] = 0
+    _check(x[3:], keep[3:], 4, ops.token_logprobs(x[3:].to(dev), keep[3:].to(dev), 4))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T", [4, 300])
+def test_strides_and_odd_places(dev, T, dtype):
+    """Rows of a wider matrix, starting at any element."""
+    wide, tok = _case(T, 5000, dtype, 4)
+    for a, b in ((0, 4999), (1, 4500), (3, 1030), (7, 4097)):
+        x = wide.to(dev)[:, a:b]
+        t = (tok % (b - a)).to(dev)
+        _check(wide[:, a:b], t.cpu(), 6, ops.token_logprobs(x, t, 6))
+    lead = ops.token_logprobs(wide.to(dev).view(2, T // 2, 5000), tok.to(dev).view(2, T // 2), 3)
+    flat = ops.token_logprobs(wide.to(dev), tok.to(dev), 3)
+    assert lead.top_ids.shape == (2, T // 2, 3) and all(torch.equal(a.flatten(), b.flatten()) for a, b in zip(lead, flat))
+
+
+def test_no_rows(dev):
+    r = ops.token_logprobs(torch.empty(0, 9, device=dev), torch.empty(0, dtype=torch.int32, device=dev), 3)
+    assert r.logprob.shape == (0,) and r.top_ids.shape == (0, 3)
+
+
+def _head(kind, V, K, seed, dev):
+    """(weight argument, scale argument, fp64 matrix)"""
+    g = torch.Generator().manual_seed(seed)
+    if kind == "q4":
+        codes = torch.randint(0, 256, (V, K // 2), generator=g, dtype=torch.uint8)
+        sc = (0.007 * (0.5 + torch.rand(V, K // 64, generator=g))).half()
+        mn = (-7.5 * sc.float()).half()
+        return ops.q4_pack(codes.to(dev), sc.to(dev), mn.to(dev)), None, R.q4_dequantize(codes, sc, mn, 64)
+    w = torch.randn(V, K, generator=g) * 0.03
+    if kind == "int8":
+        q, s = R.qlinear_quantize(w)
+        return q.to(dev), s.to(dev), q.double() * s.double().unsqueeze(1)
+    return w.bfloat16().to(dev), None, w.bfloat16().double()
+
+
+@pytest.mark.parametrize("kind", ["q4", "bf16", "int8"])
+@pytest.mark.parametrize("T,V,K,top", [(1, 1000, 64, 5), (3, 5003, 128, 3), (17, 32768, 256, 1), (90, 4100, 192, 2), (700, 9001, 128, 1)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_head_logprobs(dev, kind, T, V, K, top, dtype):
+    """Against fp64 logits. A logit is off by at most (2^-16 (fp32 rows of int8 and bf16 weights count with 16 bits) +
+    K 2^-24) sum |x w|; ids are compared where the logits of the list stand further apart than that."""
+    w, s, wd = _head(kind, V, K, V + K, dev)
+    g = torch.Generator().manual_seed(T)
+    x = torch.randn(T, K, generator=g).to(dtype)
+    tok = torch.randint(0, V, (T,), generator=g, dtype=torch.int32)
+    r = ops.head_logprobs(x.to(dev), w, tok.to(dev), top, scale=s)
+    logits = x.double() @ wd.t()
+    # (q4: the minimum's and the codes' terms are summed apart, 16 scales at most where the weight is under 8.5)
+    off = ((2.0 ** -16 + K * 2.0 ** -24) * 2 * (x.double().abs() @ wd.abs().t())).amax(1)
+    lp, ent, ids, lps, _ = _ref(logits, tok, min(top + 1, V))
+    assert ((r.logprob.cpu().double() - lp).abs() <= 2 * off + 2.0 ** -15).all()
+    assert ((r.entropy.cpu().double() - ent).abs() <= 40 * off + 30 * 2.0 ** -16).all()
+    gap = (lps[:, :-1] - lps[:, 1:]) > 2 * off.unsqueeze(1)
+    sure = gap & torch.cat([torch.ones(T, 1, dtype=torch.bool), gap[:, :-1]], 1)
+    assert sure.float().mean() > 0.5
+    assert (r.top_ids.cpu().long() == ids[:, :top])[sure].all()
+    assert ((r.top_logprobs.cpu().double() - lps[:, :top]).abs() <= 2 * off.unsqueeze(1) + 2.0 ** -15).all()
+
+
+@pytest.mark.parametrize("T", [1, 20, 300])
+def test_quantize_project_score_together(dev, T):
+    """A head quantised, multiplied and scored: the head's answers are those of the logits that linear_q4 makes of
+    the same rows, whichever way the vocabulary is cut."""
+    V, K = 20011, 256
+    w4 = ops.q4_quantize(0.05 * torch.randn(V, K, device=dev), 32)
+    x = torch.randn(T, K, device=dev)
+    tok = torch.randint(0, V, (T,), device=dev, dtype=torch.int32)
+    a = ops.head_logprobs(x, w4, tok, 8)
+    logits = ops.linear_q4(x, w4)
+    b = ops.token_logprobs(logits, tok, 8)
+    # the product may be cut into other tiles: the bound of two ways of adding K products in fp32
+    off = 2 * (K * 2.0 ** -24) * (x.abs().double() @ (ops.q4_dequantize(w4).abs().double().t() + 0.3)).amax()
+    assert (a.logprob - b.logprob).abs().max() <= 2 * off and (a.top_logprobs - b.top_logprobs).abs().max() <= 2 * off
+    ref = torch.log_softmax(x.double() @ ops.q4_dequantize(w4).double().t(), 1)
+    assert (a.logprob.double() - ref.gather(1, tok.long().unsqueeze(1))[:, 0]).abs().max() <= 2 * off + 2.0 ** -15
+
+
+@pytest.mark.parametrize("T", [1, 70, 600])
+def test_same_bits_again_and_in_graphs(dev, T):
+    V, K, top = 30011, 128, 7
+    w4 = ops.q4_quantize(0.05 * torch.randn(V, K, device=dev))
+    x = torch.randn(T, K, device=dev)
+    tok = torch.randint(0, V, (T,), device=dev, dtype=torch.int32)
+    xs, graphs, outs = [x.clone(), x.clone()], [], []
+    first = ops.head_logprobs(x, w4, tok, top)
+    assert all(torch.equal(a, b) for a, b in zip(first, ops.head_logprobs(x, w4, tok, top)))
+    for xi in xs:
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            outs.append((ops.head_logprobs(xi, w4, tok, top), ops.token_logprobs(xi, tok % K, top)))
+        graphs.append(gr)
+    for _ in range(3):
+        for xi, gr, o in zip(xs, graphs, outs):
+            xi.copy_(torch.randn(T, K, device=dev))
+            gr.replay()
+            ops.head_logprobs(torch.randn(T + 5, K, device=dev), w4, torch.zeros(T + 5, device=dev, dtype=torch.int32), top)
+            torch.cuda.synchronize()
+            for a, b in zip(o[0] + o[1], ops.head_logprobs(xi, w4, tok, top) + ops.token_logprobs(xi, tok % K, top)):
+                assert torch.equal(a, b)
