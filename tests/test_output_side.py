@@ -159,7 +159,7 @@ def test_a_row_stride_below_the_row_reaches_the_library(monkeypatch):
     monkeypatch.setattr(ops, "_stream", lambda device=None: 0)
     x = _t(1, 64).expand(3, 64)
     with pytest.raises(ops.AegistError, match="ldx >= K"):
-        ops.linear_q4(x, _w4())
+        ops.linear_q4(x, _w4(), out=_t(3, 16))
     with pytest.raises(ops.AegistError, match="ld < V"):
         ops.token_logprobs(_t(1, 10).expand(3, 10), _t(3, dtype=torch.int32))
 
