@@ -6,8 +6,8 @@
 //   codes   [N / 16][K / 128][64 lanes][16 bytes]: 1 KB holds 16 rows x 128 k in the order of the matrix
 //           operand of v_mfma_f32_16x16x32_f16, so that a wave reads 1 KB in one contiguous piece and needs no
 //           exchange between lanes. Lane 16 q + r has row r; its dword j has the 8 codes k = 32 j + 8 q + e,
-//           element e at nibble e / 2 + 4 (e % 2): the two codes of a dword's halves, masked out in place, are
-//           two fp16 subnormals.
+//           element e from bit q4_bit(e) on (element 7 from bit 30 round to bit 1): in place, shifted by 4 either
+//           way and turned by 8, two codes at a time come to lie at bits 6 to 9 of a dword's halves.
 //   scale   [N / 16][K / G / 8][16 rows][8 groups] fp16: 16 bytes are 8 consecutive groups of a row
 //   min     the same
 // Rows, k and groups past the matrix are zeros.
@@ -16,6 +16,14 @@
 #include "common.h"
 
 namespace aegist {
+
+__host__ __device__ constexpr int q4_bit(int e) { return (e % 2) * 16 + (e < 2 ? 6 : e < 4 ? 2 : e < 6 ? 10 : 14); }
+__host__ __device__ constexpr uint32_t q4_put(uint32_t code, int e) {
+    return code << q4_bit(e) | (q4_bit(e) > 28 ? code >> (32 - q4_bit(e)) : 0);
+}
+__host__ __device__ constexpr uint32_t q4_get(uint32_t d, int e) {
+    return (d >> q4_bit(e) | (q4_bit(e) > 28 ? d << (32 - q4_bit(e)) : 0)) & 15;
+}
 
 struct Q4Dims {
     int N, K, G;
@@ -26,6 +34,15 @@ struct Q4Dims {
     __host__ __device__ size_t scale_bytes() const { return (size_t)tiles() * blocks8() * 256; }
     __host__ __device__ size_t bytes() const { return code_bytes() + 2 * scale_bytes(); }
 };
+
+struct Q4Ptr {
+    const unsigned char* codes;
+    const _Float16 *scale, *mins;
+};
+__host__ __device__ inline Q4Ptr q4_ptr(const void* w, const Q4Dims& d) {
+    const unsigned char* p = (const unsigned char*)w;
+    return {p, (const _Float16*)(p + d.code_bytes()), (const _Float16*)(p + d.code_bytes() + d.scale_bytes())};
+}
 
 // AEGIST_OK, or the error of sizes that no Q4 weight has.
 int check_q4(const char* who, int N, int K, int G);

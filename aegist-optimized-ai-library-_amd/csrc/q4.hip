@@ -1,6 +1,4 @@
-// Projections with 4-bit weights, and the making of those weights.
-//
-//   Y[m, n] (+)= sum_k X[m, k] (code[n, k] * scale[n, k / G] + min[n, k / G])
+// The making of 4-bit weights: rounding, packing and reading back. (The product is q4_linear.hip.)
 #include "q4.h"
 
 #include <algorithm>
@@ -11,17 +9,6 @@ namespace {
 
 typedef uint32_t u4v __attribute__((ext_vector_type(4)));
 
-// nibble of element e (0..7) in a dword of codes
-__host__ __device__ constexpr int q4_shift(int e) { return 4 * (e / 2 + 4 * (e % 2)); }
-
-struct Q4Ptr {
-    const unsigned char* codes;
-    const _Float16 *scale, *mins;
-};
-__host__ __device__ inline Q4Ptr q4_ptr(const void* w, const Q4Dims& d) {
-    const unsigned char* p = (const unsigned char*)w;
-    return {p, (const _Float16*)(p + d.code_bytes()), (const _Float16*)(p + d.code_bytes() + d.scale_bytes())};
-}
 // index of (row n, group g) in the scale and min sections
 __device__ __forceinline__ size_t q4_group(const Q4Dims& d, int n, int g) {
     return ((size_t)(n / 16) * d.blocks8() + g / 8) * 128 + (n % 16) * 8 + g % 8;
@@ -94,7 +81,7 @@ __global__ void __launch_bounds__(256) q4_quantize_kernel(const TW* __restrict__
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             const double v = sc > (_Float16)0.f ? rint(((double)w[j][e] - (double)mn) / (double)sc) : 0.0;
-            p |= (uint32_t)(int)fmin(fmax(v, 0.0), 15.0) << q4_shift(e);
+            p |= q4_put((uint32_t)(int)fmin(fmax(v, 0.0), 15.0), e);
         }
         const int k = c * 128 + 32 * j;
         codes[j] = row && k < d.K ? p : 0;
@@ -121,7 +108,7 @@ __global__ void __launch_bounds__(256) q4_pack_kernel(const unsigned char* __res
         uint32_t s = 0, p = 0;
         if (n < d.N && k < d.K) s = *(const uint32_t*)(codes + ((size_t)n * d.K + k) / 2);
 #pragma unroll
-        for (int e = 0; e < 8; e++) p |= (s >> (4 * e) & 15) << q4_shift(e);
+        for (int e = 0; e < 8; e++) p |= q4_put(s >> (4 * e) & 15, e);
         v[j] = p;
     }
     ((u4v*)out)[((size_t)nt * d.chunks() + c) * 64 + lane] = v;
@@ -162,41 +149,10 @@ __global__ void __launch_bounds__(256) q4_dequantize_kernel(const unsigned char*
         const float s = (float)w.scale[gi], m = (float)w.mins[gi];
         float f[8];
 #pragma unroll
-        for (int e = 0; e < 8; e++) f[e] = fmaf((float)(v[j] >> q4_shift(e) & 15), s, m);
+        for (int e = 0; e < 8; e++) f[e] = fmaf((float)q4_get(v[j], e), s, m);
         float4* o = (float4*)(out + (size_t)n * d.K + k);
         o[0] = float4{f[0], f[1], f[2], f[3]};
         o[1] = float4{f[4], f[5], f[6], f[7]};
-    }
-}
-
-// 16 rows of W x 16 rows of X per workgroup, a product per thread.
-template <typename TX>
-__global__ void __launch_bounds__(256) linear_q4_kernel(const TX* __restrict__ X, long long ldx,
-                                                        const unsigned char* __restrict__ W, float* __restrict__ Y,
-                                                        long long ldy, int M, const Q4Dims d, int accumulate) {
-    const int r = threadIdx.x % 16, n = blockIdx.x * 16 + r;
-    const Q4Ptr w = q4_ptr(W, d);
-    for (int m = blockIdx.y * 16 + threadIdx.x / 16; m < M; m += gridDim.y * 16) {
-        if (n >= d.N) return;
-        const TX* x = X + (size_t)m * ldx;
-        float acc = 0.f;
-        for (int g = 0; g < d.K / d.G; g++) {
-            float p = 0.f, s = 0.f;
-            for (int k = g * d.G; k < (g + 1) * d.G; k += 8) {
-                const int lane = k % 32 / 8 * 16 + r;
-                const uint32_t v = ((const uint32_t*)w.codes)[(((size_t)blockIdx.x * d.chunks() + k / 128) * 64 + lane) * 4 +
-                                                              k % 128 / 32];
-                for (int e = 0; e < 8; e++) {
-                    const float f = Act<TX>::ld(x, k + e);
-                    p = fmaf((float)(v >> q4_shift(e) & 15), f, p);
-                    s += f;
-                }
-            }
-            const size_t gi = q4_group(d, n, g);
-            acc = fmaf(p, (float)w.scale[gi], fmaf(s, (float)w.mins[gi], acc));
-        }
-        float* y = Y + (size_t)m * ldy + n;
-        *y = accumulate ? *y + acc : acc;
     }
 }
 
@@ -214,31 +170,6 @@ int check_q4(const char* who, int N, int K, int G) {
     if (G != 32 && G != 64 && G != 128) return fail(AEGIST_ERR_SHAPE, w + ": groups of 32, 64 or 128 values");
     if (N < 0 || K <= 0 || K % G) return fail(AEGIST_ERR_SHAPE, w + ": K must be a positive multiple of the group");
     return 0;
-}
-
-size_t linear_q4_workspace(int, int, int, int, int) { return 0; }
-
-int launch_linear_q4(const void* X, int x_dtype, long long ldx, const void* W, float* Y, long long ldy, int M, int N,
-                     int K, int G, int accumulate, void*, size_t, hipStream_t st) {
-    int rc = check_q4("linear_q4", N, K, G);
-    if (rc) return rc;
-    if (x_dtype != AEGIST_F32 && x_dtype != AEGIST_BF16)
-        return fail(AEGIST_ERR_DTYPE, "linear_q4: X must be AEGIST_F32 or AEGIST_BF16");
-    if (M < 0) return fail(AEGIST_ERR_SHAPE, "linear_q4: negative size");
-    if (M == 0 || N == 0) return 0;
-    if (!X || !W || !Y) return fail(AEGIST_ERR_SHAPE, "linear_q4: null operand");
-    const int xs = x_dtype == AEGIST_F32 ? 4 : 2;
-    if (ldx < K || (ldx * xs) % 16 || (uintptr_t)X % 16)
-        return fail(AEGIST_ERR_SHAPE, "linear_q4: X needs 16-byte aligned rows (ldx >= K)");
-    if (ldy < N) return fail(AEGIST_ERR_SHAPE, "linear_q4: ldy < N");
-    if ((uintptr_t)W % 16) return fail(AEGIST_ERR_SHAPE, "linear_q4: W must be 16-byte aligned");
-    const Q4Dims d{N, K, G};
-    const dim3 grid(d.tiles(), std::min((M + 15) / 16, 65535));
-    if (x_dtype == AEGIST_F32)
-        linear_q4_kernel<float><<<grid, 256, 0, st>>>((const float*)X, ldx, (const unsigned char*)W, Y, ldy, M, d, accumulate);
-    else
-        linear_q4_kernel<uint16_t><<<grid, 256, 0, st>>>((const uint16_t*)X, ldx, (const unsigned char*)W, Y, ldy, M, d, accumulate);
-    return after_launch("linear_q4");
 }
 
 }  // namespace aegist
@@ -298,15 +229,4 @@ extern "C" int aegist_q4_dequantize(const void* q4, float* out, int N, int K, in
     const Q4Dims d{N, K, group};
     q4_dequantize_kernel<<<q4_grid(d), 256, 0, AEG_STREAM(stream)>>>((const unsigned char*)q4, out, d);
     return after_launch("q4_dequantize");
-}
-
-extern "C" size_t aegist_linear_q4_workspace_bytes(int x_dtype, int M, int N, int K, int group) {
-    if (M < 0 || check_q4("linear_q4_workspace", N, K, group)) return 0;
-    return linear_q4_workspace(x_dtype, M, N, K, group);
-}
-
-extern "C" int aegist_linear_q4(const void* X, int x_dtype, long long ldx, const void* q4, float* Y, long long ldy,
-                                int M, int N, int K, int group, int accumulate, void* ws, size_t ws_bytes,
-                                void* stream) {
-    return launch_linear_q4(X, x_dtype, ldx, q4, Y, ldy, M, N, K, group, accumulate, ws, ws_bytes, AEG_STREAM(stream));
 }
