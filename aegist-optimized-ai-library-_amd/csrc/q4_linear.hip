@@ -43,23 +43,35 @@ __device__ __forceinline__ int row_exp(float amax) {
                                          : 0;
 }
 
-// 8 consecutive values of X as floats
-__device__ __forceinline__ void x8(const float* p, float (&f)[8]) {
-    const float4 a = ((const float4*)p)[0], b = ((const float4*)p)[1];
-    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-}
-__device__ __forceinline__ void x8(const uint16_t* p, float (&f)[8]) {
-    const uint4 a = *(const uint4*)p;
-    f[0] = bf_lo(a.x); f[1] = bf_hi(a.x); f[2] = bf_lo(a.y); f[3] = bf_hi(a.y);
-    f[4] = bf_lo(a.z); f[5] = bf_hi(a.z); f[6] = bf_lo(a.w); f[7] = bf_hi(a.w);
-}
+// 8 consecutive values of X
+template <typename TX> struct X8;
+template <> struct X8<float> {
+    f32x4 v[2];
+    // zeros where k is past the row's K (a multiple of 8)
+    __device__ __forceinline__ void load(const float* row, int k, int K) {
+        const f32x4* p = (const f32x4*)(row + min(k, K - 8));
+        const f32x4 a = p[0], b = p[1];
+        v[0] = k < K ? a : f32x4{0, 0, 0, 0};
+        v[1] = k < K ? b : f32x4{0, 0, 0, 0};
+    }
+    __device__ __forceinline__ float get(int i) const { return v[i / 4][i % 4]; }
+};
+template <> struct X8<uint16_t> {
+    u4v v;
+    __device__ __forceinline__ void load(const uint16_t* row, int k, int K) {
+        const u4v a = *(const u4v*)(row + min(k, K - 8));
+        v = k < K ? a : u4v{0, 0, 0, 0};
+    }
+    __device__ __forceinline__ float get(int i) const { return i % 2 ? bf_hi(v[i / 2]) : bf_lo(v[i / 2]); }
+};
 
 // 8 scaled values as fp16; `lo` gets the remainders
-__device__ __forceinline__ half8 x_parts(const float (&f)[8], int e, half8* lo) {
+template <typename TX>
+__device__ __forceinline__ half8 x_parts(const X8<TX>& x, int e, half8* lo) {
     half8 hi;
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-        const float v = __builtin_ldexpf(f[i], e);
+        const float v = __builtin_ldexpf(x.get(i), e);
         hi[i] = (_Float16)v;
         if (lo) (*lo)[i] = (_Float16)(v - (float)hi[i]);
     }
@@ -67,7 +79,7 @@ __device__ __forceinline__ half8 x_parts(const float (&f)[8], int e, half8* lo) 
 }
 
 struct Q4Args {
-    const void* X;
+    const void* X;  // rows, or the operands made of them (XOps)
     long long ldx;
     const unsigned char* W;
     float* Y;
@@ -77,257 +89,352 @@ struct Q4Args {
 };
 
 // ---------------------------------------------------------------------------------------------
-// Few rows: the weight stream. A workgroup stages X in LDS as fp16 rows and its waves then take whole 1 KB pieces
-// of the weight as they lie in memory, PD pieces in flight each; KS waves share a tile of 16 rows of W, every KS-th
-// piece each, and meet in LDS. The pieces of X are on their way from L2, and its rows are scaled, while the first
-// pieces of the weight come from HBM.
-constexpr int SW = 8;           // waves of a workgroup
-constexpr int SPD = 8;          // pieces in flight per wave
-constexpr int SK = 128;         // k per piece
-
-struct StreamLds {              // byte offsets
-    int rows, row_bytes, xs, xs_bytes, exps, red, total;
+// More than a few rows: X is made into matrix operands once, in the workspace, in the order in which waves load
+// them (1 KB for 16 rows x 32 k):
+//   parts [M / 16][parts][K / 32][64 lanes][8 fp16]: lane 16 q + r has k = 32 j + 8 q .. + 7 of row r, with zeros
+//         from K to a multiple of 256
+//   sums  [M / 16][2 parts][K / G / 32][64 lanes][8 fp16]: the sums of the groups 32 b + 8 q .. + 7
+//   exps  [M] int: the power of two each row was scaled by
+struct XOps {
+    int parts, steps, blocks;  // 32 k each, 32 groups each
+    size_t tiles;
+    __host__ __device__ XOps(int M, int parts, const Q4Dims& d)
+        : parts(parts), steps((d.K + 255) / 256 * 8), blocks((d.K / d.G + 31) / 32), tiles((M + 15) / 16) {}
+    __host__ __device__ size_t sums_at() const { return tiles * parts * steps * 1024; }
+    __host__ __device__ size_t exps_at() const { return sums_at() + tiles * 2 * blocks * 1024; }
+    __host__ __device__ size_t bytes() const { return exps_at() + (tiles * 64 + 255) / 256 * 256; }
 };
-__host__ __device__ inline StreamLds stream_lds(int M, int parts, const Q4Dims& d, int ks) {
-    StreamLds l;
-    l.rows = 0;
-    l.row_bytes = d.chunks() * SK * 2 + 16;  // (16 bytes on: the 16 rows of an operand read lie in different banks)
-    l.xs = M * parts * l.row_bytes;
-    l.xs_bytes = (d.K / d.G + 31) / 32 * 64 + 16;
-    l.exps = l.xs + 2 * M * l.xs_bytes;
-    l.red = l.exps + 64;
-    l.total = l.red + (ks > 1 ? 2 * SW * 1024 : 0);
-    return l;
+
+// One workgroup per 16 rows; XW waves take the steps in turn, XJ of them held in registers between the row's maximum
+// and its conversion (longer rows are read again, from L2).
+constexpr int XW = 16, XJ = 4;
+
+template <typename TX>
+__global__ void __launch_bounds__(XW * WAVE) q4_rows_kernel(const Q4Args a, unsigned char* out) {
+    constexpr bool F32 = std::is_same<TX, float>::value;
+    __shared__ float top[XW][16];
+    const Q4Dims d = a.d;
+    const XOps o(a.M, F32 ? 2 : 1, d);
+    const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+    const int r = lane % 16, q = lane / 16, spg = d.G / 32, NG = d.K / d.G;
+    const size_t mt = blockIdx.x;
+    const TX* x = (const TX*)a.X + (mt * 16 + min(r, (int)(a.M - 1 - mt * 16))) * a.ldx;
+    // consecutive steps of XJ = 4 hold whole groups
+    const int rounds = (o.steps + XW * XJ - 1) / (XW * XJ);
+    X8<TX> f[XJ];
+    float amax = 0.f;
+    for (int i = rounds - 1; i >= 0; i--) {  // (the first is read last and stays)
+#pragma unroll
+        for (int j = 0; j < XJ; j++) {
+            const int k = ((i * XW + wave) * XJ + j) * 32 + 8 * q;
+            f[j].load(x, k, d.K);
+        }
+#pragma unroll
+        for (int j = 0; j < XJ; j++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) amax = fmaxf(amax, fabsf(f[j].get(e)));
+    }
+    amax = fmaxf(amax, __shfl_xor(amax, 16, WAVE));
+    amax = fmaxf(amax, __shfl_xor(amax, 32, WAVE));
+    if (q == 0) top[wave][r] = amax;
+    lds_barrier();
+#pragma unroll
+    for (int i = 0; i < XW; i++) amax = fmaxf(amax, top[i][r]);
+    const int e = row_exp(amax);
+    if (wave == 0 && q == 0) ((int*)(out + o.exps_at()))[mt * 16 + r] = e;
+    half8* parts = (half8*)out;
+    _Float16* sums = (_Float16*)(out + o.sums_at());
+    for (int i = 0; i < rounds; i++) {
+        const int j0 = (i * XW + wave) * XJ;
+        if (j0 >= o.steps) break;
+        if (i > 0) {
+#pragma unroll
+            for (int j = 0; j < XJ; j++) {
+                const int k = (j0 + j) * 32 + 8 * q;
+                f[j].load(x, k, d.K);
+            }
+        }
+        float s = 0.f;
+#pragma unroll
+        for (int j = 0; j < XJ; j++) {
+            half8 lo;
+            const half8 hi = x_parts(f[j], e, F32 ? &lo : nullptr);
+            parts[(mt * o.parts * o.steps + j0 + j) * 64 + lane] = hi;
+            if (F32) parts[((mt * o.parts + 1) * o.steps + j0 + j) * 64 + lane] = lo;
+            s += ((f[j].get(0) + f[j].get(1)) + (f[j].get(2) + f[j].get(3))) + ((f[j].get(4) + f[j].get(5)) + (f[j].get(6) + f[j].get(7)));
+            if ((j + 1) % spg) continue;
+            s += __shfl_xor(s, 16, WAVE);
+            s += __shfl_xor(s, 32, WAVE);
+            s = __builtin_ldexpf(s, e - 7);
+            const int g = (j0 + j) / spg;
+            const _Float16 hs = (_Float16)s;
+            if (q < 2 && g < NG)  // lane 16 q + r writes part q
+                sums[(((mt * 2 + q) * o.blocks + g / 32) * 64 + g % 32 / 8 * 16 + r) * 8 + g % 8] = q ? (_Float16)(s - (float)hs) : hs;
+            s = 0.f;
+        }
+    }
+    // groups past the last
+    for (int g = NG + wave; g < o.blocks * 32; g += XW)
+        if (q < 2) sums[(((mt * 2 + q) * o.blocks + g / 32) * 64 + g % 32 / 8 * 16 + r) * 8 + g % 8] = 0;
 }
 
+// ---------------------------------------------------------------------------------------------
+// Few rows: the weight as a stream, X in registers. The waves of a workgroup cut K into slices of CPS pieces (128 k
+// each); a wave holds its slice of 16 RT rows of X as matrix operands and takes its pieces of one tile (16 rows of
+// W) after the other, the next two in flight; per round of two tiles the waves' sums meet in LDS. So a weight
+// is one contiguous 1 KB load and no more, nothing in the loop reads LDS but the sums, and a slice is
+// scaled by its own largest value, which needs no exchange between waves.
+//
+// Waves that staged X in LDS, once per workgroup, and read it back per piece took 16.5 us at 16 rows of 2048 x 4096,
+// mostly the staging (two rows per wave one after the other).
+
+template <int SPG, int CPS>
+struct Q4Slice {
+    static constexpr int GROUPS = CPS * 4 / SPG;           // groups of a slice
+    static constexpr int SB = (GROUPS + 7) / 8;            // blocks of 8 groups that they touch
+    u4v code[CPS];
+    u4v scale[SB], mins;
+};
+
 // SPG: steps of 32 k per group. PK: fp32 X of up to 8 rows, its two parts as rows m and m + 8 of one operand.
-template <typename TX, int SPG, bool PK, int KS>
-__global__ void __launch_bounds__(64 * SW) q4_stream_kernel(const Q4Args a) {
-    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+// MW: waves at most. PRE: X is there as operands (XOps), else every workgroup makes them of the rows.
+template <typename TX, int SPG, bool PK, int RT, int CPS, int MW, bool PRE>
+__global__ void __launch_bounds__(MW * WAVE) q4_stream_kernel(const Q4Args a) {
     constexpr bool F32 = std::is_same<TX, float>::value;
-    constexpr int PARTS = F32 ? 2 : 1, NA = F32 && !PK ? 2 : 1, TW = SW / KS;
-    constexpr int GP = 4 / SPG;  // groups per piece
+    constexpr int NA = F32 && !PK ? 2 : 1, NS = PK ? 1 : 2, ST = CPS * 4;
+    constexpr int SUMS = RT < 2 ? 2 : RT;  // sums per meeting of the waves
+    typedef Q4Slice<SPG, CPS> Slice;
+    constexpr int NB = SUMS / RT;  // tiles of such a meeting
+    extern __shared__ f32x4 red_raw[];  // [2][SUMS][KS][WAVE]
     const Q4Dims d = a.d;
     const Q4Ptr w = q4_ptr(a.W, d);
     const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
-    const int r = lane % 16, q = lane / 16, ks = wave % KS, tw = wave / KS;
-    const int M = a.M, KC = d.chunks(), NG = d.K / d.G, B8 = d.blocks8(), tiles = d.tiles();
-    const StreamLds sl = stream_lds(M, PARTS, d, KS);
-    // a tile's items of this wave: pieces of codes, then blocks of 32 groups' minima
-    const int ni = (KC + KS - 1) / KS, nb = ((NG + 31) / 32 + KS - 1) / KS, n1 = ni + nb;
-    const int t0 = blockIdx.x * TW, tstep = gridDim.x * TW;
-    const int its = (tiles - t0 + tstep - 1) / tstep;  // rounds of this workgroup's tiles (the same for its waves)
+    const int r = lane % 16, q = lane / 16, KS = blockDim.x / WAVE;
+    const int KC = d.chunks(), B8 = d.blocks8(), tiles = d.tiles();
+    const int c0 = wave * CPS, g0 = c0 * (4 / SPG);       // first piece and first group of the slice
+    const int m0 = blockIdx.y * (16 * RT), M = a.M - m0;  // rows of this workgroup
 
-    u4v code[SPD];
-    u2v sc[SPD];
-    int lt = t0 + tw, li = 0;
-    auto load = [&](int slot) {
-        code[slot] = u4v{0, 0, 0, 0};
-        sc[slot] = u2v{0, 0};
-        if (lt < tiles) {
-            if (li < ni) {
-                const int c = ks + KS * li;
-                if (c < KC) {
-                    code[slot] = __builtin_nontemporal_load((const u4v*)w.codes + ((size_t)lt * KC + c) * 64 + lane);
-                    const _Float16* p = w.scale + ((size_t)lt * B8 + c * GP / 8) * 128 + r * 8 + c * GP % 8;
-                    if (GP == 4) sc[slot] = *(const u2v*)p;
-                    else if (GP == 2) sc[slot][0] = *(const uint32_t*)p;
-                    else sc[slot][0] = *(const uint16_t*)p;
-                }
-            } else {
-                const int b8 = (ks + KS * (li - ni)) * 4 + q;
-                if (b8 < B8) code[slot] = *(const u4v*)(w.mins + ((size_t)lt * B8 + b8) * 128 + r * 8);
-            }
-        }
-        if (++li == n1) li = 0, lt += tstep;
+    // tiles blockIdx.x, + gridDim.x, ... Pieces and groups past K repeat the last ones: X is zero there.
+    Slice sl[2];
+    const int cl = KC - 1 - c0, bl = B8 - 1 - g0 / 8;
+    const int mb = PRE ? min(wave * 4 + q, B8 - 1) : g0 / 8 + min(q, min(Slice::SB - 1, bl));
+    auto load = [&](Slice& s, int t) {
+        if (t >= tiles) return;
+        const u4v* cp = (const u4v*)w.codes + ((size_t)t * KC + c0) * 64 + lane;
+        const _Float16* sp = w.scale + ((size_t)t * B8 + g0 / 8) * 128 + r * 8;
+#pragma unroll
+        for (int c = 0; c < CPS; c++) s.code[c] = __builtin_nontemporal_load(cp + min(c, cl) * 64);
+#pragma unroll
+        for (int b = 0; b < Slice::SB; b++) s.scale[b] = *(const u4v*)(sp + min(b, bl) * 128);
+        s.mins = *(const u4v*)(w.mins + ((size_t)t * B8 + mb) * 128 + r * 8);
     };
-#pragma unroll
-    for (int s = 0; s < SPD; s++) load(s);
+    load(sl[0], blockIdx.x);
+    load(sl[1], blockIdx.x + gridDim.x);
 
-    // X: `wpr` waves per row, 8 consecutive values per lane and step
-    {
-        int* exps = (int*)(lds + sl.exps);
-        float* part = (float*)(lds + sl.exps);  // one maximum per wave, before the exponents take their place
-        const int wpr = M == 1 ? 8 : M == 2 ? 4 : M <= 4 ? 2 : 1, seg = wave % wpr;
-        const int KP = KC * SK;
-        auto amax_of = [&](int m) {
-            const TX* x = (const TX*)a.X + (size_t)m * a.ldx;
-            float v = 0.f;
-            for (int k = (seg * WAVE + lane) * 8; k < d.K; k += wpr * WAVE * 8) {
-                float f[8];
-                x8(x + k, f);
+    // the slice of X: lane (r, q) has k = 32 j + 8 q .. + 7 of the steps j, of row r (PK: of row r % 8)
+    half8 xa[RT][NA][ST], xs[PRE ? 1 : RT][NS];
+    int e4[PRE ? 1 : RT][4];  // exponents of the rows 4 q + i whose sums this lane holds
+    // PRE: the waves' blocks of sums [blocks][RT][2][WAVE], which a tile reads once
+    half8* xsl = (half8*)(red_raw + 2 * SUMS * KS * WAVE);
+    const int nblocks = (d.K / d.G + 31) / 32;
 #pragma unroll
-                for (int i = 0; i < 8; i++) v = fmaxf(v, fabsf(f[i]));
-            }
-            return wave_max(v);
-        };
-        auto convert = [&](int m, int e) {
-            const TX* x = (const TX*)a.X + (size_t)m * a.ldx;
-            for (int k0 = seg * WAVE * 8; k0 < KP; k0 += wpr * WAVE * 8) {
-                const int k = k0 + lane * 8;
-                float f[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-                if (k < d.K) x8(x + k, f);
-                half8 lo;
-                const half8 hi = x_parts(f, e, F32 ? &lo : nullptr);
-                if (k < KP) {
-                    *(half8*)(lds + m * sl.row_bytes + 2 * k) = hi;
-                    if (F32) *(half8*)(lds + (M + m) * sl.row_bytes + 2 * k) = lo;
-                }
-                // the group's sum: 4, 8 or 16 lanes
-                float s = ((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7]));
+    for (int t = 0; t < RT; t++) {
+        if constexpr (PRE) {
+            const XOps o(a.M, NA, d);
+            const size_t mt = min((size_t)(m0 / 16 + t), o.tiles - 1);
+            const half8* parts = (const half8*)a.X;
+            const half8* sums = (const half8*)((const unsigned char*)a.X + o.sums_at());
 #pragma unroll
-                for (int o = 1; o < 4 * SPG; o *= 2) s += __shfl_xor(s, o, WAVE);
-                if (lane % (4 * SPG) == 0 && k < d.K) {
-                    s = __builtin_ldexpf(s, e - 7);
-                    const _Float16 h = (_Float16)s;
-                    *(_Float16*)(lds + sl.xs + m * sl.xs_bytes + k / d.G * 2) = h;
-                    *(_Float16*)(lds + sl.xs + (M + m) * sl.xs_bytes + k / d.G * 2) = (_Float16)(s - (float)h);
-                }
+            for (int n = 0; n < NA; n++)
+#pragma unroll
+                for (int j = 0; j < ST; j++) xa[t][n][j] = parts[((mt * NA + n) * o.steps + c0 * 4 + j) * 64 + lane];
+            if (wave < nblocks) {
+#pragma unroll
+                for (int n = 0; n < 2; n++)
+                    xsl[((wave * RT + t) * 2 + n) * WAVE + lane] = sums[((mt * 2 + n) * o.blocks + wave) * 64 + lane];
             }
-            if (seg == 0)
-                for (int g = NG + lane; g < (NG + 31) / 32 * 32; g += WAVE) {
-                    *(_Float16*)(lds + sl.xs + m * sl.xs_bytes + g * 2) = 0;
-                    *(_Float16*)(lds + sl.xs + (M + m) * sl.xs_bytes + g * 2) = 0;
-                }
-        };
-        if (wpr > 1) {
-            const int m = wave / wpr;
-            const float v = m < M ? amax_of(m) : 0.f;
-            if (lane == 0) part[wave] = v;
-            lds_barrier();
-            float v2 = 0.f;
-            for (int i = 0; i < wpr; i++) v2 = fmaxf(v2, part[wave / wpr * wpr + i]);
-            const int e = row_exp(v2);
-            lds_barrier();
-            if (m < M) {
-                convert(m, e);
-                if (seg == 0 && lane == 0) exps[m] = e;
-            }
-        } else {
-            for (int m = wave; m < M; m += SW) {
-                const int e = row_exp(amax_of(m));
-                convert(m, e);
-                if (lane == 0) exps[m] = e;
-            }
+            continue;
         }
-        lds_barrier();
+        const int m = min(PK ? r % 8 : 16 * t + r, M - 1);
+        const TX* x = (const TX*)a.X + (size_t)(m0 + m) * a.ldx;
+        X8<TX> f[ST];
+        float amax = 0.f;
+#pragma unroll
+        for (int j = 0; j < ST; j++) {
+            const int k = c0 * 128 + 32 * j + 8 * q;
+            f[j].load(x, k, d.K);
+        }
+#pragma unroll
+        for (int j = 0; j < ST; j++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) amax = fmaxf(amax, fabsf(f[j].get(i)));
+        amax = fmaxf(amax, __shfl_xor(amax, 16, WAVE));
+        amax = fmaxf(amax, __shfl_xor(amax, 32, WAVE));
+        const int e = row_exp(amax);
+#pragma unroll
+        for (int i = 0; i < 4; i++) e4[t][i] = 7 - __shfl(e, (4 * q + i) % (PK ? 8 : 16), WAVE);
+        float s = 0.f;
+        half8 hi{}, lo{};
+#pragma unroll
+        for (int j = 0; j < ST; j++) {
+            half8 l;
+            const half8 h = x_parts(f[j], e, F32 ? &l : nullptr);
+            if (PK) xa[t][0][j] = r < 8 ? h : l;
+            else {
+                xa[t][0][j] = h;
+                if (NA == 2) xa[t][NA - 1][j] = l;
+            }
+            s += ((f[j].get(0) + f[j].get(1)) + (f[j].get(2) + f[j].get(3))) + ((f[j].get(4) + f[j].get(5)) + (f[j].get(6) + f[j].get(7)));
+            if (j % SPG < SPG - 1) continue;
+            // the group's sum, and its place among the 8 of the block that lanes q read the minima of
+            s += __shfl_xor(s, 16, WAVE);
+            s += __shfl_xor(s, 32, WAVE);
+            s = __builtin_ldexpf(s, e - 7);
+            const _Float16 sh = (_Float16)s, slo = (_Float16)(s - (float)sh);
+            const int g = j / SPG;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const bool here = Slice::GROUPS >= 8 ? g % 8 == i && q == g / 8 : q == 0 && (g0 + g) % 8 == i;
+                hi[i] = here ? sh : hi[i];
+                lo[i] = here ? slo : lo[i];
+            }
+            s = 0.f;
+        }
+        if (PK) xs[t][0] = r < 8 ? hi : lo;
+        else xs[t][0] = hi, xs[t][NS - 1] = lo;
     }
 
-    // LDS rows of this lane's operand row
-    const int mr = min(PK ? r % 8 : r, M - 1);
-    const unsigned char* xrow[NA];
-    xrow[0] = lds + ((PK && r >= 8 ? M : 0) + mr) * sl.row_bytes + q * 16;
-    if (NA == 2) xrow[NA - 1] = lds + (M + mr) * sl.row_bytes + q * 16;
-    const unsigned char* srow = lds + sl.xs + min(r, M - 1) * sl.xs_bytes + q * 16;
-
-    f32x4 acc{0.f, 0.f, 0.f, 0.f}, accm{0.f, 0.f, 0.f, 0.f};
-    int ct = t0 + tw, ci = 0, it = 0;
-    const int total = its * n1;
-    for (int f = 0; f < total; f += SPD) {
+    // a tile: this wave's share of its sums, in units of Y
+    auto product = [&](const Slice& s, f32x4 (&v)[RT]) {
+        f32x4 acc[RT], p[RT];
 #pragma unroll
-        for (int s = 0; s < SPD; s++) {
-            if (f + s >= total) break;
-            if (ci < ni) {
-                const int c = ks + KS * ci;
-                if (c < KC) {
-                    f32x4 p{0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < RT; t++) acc[t] = p[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const half8 b = q4_codes(code[s][j]);
+        for (int j = 0; j < ST; j++) {
+            const half8 b = q4_codes(s.code[j / 4][j % 4]);
 #pragma unroll
-                        for (int n = 0; n < NA; n++) {
-                            const half8 x = *(const half8*)(xrow[n] + c * (SK * 2) + j * 64);
-                            p = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, b, p, 0, 0, 0);
-                        }
-                        if (j % SPG == SPG - 1) {
-                            const int g = j / SPG;
-                            const float scale = (float)__builtin_bit_cast(_Float16, (uint16_t)(sc[s][g / 2] >> (16 * (g % 2))));
-                            acc += p * scale;
-                            p = f32x4{0.f, 0.f, 0.f, 0.f};
-                        }
-                    }
+            for (int n = 0; n < NA; n++)
+#pragma unroll
+                for (int t = 0; t < RT; t++) p[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xa[t][n][j], b, p[t], 0, 0, 0);
+            if (j % SPG < SPG - 1) continue;
+            const int g = j / SPG;
+            uint32_t sw;  // (a slice of 4 or 2 groups begins in the middle of its block)
+            if (Slice::GROUPS >= 8) sw = s.scale[g / 8][g % 8 / 2];
+            else if (Slice::GROUPS == 4) sw = g0 % 8 ? s.scale[0][2 + g / 2] : s.scale[0][g / 2];
+            else if (Slice::GROUPS == 2) sw = s.scale[0][g0 / 2 % 4];
+            else sw = s.scale[0][g0 / 2 % 4] >> (16 * (g0 % 2));
+            const float sc = (float)__builtin_bit_cast(_Float16, (uint16_t)(Slice::GROUPS > 1 ? sw >> (16 * (g % 2)) : sw));
+#pragma unroll
+            for (int t = 0; t < RT; t++) {
+                acc[t] += p[t] * sc;
+                p[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+            }
+            __builtin_amdgcn_sched_barrier(0);  // (codes are unpacked a group at a time: registers)
+        }
+        const half8 mn = __builtin_bit_cast(half8, s.mins);
+#pragma unroll
+        for (int t = 0; t < RT; t++) {
+            f32x4 am = acc[t] * kCodeUnit;
+            if constexpr (PRE) {
+                if (wave < nblocks) {
+#pragma unroll
+                    for (int n = 0; n < 2; n++)
+                        am = __builtin_amdgcn_mfma_f32_16x16x32_f16(xsl[((wave * RT + t) * 2 + n) * WAVE + lane], mn, am, 0, 0, 0);
                 }
+                v[t] = am;
             } else {
-                const int b = ks + KS * (ci - ni);
-                if (b * 32 < NG) {
-                    const half8 mn = __builtin_bit_cast(half8, code[s]);
 #pragma unroll
-                    for (int n = 0; n < 2; n++) {
-                        const half8 x = *(const half8*)(srow + n * M * sl.xs_bytes + b * 64);
-                        accm = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, mn, accm, 0, 0, 0);
-                    }
+                for (int n = 0; n < NS; n++) am = __builtin_amdgcn_mfma_f32_16x16x32_f16(xs[t][n], mn, am, 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < 4; i++) v[t][i] = __builtin_ldexpf(PK ? pair_sum32(am[i]) : am[i], e4[t][i]);
+            }
+        }
+    };
+
+    auto red = [&](int buf, int i, int k) -> f32x4& { return red_raw[((buf * SUMS + i) * KS + k) * WAVE + lane]; };
+    int buf = 0;
+    for (int t0 = blockIdx.x; t0 < tiles; t0 += 2 * gridDim.x) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int ct = t0 + h * gridDim.x;  // (the same for all waves)
+            if (ct < tiles) {
+                f32x4 v[RT];
+                product(sl[h], v);
+                load(sl[h], ct + 2 * gridDim.x);
+#pragma unroll
+                for (int t = 0; t < RT; t++) red(buf, h % NB + t, wave) = v[t];
+            }
+            if (h % NB < NB - 1) continue;
+            lds_barrier();  // (the other buffer's readers are past it when they reach the next one)
+            // the sums over the waves: lane (r, q) has rows 4 q .. 4 q + 3 of Y's column 16 ct + r
+            for (int i = wave; i < SUMS; i += KS) {
+                const int t = RT == 1 ? 0 : i, tt = RT == 1 ? t0 + i * gridDim.x : ct, n = tt * 16 + r;
+                if (tt >= tiles) break;
+                f32x4 v = red(buf, i, 0);
+                for (int k = 1; k < KS; k++) v += red(buf, i, k);
+                if constexpr (PRE) {  // (one power of two for all slices of a row)
+                    const XOps o(a.M, NA, d);
+                    const int4 e = *((const int4*)((const unsigned char*)a.X + o.exps_at()) + min((size_t)(m0 / 16 + t), o.tiles - 1) * 4 + q);
+                    v = f32x4{__builtin_ldexpf(v[0], 7 - e.x), __builtin_ldexpf(v[1], 7 - e.y), __builtin_ldexpf(v[2], 7 - e.z),
+                              __builtin_ldexpf(v[3], 7 - e.w)};
                 }
-            }
-            load(s);
-            if (++ci < n1) continue;
-            // the tile's last item: lane (r, q) holds rows 4 q .. 4 q + 3 of Y's column 16 ct + r
-            f32x4 v = acc * kCodeUnit;
-            if (PK) {
+                if (n >= d.N) continue;
 #pragma unroll
-                for (int i = 0; i < 4; i++) v[i] = pair_sum32(v[i]);
-            }
-            v += accm;
-            bool mine = true;
-            if (KS > 1) {
-                f32x4* red = (f32x4*)(lds + sl.red + it % 2 * (SW * 1024));
-                red[wave * 64 + lane] = v;
-                lds_barrier();
-                mine = ks == 0;
-                if (mine) {
-#pragma unroll
-                    for (int i = 1; i < KS; i++) v += red[(wave + i) * 64 + lane];
-                }
-            }
-            const int n = ct * 16 + r;
-            if (mine && ct < tiles && n < d.N) {
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int m = 4 * q + i;
+                for (int j = 0; j < 4; j++) {
+                    const int m = 16 * t + 4 * q + j;
                     if (m < M) {
-                        float* y = a.Y + (size_t)m * a.ldy + n;
-                        const float o = __builtin_ldexpf(v[i], 7 - ((const int*)(lds + sl.exps))[m]);
-                        *y = a.accumulate ? *y + o : o;
+                        float* y = a.Y + (size_t)(m0 + m) * a.ldy + n;
+                        *y = a.accumulate ? *y + v[j] : v[j];
                     }
                 }
             }
-            acc = accm = f32x4{0.f, 0.f, 0.f, 0.f};
-            ci = 0;
-            ct += tstep;
-            it++;
+            buf ^= 1;
         }
     }
 }
 
-template <typename TX, int SPG, bool PK, int KS>
-int launch_stream(const Q4Args& a, int grid, hipStream_t st) {
-    const int bytes = stream_lds(a.M, std::is_same<TX, float>::value ? 2 : 1, a.d, KS).total;
-    if (bytes > 65536)
-        AEG_HIP(hipFuncSetAttribute((const void*)q4_stream_kernel<TX, SPG, PK, KS>,
-                                    hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
-    q4_stream_kernel<TX, SPG, PK, KS><<<grid, 64 * SW, bytes, st>>>(a);
+template <typename TX, int SPG, bool PK, int RT, int CPS, int MW, bool PRE>
+int launch_stream(const Q4Args& a, hipStream_t st) {
+    const int ks = (a.d.chunks() + CPS - 1) / CPS, tiles = a.d.tiles(), gy = (a.M + 16 * RT - 1) / (16 * RT);
+    // 16 waves per CU, or 8 with X's operands in twice the registers; every workgroup as many tiles as the others
+    const int cu = PRE ? 8 : 16, most = std::max(1, 256 * std::max(1, cu / ks) / gy), rounds = (tiles + most - 1) / most;
+    const int lds = ((RT < 2 ? 4 : 2 * RT) * ks + (PRE ? (a.d.K / a.d.G + 31) / 32 * 2 * RT : 0)) * 1024;
+    if (lds > 65536)
+        AEG_HIP(hipFuncSetAttribute((const void*)q4_stream_kernel<TX, SPG, PK, RT, CPS, MW, PRE>,
+                                    hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+    q4_stream_kernel<TX, SPG, PK, RT, CPS, MW, PRE><<<dim3((tiles + rounds - 1) / rounds, gy), ks * WAVE,
+                                                      lds, st>>>(a);
     return after_launch("linear_q4");
 }
 
-template <typename TX, int SPG, bool PK>
-int stream_ks(const Q4Args& a, hipStream_t st) {
-    const int tiles = a.d.tiles();
-    // waves per tile
-    const int ks = tiles >= 4096 ? 1 : tiles >= 1024 ? 4 : 8;
-    auto grid = [&](int k) { return std::min((tiles + SW / k - 1) / (SW / k), 512); };
-    switch (ks) {
-        case 1: return launch_stream<TX, SPG, PK, 1>(a, grid(1), st);
-        case 4: return launch_stream<TX, SPG, PK, 4>(a, grid(4), st);
-        default: return launch_stream<TX, SPG, PK, 8>(a, grid(8), st);
+template <typename TX, bool PK, int RT, int CPS, int MW, bool PRE>
+int stream_spg(const Q4Args& a, hipStream_t st) {
+    switch (a.d.G) {
+        case 32: return launch_stream<TX, 1, PK, RT, CPS, MW, PRE>(a, st);
+        case 64: return launch_stream<TX, 2, PK, RT, CPS, MW, PRE>(a, st);
+        default: return launch_stream<TX, 4, PK, RT, CPS, MW, PRE>(a, st);
     }
 }
 
-template <typename TX, bool PK>
-int stream_spg(const Q4Args& a, hipStream_t st) {
-    switch (a.d.G) {
-        case 32: return stream_ks<TX, 1, PK>(a, st);
-        case 64: return stream_ks<TX, 2, PK>(a, st);
-        default: return stream_ks<TX, 4, PK>(a, st);
-    }
+// Rows of X and K that the stream takes: what of X fits in the registers beside the pieces in flight.
+bool stream_fits(int M, const Q4Dims& d) { return M <= 16 && d.K <= 4096; }
+bool pre_fits(int M, const Q4Dims& d) { return M <= 4096 && d.K <= 2048; }
+
+int run_stream(const Q4Args& a, int x_dtype, hipStream_t st) {
+    if (x_dtype == AEGIST_BF16) return stream_spg<uint16_t, false, 1, 2, 16, false>(a, st);
+    if (a.M <= 8) return stream_spg<float, true, 1, 2, 16, false>(a, st);
+    return a.d.K > 2048 ? stream_spg<float, false, 1, 4, 8, false>(a, st) : stream_spg<float, false, 1, 2, 8, false>(a, st);
+}
+
+int run_rows(Q4Args a, int x_dtype, void* ws, hipStream_t st) {
+    const int tiles = (a.M + 15) / 16;
+    if (x_dtype == AEGIST_F32) q4_rows_kernel<float><<<tiles, XW * WAVE, 0, st>>>(a, (unsigned char*)ws);
+    else q4_rows_kernel<uint16_t><<<tiles, XW * WAVE, 0, st>>>(a, (unsigned char*)ws);
+    int rc = after_launch("linear_q4");
+    if (rc) return rc;
+    a.X = ws;
+    if (x_dtype == AEGIST_F32) return stream_spg<float, false, 2, 2, 8, true>(a, st);
+    return a.M <= 32 ? stream_spg<uint16_t, false, 2, 2, 8, true>(a, st) : stream_spg<uint16_t, false, 4, 2, 8, true>(a, st);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -362,24 +469,17 @@ __global__ void __launch_bounds__(256) linear_q4_kernel(const TX* __restrict__ X
     }
 }
 
-// LDS that a workgroup may take: 160 KB per CU
-constexpr int kStreamLds = 160 * 1024;
-
-bool stream_fits(int x_dtype, int M, const Q4Dims& d) {
-    return M <= 16 && stream_lds(M, x_dtype == AEGIST_F32 ? 2 : 1, d, SW).total <= kStreamLds;
-}
-
 }  // namespace
 
 namespace aegist {
 
 size_t linear_q4_workspace(int x_dtype, int M, int N, int K, int G) {
-    (void)x_dtype, (void)M, (void)N, (void)K, (void)G;
-    return 0;
+    const Q4Dims d{N, K, G};
+    return M == 0 || N == 0 || stream_fits(M, d) || !pre_fits(M, d) ? 0 : XOps(M, x_dtype == AEGIST_F32 ? 2 : 1, d).bytes();
 }
 
 int launch_linear_q4(const void* X, int x_dtype, long long ldx, const void* W, float* Y, long long ldy, int M, int N,
-                     int K, int G, int accumulate, void*, size_t, hipStream_t st) {
+                     int K, int G, int accumulate, void* ws, size_t ws_bytes, hipStream_t st) {
     int rc = check_q4("linear_q4", N, K, G);
     if (rc) return rc;
     if (x_dtype != AEGIST_F32 && x_dtype != AEGIST_BF16)
@@ -393,11 +493,10 @@ int launch_linear_q4(const void* X, int x_dtype, long long ldx, const void* W, f
     if (ldy < N) return fail(AEGIST_ERR_SHAPE, "linear_q4: ldy < N");
     if ((uintptr_t)W % 16) return fail(AEGIST_ERR_SHAPE, "linear_q4: W must be 16-byte aligned");
     const Q4Dims d{N, K, G};
-    if (stream_fits(x_dtype, M, d)) {
-        const Q4Args a{X, ldx, (const unsigned char*)W, Y, ldy, M, accumulate, d};
-        if (x_dtype == AEGIST_BF16) return stream_spg<uint16_t, false>(a, st);
-        return M <= 8 ? stream_spg<float, true>(a, st) : stream_spg<float, false>(a, st);
-    }
+    const Q4Args a{X, ldx, (const unsigned char*)W, Y, ldy, M, accumulate, d};
+    if (stream_fits(M, d)) return run_stream(a, x_dtype, st);
+    if ((rc = check_workspace(ws, ws_bytes, linear_q4_workspace(x_dtype, M, N, K, G), "linear_q4"))) return rc;
+    if (pre_fits(M, d)) return run_rows(a, x_dtype, ws, st);
     const dim3 grid(d.tiles(), std::min((M + 15) / 16, 65535));
     if (x_dtype == AEGIST_F32)
         linear_q4_kernel<float><<<grid, 256, 0, st>>>((const float*)X, ldx, (const unsigned char*)W, Y, ldy, M, d, accumulate);
