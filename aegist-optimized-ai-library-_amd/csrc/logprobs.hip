@@ -6,6 +6,10 @@
 // (the entropy's sum is taken over x - m, not x, so that a common offset of the logits costs no digits). Logits
 // of -inf have no probability; a row of nothing else has logprob -inf for every token and entropy 0. NaN or
 // +inf anywhere in a row makes its logprobs and entropy NaN.
+//
+// One pass: a workgroup holds a segment of a row in registers, so the maximum, the sums relative to it and the
+// selection of the alternatives read it from there. Segments of a row (and, for a head, blocks of the vocabulary)
+// are joined by their maxima in fixed order; few rows are cut into many splits, which a second launch joins.
 #include "q4.h"
 
 #include <algorithm>
@@ -20,16 +24,27 @@ int launch_proj(const void* X, int x_dtype, long long ldx, const void* W, int w_
 namespace {
 
 constexpr int MAX_TOP = 64;
+constexpr int NT = 256, NW = NT / WAVE;  // threads, waves
+constexpr int CAP = 512;                 // candidates that are ranked at once
+
+typedef uint32_t u4v __attribute__((ext_vector_type(4)));
+typedef unsigned long long u64;
 
 // Order of the alternatives as one number: the larger value first (NaN before all, -0 as +0), then the lower
 // token. Larger keys come first; 0 is below every element's.
-__device__ __forceinline__ uint64_t lp_key(float v, uint32_t id) {
+__device__ __forceinline__ u64 lp_key(float v, uint32_t id) {
     const uint32_t b = v != v ? 0x7fc00000u : __float_as_uint(v + 0.f);
-    return (uint64_t)(b & 0x80000000u ? ~b : b | 0x80000000u) << 32 | (uint32_t)~id;
+    return (u64)(b & 0x80000000u ? ~b : b | 0x80000000u) << 32 | (uint32_t)~id;
 }
-__device__ __forceinline__ float lp_key_value(uint64_t k) {
+__device__ __forceinline__ float lp_key_value(u64 k) {
     const uint32_t b = (uint32_t)(k >> 32);
     return __uint_as_float(b & 0x80000000u ? b & 0x7fffffffu : ~b);
+}
+__device__ __forceinline__ u64 max64(u64 a, u64 b) { return a > b ? a : b; }
+__device__ __forceinline__ u64 wave_max64(u64 k) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) k = max64(k, __shfl_xor(k, o, WAVE));
+    return k;
 }
 
 struct LogprobOut {
@@ -40,65 +55,250 @@ struct LogprobOut {
     int top;
 };
 
-// one workgroup per row
-template <typename T>
-__global__ void __launch_bounds__(256) logprobs_kernel(const T* __restrict__ L, long long ld, int rows, int V,
-                                                       const LogprobOut o) {
-    __shared__ float red[4];
-    __shared__ uint64_t best[4];
-    for (int t = blockIdx.x; t < rows; t += gridDim.x) {
+// What a split of a row leaves: maximum, sums relative to it, the token's logit if it lies in the split; NaN or
+// +inf seen. Its alternatives follow apart.
+struct Part {
+    float m, z, s, tok;
+    int bad, pad[3];
+};
+__host__ __device__ inline size_t parts_bytes(int T, int splits, int top) {
+    return ((size_t)T * splits * (sizeof(Part) + (size_t)top * sizeof(u64)) + 255) / 256 * 256;
+}
+
+__device__ __forceinline__ void join(Part& a, const Part& b) {
+    const float m = fmaxf(a.m, b.m);
+    // (a side that is empty, or any side of a bad row, is not scaled: no inf - inf)
+    const float da = a.m == m ? 0.f : a.m - m, db = b.m == m ? 0.f : b.m - m;
+    const float fa = a.m == -INFINITY ? 0.f : expf(da), fb = b.m == -INFINITY ? 0.f : expf(db);
+    // s = sum e^(x - m') (x - m'), moved to m: e^d (s + d z)
+    const float sa = fa > 0.f ? fa * fmaf(da, a.z, a.s) : 0.f, sb = fb > 0.f ? fb * fmaf(db, b.z, b.s) : 0.f;
+    a.z = fa * a.z + fb * b.z;
+    a.s = sa + sb;
+    a.m = m;
+    a.tok = b.tok > a.tok || b.tok != b.tok ? b.tok : a.tok;  // (-inf where the token is not)
+    a.bad |= b.bad;
+}
+
+__device__ __forceinline__ void finish(const LogprobOut& o, int t, int V, const Part& p) {
+    const bool bad = p.bad, empty = p.m == -INFINITY;
+    const float lz = bad ? __builtin_nanf("") : logf(p.z);
+    const int tok = o.tokens[t];
+    float lp = tok < 0 ? 0.f : __builtin_nanf("");
+    if (tok >= 0 && tok < V && !bad) lp = empty ? -INFINITY : p.tok - p.m - lz;
+    o.logprob[t] = lp;
+    o.entropy[t] = empty && !bad ? 0.f : lz - p.s / p.z;
+}
+__device__ __forceinline__ void finish_top(const LogprobOut& o, int t, int j, const Part& p, u64 key) {
+    o.top_ids[(size_t)t * o.top + j] = (int)~(uint32_t)key;
+    o.top_logprobs[(size_t)t * o.top + j] = p.bad              ? __builtin_nanf("")
+                                            : p.m == -INFINITY ? -INFINITY
+                                                               : lp_key_value(key) - p.m - logf(p.z);
+}
+
+// 4 consecutive logits
+template <typename T> struct L4;
+template <> struct L4<float> {
+    typedef float v __attribute__((ext_vector_type(4), aligned(4)));
+    v x;
+    __device__ __forceinline__ void load(const float* p) { x = __builtin_nontemporal_load((const v*)p); }
+    __device__ __forceinline__ float get(int i) const { return x[i]; }
+    __device__ __forceinline__ void set(int i, float f) { x[i] = f; }
+};
+template <> struct L4<uint16_t> {
+    typedef uint16_t v __attribute__((ext_vector_type(4), aligned(2)));
+    v x;
+    __device__ __forceinline__ void load(const uint16_t* p) { x = __builtin_nontemporal_load((const v*)p); }
+    __device__ __forceinline__ float get(int i) const { return bf2f(x[i]); }
+    __device__ __forceinline__ void set(int i, float f) { x[i] = f2bf(f); }
+};
+
+struct Lds {
+    float red[3][NW];
+    int flag[NW];
+    u64 thr[NW];
+    int count;
+    u64 cand[CAP + MAX_TOP];   // candidates of a segment, after the alternatives so far
+    u64 list[MAX_TOP];
+};
+
+// the `top` largest of n <= CAP + MAX_TOP keys (all different, or 0) into list, descending
+__device__ __forceinline__ void rank_keys(const u64* cand, int n, u64* list, int top) {
+    for (int i = threadIdx.x; i < n; i += NT) {
+        const u64 k = cand[i];
+        int r = 0;
+        for (int j = 0; j < n; j++) r += cand[j] > k;
+        if (r < top && k) list[r] = k;
+    }
+}
+
+// A workgroup's splits: rows x splits items, each `span` logits (the last fewer) in segments of 4 VPT NT. `base` is
+// the first token of these logits, V the whole vocabulary's. With one split the outputs are written here.
+template <typename T, int VPT>
+__global__ void __launch_bounds__(NT) logprobs_kernel(const T* __restrict__ L, long long ld, int rows, int cols, int base,
+                                                      int V, int span, int split0, int splits, int all_splits,
+                                                      Part* __restrict__ parts, u64* __restrict__ tops, const LogprobOut o) {
+    __shared__ Lds s;
+    const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE, top = o.top;
+    constexpr int SEG = 4 * VPT * NT;
+    for (long long item = blockIdx.x; item < (long long)rows * splits; item += gridDim.x) {
+        const int t = (int)(item / splits), sp = (int)(item % splits);
+        const int c0 = sp * span, c1 = min(cols, c0 + span);
         const T* x = L + (size_t)t * ld;
-        float m = -INFINITY;
-        bool bad = false;
-        for (int i = threadIdx.x; i < V; i += 256) {
-            const float v = Act<T>::ld(x, i);
-            m = fmaxf(m, v);
-            bad |= v != v || v == INFINITY;
+        const int tok = o.tokens[t] - base;
+        Part p{-INFINITY, 0.f, 0.f, -INFINITY, 0, {}};
+        if (tok >= c0 && tok < c1) p.tok = Act<T>::ld(x, tok);
+        int have = 0;  // alternatives so far (the same in all threads)
+        for (int b = c0; b < c1; b += SEG) {
+            L4<T> v[VPT];
+            // thread's logits: b + 4 (NT i + thread) ..
+#pragma unroll
+            for (int i = 0; i < VPT; i++) {
+                const int c = b + 4 * (NT * i + (int)threadIdx.x);
+                if (c + 4 <= c1) {
+                    v[i].load(x + c);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) v[i].set(e, c + e < c1 ? Act<T>::ld(x, c + e) : -INFINITY);
+                }
+            }
+            float m = -INFINITY;
+            bool bad = false;
+#pragma unroll
+            for (int i = 0; i < VPT; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float f = v[i].get(e);
+                    m = fmaxf(m, f);
+                    bad |= !(f < INFINITY);
+                }
+            m = wave_max(m);
+            const bool wbad = __any(bad);
+            __syncthreads();
+            if (lane == 0) s.red[0][wave] = m, s.flag[wave] = wbad;
+            if (threadIdx.x == 0) s.count = have;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < NW; w++) m = fmaxf(m, s.red[0][w]);
+            Part q{m, 0.f, 0.f, -INFINITY, s.flag[0] | s.flag[1] | s.flag[2] | s.flag[3], {}};
+            if (m > -INFINITY && !q.bad) {
+#pragma unroll
+                for (int i = 0; i < VPT; i++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const float d = v[i].get(e) - m, ex = __expf(d);
+                        q.z += ex;
+                        q.s += ex > 0.f ? ex * d : 0.f;
+                    }
+            }
+            q.z = wave_sum(q.z);
+            q.s = wave_sum(q.s);
+            if (lane == 0) s.red[1][wave] = q.z, s.red[2][wave] = q.s;
+            // alternatives: a lower bound of the last one's key, then everything from there on
+            if (top) {
+                u64 k = 0;
+#pragma unroll
+                for (int i = 0; i < VPT; i++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int c = b + 4 * (NT * i + (int)threadIdx.x) + e;
+                        if (c < c1) k = max64(k, lp_key(v[i].get(e), base + c));
+                    }
+                // the top-th largest of the wave's 64 lane maxima has that many keys of the wave at or above it
+                int r = 0;
+                for (int j = 0; j < WAVE; j++) r += __shfl(k, j, WAVE) > k;
+                const u64 nth = wave_max64(r == top - 1 ? k : 0);
+                if (lane == 0) s.thr[wave] = nth;
+                __syncthreads();
+                u64 thr = 1;
+#pragma unroll
+                for (int w = 0; w < NW; w++) thr = max64(thr, s.thr[w]);
+                if (have == top) thr = max64(thr, s.list[top - 1]);
+                if ((int)threadIdx.x < have) s.cand[threadIdx.x] = s.list[threadIdx.x];
+                if (k >= thr) {
+#pragma unroll
+                    for (int i = 0; i < VPT; i++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const int c = b + 4 * (NT * i + (int)threadIdx.x) + e;
+                            const u64 ke = lp_key(v[i].get(e), base + c);
+                            if (c < c1 && ke >= thr) {
+                                const int at = atomicAdd(&s.count, 1);
+                                if (at < CAP + MAX_TOP) s.cand[at] = ke;
+                            }
+                        }
+                }
+                __syncthreads();
+                const int n = s.count;
+                if (n <= CAP + MAX_TOP) {
+                    rank_keys(s.cand, n, s.list, top);
+                    have = min(top, n);
+                } else {
+                    // too many (values in order, or mostly alike): one after the other
+                    u64 last = ~0ull;
+                    const u64 mine = (int)threadIdx.x < have ? s.cand[threadIdx.x] : 0;
+                    for (int j = 0; j < top; j++) {
+                        u64 best = mine < last ? mine : 0;
+#pragma unroll
+                        for (int i = 0; i < VPT; i++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                const int c = b + 4 * (NT * i + (int)threadIdx.x) + e;
+                                const u64 ke = lp_key(v[i].get(e), base + c);
+                                if (c < c1 && ke < last) best = max64(best, ke);
+                            }
+                        best = wave_max64(best);
+                        __syncthreads();
+                        if (lane == 0) s.thr[wave] = best;
+                        __syncthreads();
+#pragma unroll
+                        for (int w = 0; w < NW; w++) best = max64(best, s.thr[w]);
+                        if (threadIdx.x == 0) s.list[j] = best;
+                        last = best;
+                    }
+                    have = top;
+                }
+            }
+            __syncthreads();
+            q.z = (s.red[1][0] + s.red[1][1]) + (s.red[1][2] + s.red[1][3]);
+            q.s = (s.red[2][0] + s.red[2][1]) + (s.red[2][2] + s.red[2][3]);
+            join(p, q);
         }
-        bad = __syncthreads_or(bad);
-        m = wave_max(m);
-        if (threadIdx.x % WAVE == 0) red[threadIdx.x / WAVE] = m;
+        if (all_splits == 1) {
+            if (threadIdx.x == 0) finish(o, t, V, p);
+            if ((int)threadIdx.x < top) finish_top(o, t, threadIdx.x, p, s.list[threadIdx.x]);
+        } else {
+            const size_t at = (size_t)t * all_splits + split0 + sp;
+            if (threadIdx.x == 0) parts[at] = p;
+            if ((int)threadIdx.x < top) tops[at * top + threadIdx.x] = (int)threadIdx.x < have ? s.list[threadIdx.x] : 0;
+        }
         __syncthreads();
-        m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-        const bool empty = m == -INFINITY;
-        float z = 0.f, s = 0.f;
-        if (!empty && !bad)
-            for (int i = threadIdx.x; i < V; i += 256) {
-                const float d = Act<T>::ld(x, i) - m, e = expf(d);
-                z += e;
-                if (e > 0.f) s = fmaf(e, d, s);
+    }
+}
+
+// One workgroup per row joins its splits: the sums in order, the alternatives of all of them in blocks of CAP keys.
+__global__ void __launch_bounds__(NT) logprobs_join_kernel(const Part* __restrict__ parts, const u64* __restrict__ tops,
+                                                           int rows, int V, int splits, const LogprobOut o) {
+    __shared__ Lds s;
+    for (int t = blockIdx.x; t < rows; t += gridDim.x) {
+        Part p = parts[(size_t)t * splits];
+        for (int i = 1; i < splits; i++) join(p, parts[(size_t)t * splits + i]);
+        if (threadIdx.x == 0) finish(o, t, V, p);
+        if (o.top) {
+            const u64* k = tops + (size_t)t * splits * o.top;
+            const int n = splits * o.top;
+            int have = 0;
+            for (int b = 0; b < n; b += CAP) {
+                const int m = min(CAP, n - b);
+                if ((int)threadIdx.x < have) s.cand[threadIdx.x] = s.list[threadIdx.x];
+                for (int i = threadIdx.x; i < m; i += NT) s.cand[have + i] = k[b + i];
+                __syncthreads();
+                if ((int)threadIdx.x < o.top) s.list[threadIdx.x] = 0;
+                __syncthreads();
+                rank_keys(s.cand, have + m, s.list, o.top);
+                have = o.top;
+                __syncthreads();
             }
-        z = block_sum(z, red);
-        s = block_sum(s, red);
-        const float lz = bad ? __builtin_nanf("") : logf(z);
-        if (threadIdx.x == 0) {
-            const int tok = o.tokens[t];
-            float lp = tok < 0 ? 0.f : __builtin_nanf("");
-            if (tok >= 0 && tok < V && !bad) lp = empty ? -INFINITY : Act<T>::ld(x, tok) - m - lz;
-            o.logprob[t] = lp;
-            o.entropy[t] = empty && !bad ? 0.f : lz - s / z;
-        }
-        uint64_t last = ~0ull;
-        for (int j = 0; j < o.top; j++) {
-            uint64_t k = 0;
-            for (int i = threadIdx.x; i < V; i += 256) {
-                const uint64_t ki = lp_key(Act<T>::ld(x, i), i);
-                if (ki < last && ki > k) k = ki;
-            }
-            for (int w = 32; w > 0; w >>= 1) {
-                const uint64_t k2 = __shfl_xor((unsigned long long)k, w, WAVE);
-                k = k2 > k ? k2 : k;
-            }
-            __syncthreads();
-            if (threadIdx.x % WAVE == 0) best[threadIdx.x / WAVE] = k;
-            __syncthreads();
-            for (int w = 0; w < 4; w++) k = best[w] > k ? best[w] : k;
-            if (threadIdx.x == 0) {
-                o.top_ids[(size_t)t * o.top + j] = (int)~(uint32_t)k;
-                o.top_logprobs[(size_t)t * o.top + j] =
-                    bad ? __builtin_nanf("") : empty ? -INFINITY : lp_key_value(k) - m - lz;
-            }
-            last = k;
+            if ((int)threadIdx.x < o.top) finish_top(o, t, threadIdx.x, p, s.list[threadIdx.x]);
         }
         __syncthreads();
     }
@@ -115,10 +315,45 @@ int check_out(const char* who, int T, int V, const LogprobOut& o) {
     return 0;
 }
 
-int run_logprobs(const void* L, int dtype, long long ld, int T, int V, const LogprobOut& o, hipStream_t st) {
-    const int grid = std::min(T, 1 << 20);
-    if (dtype == AEGIST_F32) logprobs_kernel<float><<<grid, 256, 0, st>>>((const float*)L, ld, T, V, o);
-    else logprobs_kernel<uint16_t><<<grid, 256, 0, st>>>((const uint16_t*)L, ld, T, V, o);
+// Logits of a split: few rows are cut so that about 1024 workgroups share them.
+int split_span(int T, int cols, int* small) {
+    const long long want = std::max(1LL, 1024LL / std::max(T, 1));
+    const int seg = 4 * 4 * NT;  // a segment of the small form
+    long long span = (cols + want - 1) / want;
+    *small = span <= 2 * seg;
+    const int unit = *small ? seg : 4 * seg;
+    return (int)std::min<long long>((span + unit - 1) / unit * unit, 1 << 30);
+}
+int split_count(int T, int cols) {
+    int small;
+    const int span = split_span(T, cols, &small);
+    return (cols + span - 1) / span;
+}
+
+// logits [T, cols] of the tokens base .. base + cols - 1, as splits split0 .. of all_splits
+int run_splits(const void* L, int dtype, long long ld, int T, int cols, int base, int V, int split0, int all_splits, void* ws,
+               const LogprobOut& o, hipStream_t st) {
+    int small;
+    const int span = split_span(T, cols, &small), splits = (cols + span - 1) / span;
+    Part* parts = (Part*)ws;
+    u64* tops = (u64*)(parts + (size_t)T * all_splits);
+    const int grid = (int)std::min<long long>((long long)T * splits, 1 << 20);
+#define AEG_LP(TY, VPT) \
+    logprobs_kernel<TY, VPT><<<grid, NT, 0, st>>>((const TY*)L, ld, T, cols, base, V, span, split0, splits, all_splits, parts, tops, o)
+    if (dtype == AEGIST_F32) {
+        if (small) AEG_LP(float, 4);
+        else AEG_LP(float, 16);
+    } else {
+        if (small) AEG_LP(uint16_t, 4);
+        else AEG_LP(uint16_t, 16);
+    }
+#undef AEG_LP
+    return after_launch("token_logprobs");
+}
+
+int run_join(int T, int V, int splits, const void* ws, const LogprobOut& o, hipStream_t st) {
+    const Part* parts = (const Part*)ws;
+    logprobs_join_kernel<<<std::min(T, 1 << 20), NT, 0, st>>>(parts, (const u64*)(parts + (size_t)T * splits), T, V, splits, o);
     return after_launch("token_logprobs");
 }
 
@@ -129,7 +364,11 @@ size_t head_logits_bytes(int T, int V) { return ((size_t)head_rows(T, V) * V * 4
 
 }  // namespace
 
-extern "C" size_t aegist_token_logprobs_workspace_bytes(int T, int V, int top) { return 0; }
+extern "C" size_t aegist_token_logprobs_workspace_bytes(int T, int V, int top) {
+    if (T < 1 || V < 1 || top < 0 || top > MAX_TOP) return 0;
+    const int n = split_count(T, V);
+    return n > 1 ? parts_bytes(T, n, top) : 0;
+}
 
 extern "C" int aegist_token_logprobs(const void* logits, int dtype, long long ld, const int* tokens, float* logprob,
                                      float* entropy, int* top_ids, float* top_logprobs, int T, int V, int top, void* ws,
@@ -141,12 +380,19 @@ extern "C" int aegist_token_logprobs(const void* logits, int dtype, long long ld
         return fail(AEGIST_ERR_DTYPE, "token_logprobs: logits must be AEGIST_F32 or AEGIST_BF16");
     if (T == 0) return 0;
     if (!logits || ld < V) return fail(AEGIST_ERR_SHAPE, "token_logprobs: null logits, or ld < V");
-    return run_logprobs(logits, dtype, ld, T, V, o, AEG_STREAM(stream));
+    rc = check_workspace(ws, ws_bytes, aegist_token_logprobs_workspace_bytes(T, V, top), "token_logprobs");
+    if (rc) return rc;
+    const hipStream_t st = AEG_STREAM(stream);
+    const int n = split_count(T, V);
+    rc = run_splits(logits, dtype, ld, T, V, 0, V, 0, n, ws, o, st);
+    return rc || n == 1 ? rc : run_join(T, V, n, ws, o, st);
 }
 
 extern "C" size_t aegist_head_logprobs_workspace_bytes(int x_dtype, int w_dtype, int T, int V, int K, int group, int top) {
     if (T < 1 || V < 1 || K < 1) return 0;
-    return head_logits_bytes(T, V) + (w_dtype == AEGIST_Q4 ? aegist_linear_q4_workspace_bytes(x_dtype, head_rows(T, V), V, K, group) : 0);
+    const int rows = head_rows(T, V);
+    return head_logits_bytes(T, V) + aegist_token_logprobs_workspace_bytes(rows, V, top) +
+           (w_dtype == AEGIST_Q4 ? aegist_linear_q4_workspace_bytes(x_dtype, rows, V, K, group) : 0);
 }
 
 extern "C" int aegist_head_logprobs(const void* X, int x_dtype, long long ldx, const void* W, int w_dtype,
@@ -168,18 +414,20 @@ extern "C" int aegist_head_logprobs(const void* X, int x_dtype, long long ldx, c
     if (rc) return rc;
     const hipStream_t st = AEG_STREAM(stream);
     const int block = head_rows(T, V), xs = x_dtype == AEGIST_F32 ? 4 : 2;
-    const size_t lb = head_logits_bytes(T, V);
+    const size_t lb = head_logits_bytes(T, V), pb = aegist_token_logprobs_workspace_bytes(block, V, top);
     float* logits = (float*)ws;
+    char *pws = (char*)ws + lb, *lws = pws + pb;
     for (int t = 0; t < T; t += block) {
         const int m = std::min(block, T - t);
         const void* x = (const char*)X + (size_t)t * ldx * xs;
-        rc = w_dtype == AEGIST_Q4 ? launch_linear_q4(x, x_dtype, ldx, W, logits, V, m, V, K, group, 0, (char*)ws + lb,
-                                                     ws_bytes - lb, st)
+        rc = w_dtype == AEGIST_Q4 ? launch_linear_q4(x, x_dtype, ldx, W, logits, V, m, V, K, group, 0, lws, ws_bytes - lb - pb, st)
                                   : launch_proj(x, x_dtype, ldx, W, w_dtype, scale, logits, V, m, V, K, 0, st);
         if (rc) return rc;
         const LogprobOut part{tokens + t, logprob + t, entropy + t, top_ids ? top_ids + (size_t)t * top : nullptr,
                               top_logprobs ? top_logprobs + (size_t)t * top : nullptr, top};
-        if ((rc = run_logprobs(logits, AEGIST_F32, V, m, V, part, st))) return rc;
+        const int n = split_count(m, V);
+        if ((rc = run_splits(logits, AEGIST_F32, V, m, V, 0, V, 0, n, pws, part, st))) return rc;
+        if (n > 1 && (rc = run_join(m, V, n, pws, part, st))) return rc;
     }
     return 0;
 }
