@@ -114,24 +114,105 @@ template <> struct L4<uint16_t> {
 
 struct Lds {
     float red[3][NW];
-    int flag[NW];
+    Part part[NW];
     u64 thr[NW];
     int count;
-    u64 cand[CAP + MAX_TOP];   // candidates of a segment, after the alternatives so far
-    u64 list[MAX_TOP];
+    u64 cand[CAP + MAX_TOP];   // candidates, after the alternatives so far
+    u64 list[MAX_TOP];         // the alternatives so far, descending
 };
 
-// the `top` largest of n <= CAP + MAX_TOP keys (all different, or 0) into list, descending
-__device__ __forceinline__ void rank_keys(const u64* cand, int n, u64* list, int top) {
+__device__ __forceinline__ float lane_value(float v, int j) {
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), j));
+}
+
+// The `top`-th largest of the wave's 64 values; so many of the wave's logits, where a lane's is the largest of its
+// own, are at or above it.
+__device__ __forceinline__ float nth_value(float v, int top) {
+    int r = 0;
+#pragma unroll 16
+    for (int j = 0; j < WAVE; j++) r += lane_value(v, j) > v;
+    return -wave_max(r < top ? -v : -INFINITY);
+}
+// The same of 64 different keys, or 0 for lanes without one; 0 if there are too few.
+__device__ __forceinline__ u64 nth_key(u64 k, int top) {
+    int r = 0;
+#pragma unroll 8
+    for (int j = 0; j < WAVE; j++)
+        r += ((u64)(uint32_t)__builtin_amdgcn_readlane((int)(k >> 32), j) << 32 |
+              (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)k, j)) > k;
+    return wave_max64(r == top - 1 ? k : 0);
+}
+
+__device__ __forceinline__ void add_candidate(Lds& s, u64 k) {
+    const int at = atomicAdd(&s.count, 1);  // (their order does not matter: they are ranked)
+    if (at < CAP + MAX_TOP) s.cand[at] = k;
+}
+
+// the `top` largest of n <= CAP + MAX_TOP keys (all different, or 0) into the list, descending
+__device__ __forceinline__ void rank_keys(Lds& s, int n, int top) {
     for (int i = threadIdx.x; i < n; i += NT) {
-        const u64 k = cand[i];
+        const u64 k = s.cand[i];
         int r = 0;
-        for (int j = 0; j < n; j++) r += cand[j] > k;
-        if (r < top && k) list[r] = k;
+#pragma unroll 8
+        for (int j = 0; j < n; j++) r += s.cand[j] > k;
+        if (r < top && k) s.list[r] = k;
     }
 }
 
-// A workgroup's splits: rows x splits items, each `span` logits (the last fewer) in segments of 4 VPT NT. `base` is
+// The `top` largest of the list's `have` keys and the N keys that each thread gives (0: none), into the list. All
+// threads call it; returns how many there are. Keys are different, so from the largest bound that the waves' lanes
+// give there are few to rank; where they are not (values in order), the largest is taken one after the other.
+template <int N, typename Key>
+__device__ __forceinline__ int select_keys(Lds& s, int have, int top, Key key) {
+    const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE;
+    u64 k = 0;
+#pragma unroll
+    for (int i = 0; i < N; i++) k = max64(k, key(i));
+    const u64 nth = nth_key(k, top);
+    __syncthreads();
+    if (lane == 0) s.thr[wave] = nth;
+    if ((int)threadIdx.x < have) s.cand[threadIdx.x] = s.list[threadIdx.x];
+    if (threadIdx.x == 0) s.count = have;
+    __syncthreads();
+    u64 thr = have == top ? max64(s.list[top - 1], 1) : 1;
+#pragma unroll
+    for (int w = 0; w < NW; w++) thr = max64(thr, s.thr[w]);
+    if (k >= thr) {
+#pragma unroll
+        for (int i = 0; i < N; i++)
+            if (key(i) >= thr) add_candidate(s, key(i));
+    }
+    __syncthreads();
+    const int n = s.count;
+    if (n <= CAP + MAX_TOP) {
+        rank_keys(s, n, top);
+        have = min(top, n);
+    } else {
+        u64 last = ~0ull;
+        const u64 mine = (int)threadIdx.x < have ? s.cand[threadIdx.x] : 0;
+        for (int j = 0; j < top; j++) {
+            u64 best = mine < last ? mine : 0;
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                const u64 ki = key(i);
+                if (ki < last) best = max64(best, ki);
+            }
+            best = wave_max64(best);
+            __syncthreads();
+            if (lane == 0) s.thr[wave] = best;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < NW; w++) best = max64(best, s.thr[w]);
+            if (threadIdx.x == 0) s.list[j] = best;
+            last = best;
+        }
+        have = top;
+    }
+    __syncthreads();
+    return have;
+}
+
+// A workgroup's items: rows x splits, each `span` logits (the last fewer) in segments of 4 VPT NT. `base` is
 // the first token of these logits, V the whole vocabulary's. With one split the outputs are written here.
 template <typename T, int VPT>
 __global__ void __launch_bounds__(NT) logprobs_kernel(const T* __restrict__ L, long long ld, int rows, int cols, int base,
@@ -140,6 +221,7 @@ __global__ void __launch_bounds__(NT) logprobs_kernel(const T* __restrict__ L, l
     __shared__ Lds s;
     const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE, top = o.top;
     constexpr int SEG = 4 * VPT * NT;
+    constexpr float LOG2E = 1.44269504f, LN2 = 0.693147181f;
     for (long long item = blockIdx.x; item < (long long)rows * splits; item += gridDim.x) {
         const int t = (int)(item / splits), sp = (int)(item % splits);
         const int c0 = sp * span, c1 = min(cols, c0 + span);
@@ -150,117 +232,97 @@ __global__ void __launch_bounds__(NT) logprobs_kernel(const T* __restrict__ L, l
         int have = 0;  // alternatives so far (the same in all threads)
         for (int b = c0; b < c1; b += SEG) {
             L4<T> v[VPT];
-            // thread's logits: b + 4 (NT i + thread) ..
+            // the thread's logits: b + 4 (NT i + thread) ..
+            const int c = b + 4 * (int)threadIdx.x;
+            if (b + SEG <= c1) {
 #pragma unroll
-            for (int i = 0; i < VPT; i++) {
-                const int c = b + 4 * (NT * i + (int)threadIdx.x);
-                if (c + 4 <= c1) {
-                    v[i].load(x + c);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; e++) v[i].set(e, c + e < c1 ? Act<T>::ld(x, c + e) : -INFINITY);
-                }
-            }
-            float m = -INFINITY;
-            bool bad = false;
-#pragma unroll
-            for (int i = 0; i < VPT; i++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float f = v[i].get(e);
-                    m = fmaxf(m, f);
-                    bad |= !(f < INFINITY);
-                }
-            m = wave_max(m);
-            const bool wbad = __any(bad);
-            __syncthreads();
-            if (lane == 0) s.red[0][wave] = m, s.flag[wave] = wbad;
-            if (threadIdx.x == 0) s.count = have;
-            __syncthreads();
-#pragma unroll
-            for (int w = 0; w < NW; w++) m = fmaxf(m, s.red[0][w]);
-            Part q{m, 0.f, 0.f, -INFINITY, s.flag[0] | s.flag[1] | s.flag[2] | s.flag[3], {}};
-            if (m > -INFINITY && !q.bad) {
+                for (int i = 0; i < VPT; i++) v[i].load(x + c + 4 * NT * i);
+            } else {
 #pragma unroll
                 for (int i = 0; i < VPT; i++)
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        const float d = v[i].get(e) - m, ex = __expf(d);
-                        q.z += ex;
-                        q.s += ex > 0.f ? ex * d : 0.f;
+                        const int ce = c + 4 * NT * i + e;
+                        v[i].set(e, ce < c1 ? Act<T>::ld(x, ce) : -INFINITY);
                     }
+            }
+            float mt = -INFINITY;  // the thread's largest (NaN apart)
+#pragma unroll
+            for (int i = 0; i < VPT; i++)
+                mt = fmaxf(fmaxf(fmaxf(mt, v[i].get(0)), fmaxf(v[i].get(1), v[i].get(2))), v[i].get(3));
+            const float mw = wave_max(mt);
+            // the alternatives' lower bound: from the first segment's lanes, then from the list
+            const float nth = top && have < top ? nth_value(mt, top) : 0.f;
+            if (lane == 0) {
+                s.red[0][wave] = mw;
+                s.thr[wave] = __float_as_uint(nth);
+            }
+            if (threadIdx.x == 0) s.count = have;
+            __syncthreads();
+            const float m = fmaxf(fmaxf(s.red[0][0], s.red[0][1]), fmaxf(s.red[0][2], s.red[0][3]));
+            // e^(x - m) = 2^y. The entropy's y is held at -200, so that a masked logit's term is 0, not 0 times -inf;
+            // NaN reaches z.
+            const float mz = m > -INFINITY ? m : 0.f;
+            Part q{m, 0.f, 0.f, -INFINITY, m == INFINITY, {}};
+            if (m < INFINITY) {
+                float z[2] = {0.f, 0.f}, y2[2] = {0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < VPT; i++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const float y = (v[i].get(e) - mz) * LOG2E, ex = __builtin_amdgcn_exp2f(y);
+                        z[e % 2] += ex;
+                        y2[e % 2] = __builtin_fmaf(ex, fmaxf(y, -200.f), y2[e % 2]);
+                    }
+                q.z = z[0] + z[1];
+                q.s = (y2[0] + y2[1]) * LN2;
             }
             q.z = wave_sum(q.z);
             q.s = wave_sum(q.s);
             if (lane == 0) s.red[1][wave] = q.z, s.red[2][wave] = q.s;
-            // alternatives: a lower bound of the last one's key, then everything from there on
+            bool few = true;
             if (top) {
-                u64 k = 0;
+                float thr = -INFINITY;
+                if (have == top) {
+                    thr = lp_key_value(s.list[top - 1]);  // (NaN: nothing is above it)
+                } else {
 #pragma unroll
-                for (int i = 0; i < VPT; i++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const int c = b + 4 * (NT * i + (int)threadIdx.x) + e;
-                        if (c < c1) k = max64(k, lp_key(v[i].get(e), base + c));
-                    }
-                // the top-th largest of the wave's 64 lane maxima has that many keys of the wave at or above it
-                int r = 0;
-                for (int j = 0; j < WAVE; j++) r += __shfl(k, j, WAVE) > k;
-                const u64 nth = wave_max64(r == top - 1 ? k : 0);
-                if (lane == 0) s.thr[wave] = nth;
-                __syncthreads();
-                u64 thr = 1;
-#pragma unroll
-                for (int w = 0; w < NW; w++) thr = max64(thr, s.thr[w]);
-                if (have == top) thr = max64(thr, s.list[top - 1]);
+                    for (int w = 0; w < NW; w++) thr = fmaxf(thr, __uint_as_float((uint32_t)s.thr[w]));
+                }
+                // later tokens lose ties with the list's
+                const bool strict = have == top;
                 if ((int)threadIdx.x < have) s.cand[threadIdx.x] = s.list[threadIdx.x];
-                if (k >= thr) {
+                if (strict ? mt > thr : mt >= thr) {
 #pragma unroll
                     for (int i = 0; i < VPT; i++)
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
-                            const int c = b + 4 * (NT * i + (int)threadIdx.x) + e;
-                            const u64 ke = lp_key(v[i].get(e), base + c);
-                            if (c < c1 && ke >= thr) {
-                                const int at = atomicAdd(&s.count, 1);
-                                if (at < CAP + MAX_TOP) s.cand[at] = ke;
+                            const float f = v[i].get(e);
+                            if (strict ? f > thr : f >= thr) {
+                                const int ce = c + 4 * NT * i + e;
+                                if (ce < c1) add_candidate(s, lp_key(f, base + ce));
                             }
                         }
-                }
-                __syncthreads();
-                const int n = s.count;
-                if (n <= CAP + MAX_TOP) {
-                    rank_keys(s.cand, n, s.list, top);
-                    have = min(top, n);
-                } else {
-                    // too many (values in order, or mostly alike): one after the other
-                    u64 last = ~0ull;
-                    const u64 mine = (int)threadIdx.x < have ? s.cand[threadIdx.x] : 0;
-                    for (int j = 0; j < top; j++) {
-                        u64 best = mine < last ? mine : 0;
-#pragma unroll
-                        for (int i = 0; i < VPT; i++)
-#pragma unroll
-                            for (int e = 0; e < 4; e++) {
-                                const int c = b + 4 * (NT * i + (int)threadIdx.x) + e;
-                                const u64 ke = lp_key(v[i].get(e), base + c);
-                                if (c < c1 && ke < last) best = max64(best, ke);
-                            }
-                        best = wave_max64(best);
-                        __syncthreads();
-                        if (lane == 0) s.thr[wave] = best;
-                        __syncthreads();
-#pragma unroll
-                        for (int w = 0; w < NW; w++) best = max64(best, s.thr[w]);
-                        if (threadIdx.x == 0) s.list[j] = best;
-                        last = best;
-                    }
-                    have = top;
                 }
             }
             __syncthreads();
             q.z = (s.red[1][0] + s.red[1][1]) + (s.red[1][2] + s.red[1][3]);
             q.s = (s.red[2][0] + s.red[2][1]) + (s.red[2][2] + s.red[2][3]);
+            if (!(q.z < INFINITY)) q.bad = 1;
+            if (top) {
+                const int n = s.count;
+                few = n <= CAP + MAX_TOP && !q.bad;  // (NaN comes first, and no float comparison finds it)
+                if (few) {
+                    if (n > have) rank_keys(s, n, top);
+                    have = min(top, n);
+                } else {
+                    have = select_keys<4 * VPT>(s, have, top, [&](int i) {
+                        const int ce = c + 4 * NT * (i / 4) + i % 4;
+                        return ce < c1 ? lp_key(v[i / 4].get(i % 4), base + ce) : 0;
+                    });
+                }
+            }
+            __syncthreads();
             join(p, q);
         }
         if (all_splits == 1) {
@@ -275,28 +337,48 @@ __global__ void __launch_bounds__(NT) logprobs_kernel(const T* __restrict__ L, l
     }
 }
 
-// One workgroup per row joins its splits: the sums in order, the alternatives of all of them in blocks of CAP keys.
+__device__ __forceinline__ Part shfl_part(const Part& p, int o) {
+    return Part{__shfl_xor(p.m, o, WAVE), __shfl_xor(p.z, o, WAVE), __shfl_xor(p.s, o, WAVE), __shfl_xor(p.tok, o, WAVE),
+                __shfl_xor(p.bad, o, WAVE), {}};
+}
+
+// One workgroup per row joins its splits: each thread's in order, then the lanes' and the waves' in a fixed tree.
 __global__ void __launch_bounds__(NT) logprobs_join_kernel(const Part* __restrict__ parts, const u64* __restrict__ tops,
                                                            int rows, int V, int splits, const LogprobOut o) {
     __shared__ Lds s;
+    constexpr int N = 4;
+    const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE;
     for (int t = blockIdx.x; t < rows; t += gridDim.x) {
-        Part p = parts[(size_t)t * splits];
-        for (int i = 1; i < splits; i++) join(p, parts[(size_t)t * splits + i]);
+        const u64* keys = tops + (size_t)t * splits * o.top;
+        const int n = splits * o.top;
+        u64 k[N];  // the first block's, requested with the parts
+#pragma unroll
+        for (int i = 0; i < N; i++) k[i] = (int)threadIdx.x + NT * i < n ? keys[threadIdx.x + NT * i] : 0;
+        Part p{-INFINITY, 0.f, 0.f, -INFINITY, 0, {}};
+        for (int i = threadIdx.x; i < splits; i += NT) join(p, parts[(size_t)t * splits + i]);
+#pragma unroll
+        for (int w = 1; w < WAVE; w *= 2) {
+            const Part b = shfl_part(p, w);
+            Part lo = lane & w ? b : p;  // (the lower lane's first, so that all lanes have the same bits)
+            join(lo, lane & w ? p : b);
+            p = lo;
+        }
+        if (lane == 0) s.part[wave] = p;
+        __syncthreads();
+        p = s.part[0];
+        if (splits > WAVE) {
+#pragma unroll
+            for (int w = 1; w < NW; w++) join(p, s.part[w]);
+        }
         if (threadIdx.x == 0) finish(o, t, V, p);
         if (o.top) {
-            const u64* k = tops + (size_t)t * splits * o.top;
-            const int n = splits * o.top;
             int have = 0;
-            for (int b = 0; b < n; b += CAP) {
-                const int m = min(CAP, n - b);
-                if ((int)threadIdx.x < have) s.cand[threadIdx.x] = s.list[threadIdx.x];
-                for (int i = threadIdx.x; i < m; i += NT) s.cand[have + i] = k[b + i];
-                __syncthreads();
-                if ((int)threadIdx.x < o.top) s.list[threadIdx.x] = 0;
-                __syncthreads();
-                rank_keys(s.cand, have + m, s.list, o.top);
-                have = o.top;
-                __syncthreads();
+            for (int b = 0; b < n; b += N * NT) {
+                if (b > 0) {
+#pragma unroll
+                    for (int i = 0; i < N; i++) k[i] = b + (int)threadIdx.x + NT * i < n ? keys[b + threadIdx.x + NT * i] : 0;
+                }
+                have = select_keys<N>(s, have, o.top, [&](int i) { return k[i]; });
             }
             if ((int)threadIdx.x < o.top) finish_top(o, t, threadIdx.x, p, s.list[threadIdx.x]);
         }
