@@ -10,6 +10,7 @@ provider here: no op computes anything in torch.
 """
 from __future__ import annotations
 
+import functools
 from typing import NamedTuple
 
 import torch
@@ -430,7 +431,8 @@ def gemv_bf16(x, weight, y=None):
 
 def _call_on(device, name: str, *args):
     """call() on the current stream of `device`, which need not be the current device."""
-    if device.index is None or device.index == torch.cuda.current_device():
+    index = device.index
+    if index is None or index == torch.cuda.current_device():
         call(name, *args, _stream(device))
     else:
         with torch.cuda.device(device):
@@ -446,23 +448,29 @@ def _one_device(*ts):
     return dev
 
 
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(name: str, *sizes) -> int:
+    """A *_workspace_bytes query, asked once per sizes."""
+    return getattr(lib(), name)(*sizes)
+
+
 def _scratch(nbytes: int, device):
-    """Workspace of one call: (pointer, bytes, tensor). From torch's allocator, which orders its reuse on the
+    """Workspace of one call (None if it needs none). From torch's allocator, which orders its reuse on the
     stream and gives a captured graph memory of its own."""
-    if nbytes == 0:
-        return None, 0, None
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    return ws.data_ptr(), nbytes, ws
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
 def _rows(x, what: str):
-    """x [..., K] as [M, K] with contiguous, 16-byte aligned rows."""
+    """x [..., K] as [M, K] with contiguous rows, and its row stride."""
     if x.dim() < 1 or x.shape[-1] == 0:
         raise AegistError("shape", -1, f"{what} needs a last dimension")
-    x2 = x.reshape(-1, x.shape[-1])
-    if x2.stride(1) != 1:
+    if x.dim() != 2:
+        x = x.reshape(-1, x.shape[-1])
+    M, K = x.shape
+    ld, one = x.stride()
+    if one != 1 and K > 1:
         raise AegistError("layout", -1, f"{what} rows must be contiguous")
-    return x2, x2.stride(0) if x2.shape[0] > 1 else -(-x2.shape[1] // 8) * 8
+    return x, ld if M > 1 else -(-K // 8) * 8
 
 
 class Q4Weight:
@@ -535,21 +543,27 @@ def linear_q4(x, weight: Q4Weight, out=None, accumulate: bool = False):
     x [..., K] fp32 or bf16 (rows contiguous, 16-byte aligned); out fp32 [..., N], contiguous (allocated if
     None; with accumulate the product is added into it)."""
     N, K = weight.shape
+    w, group = weight.data, weight.group
     x2, ldx = _rows(x, "x")
+    M = x2.shape[0]
     if x2.shape[1] != K:
         raise AegistError("shape", -1, f"weight [{N}, {K}] does not match x [..., {x2.shape[1]}]")
-    M = x2.shape[0]
+    dev = _one_device(x2, w, out)
     if out is None:
         if accumulate:
             raise AegistError("shape", -1, "accumulate needs out")
-        out = torch.empty(*x.shape[:-1], N, dtype=torch.float32, device=x.device)
-    _need_contig(out)
-    if out.dtype != torch.float32 or out.numel() != M * N:
-        raise AegistError("shape", -1, "out must be fp32 [..., N]")
-    dev = _one_device(x2, weight.data, out)
-    px, pw, po, dt = _p(x2), _p(weight.data), _p(out), _dt(x2)
-    wp, wn, ws = _scratch(lib().aegist_linear_q4_workspace_bytes(dt, M, N, K, weight.group), dev)
-    _call_on(dev, "aegist_linear_q4", px, dt, ldx, pw, po, N, M, N, K, weight.group, int(accumulate), wp, wn)
+        out = torch.empty(*x.shape[:-1], N, dtype=torch.float32, device=dev)
+        po = out.data_ptr()
+    else:
+        _need_contig(out)
+        if out.dtype != torch.float32 or out.numel() != M * N:
+            raise AegistError("shape", -1, "out must be fp32 [..., N]")
+        po = _p(out)
+    px, pw, dt = _p(x2), _p(w), _dt(x2)
+    need = _workspace_bytes("aegist_linear_q4_workspace_bytes", dt, M, N, K, group)
+    ws = _scratch(need, dev)
+    _call_on(dev, "aegist_linear_q4", px, dt, ldx, pw, po, N, M, N, K, group, int(accumulate),
+             None if ws is None else ws.data_ptr(), need)
     return out
 
 
@@ -565,13 +579,16 @@ class TokenLogprobs(NamedTuple):
 def _logprob_outputs(lead, tokens, top: int, device):
     if tokens.dtype != torch.int32:
         raise AegistError("dtype", -3, "tokens must be int32")
-    if tuple(tokens.shape) != tuple(lead):
+    if tokens.shape != lead:
         raise AegistError("shape", -1, f"tokens {tuple(tokens.shape)} for rows {tuple(lead)}")
     _need_contig(tokens)
-    both = torch.empty(2, *lead, dtype=torch.float32, device=device)
-    ids = torch.empty(*lead, top, dtype=torch.int32, device=device) if top > 0 else None
-    lps = torch.empty(*lead, top, dtype=torch.float32, device=device) if top > 0 else None
-    return TokenLogprobs(both[0], both[1], ids, lps)
+    if top <= 0:
+        return TokenLogprobs(torch.empty(lead, dtype=torch.float32, device=device),
+                             torch.empty(lead, dtype=torch.float32, device=device), None, None)
+    return TokenLogprobs(torch.empty(lead, dtype=torch.float32, device=device),
+                         torch.empty(lead, dtype=torch.float32, device=device),
+                         torch.empty(*lead, top, dtype=torch.int32, device=device),
+                         torch.empty(*lead, top, dtype=torch.float32, device=device))
 
 
 def token_logprobs(logits, tokens, top: int = 0) -> TokenLogprobs:
@@ -581,19 +598,16 @@ def token_logprobs(logits, tokens, top: int = 0) -> TokenLogprobs:
     (0 to 64) most probable tokens in descending order, ties to the lower token. A negative token (padding)
     has logprob 0, one past the vocabulary NaN. Logits of -inf have no probability; a row of nothing else has
     logprob -inf and entropy 0, a row with NaN or +inf NaN."""
-    if logits.dim() < 1 or logits.shape[-1] == 0:
-        raise AegistError("shape", -1, "logits need a vocabulary")
-    V = logits.shape[-1]
-    x = logits.reshape(-1, V)
-    if V > 1 and x.stride(1) != 1:
-        raise AegistError("layout", -1, "logits rows must be contiguous")
-    T = x.shape[0]
+    x, ld = _rows(logits, "logits")
+    T, V = x.shape
     dev = _one_device(x, tokens)
     px, pt, dt = _p(x), _p(tokens), _dt(x)
     r = _logprob_outputs(logits.shape[:-1], tokens, top, dev)
-    wp, wn, ws = _scratch(lib().aegist_token_logprobs_workspace_bytes(T, V, top), dev)
-    _call_on(dev, "aegist_token_logprobs", px, dt, x.stride(0) if T > 1 else V, pt, r.logprob.data_ptr(),
-             r.entropy.data_ptr(), _p(r.top_ids), _p(r.top_logprobs), T, V, top, wp, wn)
+    need = _workspace_bytes("aegist_token_logprobs_workspace_bytes", T, V, top)
+    ws = _scratch(need, dev)
+    _call_on(dev, "aegist_token_logprobs", px, dt, ld, pt, r.logprob.data_ptr(), r.entropy.data_ptr(),
+             r.top_ids.data_ptr() if top > 0 else None, r.top_logprobs.data_ptr() if top > 0 else None, T, V, top,
+             None if ws is None else ws.data_ptr(), need)
     return r
 
 
@@ -623,9 +637,11 @@ def head_logprobs(x, weight, tokens, top: int = 0, scale=None) -> TokenLogprobs:
     dev = _one_device(x2, w, tokens, scale)
     px, pw, pt, ps, dt = _p(x2), _p(w), _p(tokens), _p(scale), _dt(x2)
     r = _logprob_outputs(x.shape[:-1], tokens, top, dev)
-    wp, wn, ws = _scratch(lib().aegist_head_logprobs_workspace_bytes(dt, wdt, T, V, K, group, top), dev)
+    need = _workspace_bytes("aegist_head_logprobs_workspace_bytes", dt, wdt, T, V, K, group, top)
+    ws = _scratch(need, dev)
     _call_on(dev, "aegist_head_logprobs", px, dt, ldx, pw, wdt, ps, pt, r.logprob.data_ptr(), r.entropy.data_ptr(),
-             _p(r.top_ids), _p(r.top_logprobs), T, V, K, group, top, wp, wn)
+             r.top_ids.data_ptr() if top > 0 else None, r.top_logprobs.data_ptr() if top > 0 else None, T, V, K, group,
+             top, None if ws is None else ws.data_ptr(), need)
     return r
 
 

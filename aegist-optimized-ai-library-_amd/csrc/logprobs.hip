@@ -162,11 +162,11 @@ __device__ __forceinline__ void rank_keys(Lds& s, int n, int top) {
 // The `top` largest of the list's `have` keys and the N keys that each thread gives (0: none), into the list. All
 // threads call it; returns how many there are. Keys are different, so from the largest bound that the waves' lanes
 // give there are few to rank; where they are not (values in order), the largest is taken one after the other.
-template <int N, typename Key>
+template <int N, int UNROLL, typename Key>
 __device__ __forceinline__ int select_keys(Lds& s, int have, int top, Key key) {
     const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE;
     u64 k = 0;
-#pragma unroll
+#pragma unroll UNROLL
     for (int i = 0; i < N; i++) k = max64(k, key(i));
     const u64 nth = nth_key(k, top);
     __syncthreads();
@@ -178,9 +178,11 @@ __device__ __forceinline__ int select_keys(Lds& s, int have, int top, Key key) {
 #pragma unroll
     for (int w = 0; w < NW; w++) thr = max64(thr, s.thr[w]);
     if (k >= thr) {
-#pragma unroll
-        for (int i = 0; i < N; i++)
-            if (key(i) >= thr) add_candidate(s, key(i));
+#pragma unroll UNROLL
+        for (int i = 0; i < N; i++) {
+            const u64 ki = key(i);
+            if (ki >= thr) add_candidate(s, ki);
+        }
     }
     __syncthreads();
     const int n = s.count;
@@ -192,7 +194,7 @@ __device__ __forceinline__ int select_keys(Lds& s, int have, int top, Key key) {
         const u64 mine = (int)threadIdx.x < have ? s.cand[threadIdx.x] : 0;
         for (int j = 0; j < top; j++) {
             u64 best = mine < last ? mine : 0;
-#pragma unroll
+#pragma unroll UNROLL
             for (int i = 0; i < N; i++) {
                 const u64 ki = key(i);
                 if (ki < last) best = max64(best, ki);
@@ -228,7 +230,6 @@ __global__ void __launch_bounds__(NT) logprobs_kernel(const T* __restrict__ L, l
         const T* x = L + (size_t)t * ld;
         const int tok = o.tokens[t] - base;
         Part p{-INFINITY, 0.f, 0.f, -INFINITY, 0, {}};
-        if (tok >= c0 && tok < c1) p.tok = Act<T>::ld(x, tok);
         int have = 0;  // alternatives so far (the same in all threads)
         for (int b = c0; b < c1; b += SEG) {
             L4<T> v[VPT];
@@ -289,9 +290,16 @@ __global__ void __launch_bounds__(NT) logprobs_kernel(const T* __restrict__ L, l
 #pragma unroll
                     for (int w = 0; w < NW; w++) thr = fmaxf(thr, __uint_as_float((uint32_t)s.thr[w]));
                 }
-                // later tokens lose ties with the list's
-                const bool strict = have == top;
+                // later tokens lose ties with the list's. Where fewer logits than asked for are not masked, those are
+                // all of them and masked ones of the lowest tokens: of the first 2 top, at least top are
+                const bool masked = have < top && thr == -INFINITY, strict = have == top || masked;
                 if ((int)threadIdx.x < have) s.cand[threadIdx.x] = s.list[threadIdx.x];
+                if (masked) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        if (4 * (int)threadIdx.x + e < 2 * top && c + e < c1 && v[0].get(e) == -INFINITY)
+                            add_candidate(s, lp_key(-INFINITY, base + c + e));
+                }
                 if (strict ? mt > thr : mt >= thr) {
 #pragma unroll
                     for (int i = 0; i < VPT; i++)
@@ -316,15 +324,17 @@ __global__ void __launch_bounds__(NT) logprobs_kernel(const T* __restrict__ L, l
                     if (n > have) rank_keys(s, n, top);
                     have = min(top, n);
                 } else {
-                    have = select_keys<4 * VPT>(s, have, top, [&](int i) {
+                    // (read again: keys of a whole segment would take two registers per logit)
+                    have = select_keys<4 * VPT, 1>(s, have, top, [&](int i) {
                         const int ce = c + 4 * NT * (i / 4) + i % 4;
-                        return ce < c1 ? lp_key(v[i / 4].get(i % 4), base + ce) : 0;
+                        return ce < c1 ? lp_key(Act<T>::ld(x, ce), base + ce) : 0;
                     });
                 }
             }
             __syncthreads();
             join(p, q);
         }
+        if (tok >= c0 && tok < c1) p.tok = Act<T>::ld(x, tok);
         if (all_splits == 1) {
             if (threadIdx.x == 0) finish(o, t, V, p);
             if ((int)threadIdx.x < top) finish_top(o, t, threadIdx.x, p, s.list[threadIdx.x]);
@@ -337,12 +347,7 @@ __global__ void __launch_bounds__(NT) logprobs_kernel(const T* __restrict__ L, l
     }
 }
 
-__device__ __forceinline__ Part shfl_part(const Part& p, int o) {
-    return Part{__shfl_xor(p.m, o, WAVE), __shfl_xor(p.z, o, WAVE), __shfl_xor(p.s, o, WAVE), __shfl_xor(p.tok, o, WAVE),
-                __shfl_xor(p.bad, o, WAVE), {}};
-}
-
-// One workgroup per row joins its splits: each thread's in order, then the lanes' and the waves' in a fixed tree.
+// One workgroup per row joins its splits: each thread's in order, then all lanes' in a fixed tree.
 __global__ void __launch_bounds__(NT) logprobs_join_kernel(const Part* __restrict__ parts, const u64* __restrict__ tops,
                                                            int rows, int V, int splits, const LogprobOut o) {
     __shared__ Lds s;
@@ -356,17 +361,16 @@ __global__ void __launch_bounds__(NT) logprobs_join_kernel(const Part* __restric
         for (int i = 0; i < N; i++) k[i] = (int)threadIdx.x + NT * i < n ? keys[threadIdx.x + NT * i] : 0;
         Part p{-INFINITY, 0.f, 0.f, -INFINITY, 0, {}};
         for (int i = threadIdx.x; i < splits; i += NT) join(p, parts[(size_t)t * splits + i]);
-#pragma unroll
-        for (int w = 1; w < WAVE; w *= 2) {
-            const Part b = shfl_part(p, w);
-            Part lo = lane & w ? b : p;  // (the lower lane's first, so that all lanes have the same bits)
-            join(lo, lane & w ? p : b);
-            p = lo;
-        }
-        if (lane == 0) s.part[wave] = p;
-        __syncthreads();
-        p = s.part[0];
+        const float m = wave_max(p.m), f = p.m == -INFINITY ? 0.f : p.m == m ? 1.f : expf(p.m - m);
+        p.s = wave_sum(f > 0.f ? f * fmaf(p.m - m, p.z, p.s) : 0.f);
+        p.z = wave_sum(f * p.z);
+        p.tok = wave_max(p.tok);
+        p.bad = __any(p.bad);
+        p.m = m;
         if (splits > WAVE) {
+            if (lane == 0) s.part[wave] = p;
+            __syncthreads();
+            p = s.part[0];
 #pragma unroll
             for (int w = 1; w < NW; w++) join(p, s.part[w]);
         }
@@ -378,7 +382,7 @@ __global__ void __launch_bounds__(NT) logprobs_join_kernel(const Part* __restric
 #pragma unroll
                     for (int i = 0; i < N; i++) k[i] = b + (int)threadIdx.x + NT * i < n ? keys[b + threadIdx.x + NT * i] : 0;
                 }
-                have = select_keys<N>(s, have, o.top, [&](int i) { return k[i]; });
+                have = select_keys<N, N>(s, have, o.top, [&](int i) { return k[i]; });
             }
             if ((int)threadIdx.x < o.top) finish_top(o, t, threadIdx.x, p, s.list[threadIdx.x]);
         }

@@ -86,6 +86,7 @@ struct Q4Args {
     long long ldy;
     int M, accumulate;
     Q4Dims d;
+    int c0;         // first piece of K that a launch takes
 };
 
 // ---------------------------------------------------------------------------------------------
@@ -211,7 +212,7 @@ __global__ void __launch_bounds__(MW * WAVE) q4_stream_kernel(const Q4Args a) {
     const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
     const int r = lane % 16, q = lane / 16, KS = blockDim.x / WAVE;
     const int KC = d.chunks(), B8 = d.blocks8(), tiles = d.tiles();
-    const int c0 = wave * CPS, g0 = c0 * (4 / SPG);       // first piece and first group of the slice
+    const int c0 = a.c0 + wave * CPS, g0 = c0 * (4 / SPG);  // first piece and first group of the slice
     const int m0 = blockIdx.y * (16 * RT), M = a.M - m0;  // rows of this workgroup
 
     // tiles blockIdx.x, + gridDim.x, ... Pieces and groups past K repeat the last ones: X is zero there.
@@ -236,7 +237,7 @@ __global__ void __launch_bounds__(MW * WAVE) q4_stream_kernel(const Q4Args a) {
     int e4[PRE ? 1 : RT][4];  // exponents of the rows 4 q + i whose sums this lane holds
     // PRE: the waves' blocks of sums [blocks][RT][2][WAVE], which a tile reads once
     half8* xsl = (half8*)(red_raw + 2 * SUMS * KS * WAVE);
-    const int nblocks = (d.K / d.G + 31) / 32;
+    const int nblocks = a.c0 ? 0 : (d.K / d.G + 31) / 32;
 #pragma unroll
     for (int t = 0; t < RT; t++) {
         if constexpr (PRE) {
@@ -395,7 +396,7 @@ __global__ void __launch_bounds__(MW * WAVE) q4_stream_kernel(const Q4Args a) {
 
 template <typename TX, int SPG, bool PK, int RT, int CPS, int MW, bool PRE>
 int launch_stream(const Q4Args& a, hipStream_t st) {
-    const int ks = (a.d.chunks() + CPS - 1) / CPS, tiles = a.d.tiles(), gy = (a.M + 16 * RT - 1) / (16 * RT);
+    const int ks = std::min(MW, (a.d.chunks() - a.c0 + CPS - 1) / CPS), tiles = a.d.tiles(), gy = (a.M + 16 * RT - 1) / (16 * RT);
     // 16 waves per CU, or 8 with X's operands in twice the registers; every workgroup as many tiles as the others
     const int cu = PRE ? 8 : 16, most = std::max(1, 256 * std::max(1, cu / ks) / gy), rounds = (tiles + most - 1) / most;
     const int lds = ((RT < 2 ? 4 : 2 * RT) * ks + (PRE ? (a.d.K / a.d.G + 31) / 32 * 2 * RT : 0)) * 1024;
@@ -416,9 +417,170 @@ int stream_spg(const Q4Args& a, hipStream_t st) {
     }
 }
 
-// Rows of X and K that the stream takes: what of X fits in the registers beside the pieces in flight.
+// ---------------------------------------------------------------------------------------------
+// Many rows: tiles of 128 rows of X x 256 of W, 8 waves of 64 x 64. X's operands go from the workspace straight into
+// LDS (1 KB pieces as they lie there: no bank conflicts, no swizzle), 128 k ahead in a second buffer; codes go from
+// global memory to registers, a piece ahead, and are unpacked in the wave that uses them. The sums of a group join
+// the tile's in fp32 (one FMA per 32 products and lane).
+constexpr int GM = 128, GN = 256, GR = 4, GC = 4;  // tile; a wave's 16 x 16 tiles
+
+// 16 bytes per lane straight from global memory into LDS at lds + 16 lane (lds uniform)
+__device__ __forceinline__ void q4_g2lds(const void* src, void* lds) {
+    __builtin_amdgcn_global_load_lds(src, (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
+}
+
+template <int P, int SPG>
+__global__ void __launch_bounds__(512) q4_gemm_kernel(const Q4Args a, int tiles_m, int tiles_n, int ntiles, int per_xcd) {
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];  // [2][8 tiles][P][4 steps][1 KB]
+    constexpr int BUF = GM / 16 * P * 4 * 1024, GP = 4 / SPG;
+    // consecutive tiles on one XCD: 8 of M beside each other, then along N, so that its workgroups share both in L2
+    const int li = (blockIdx.x % 8) * per_xcd + blockIdx.x / 8;
+    if (li >= ntiles) return;
+    const int gm = li / (8 * tiles_n) * 8, gw = min(8, tiles_m - gm), in = li - gm * tiles_n;
+    const int bm = gm + in % gw, bn = in / gw;
+    const Q4Dims d = a.d;
+    const Q4Ptr w = q4_ptr(a.W, d);
+    const XOps o(a.M, P, d);
+    const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+    const int r = lane % 16, q = lane / 16, wm = wave % 2, wn = wave / 2;
+    const int KC = d.chunks(), B8 = d.blocks8(), tiles = d.tiles(), xt = (int)o.tiles;
+
+    // this wave's pieces of X per stage: one tile of 16 rows, all its parts and steps
+    const unsigned char* xsrc = (const unsigned char*)a.X + ((size_t)min(bm * 8 + wave, xt - 1) * P * o.steps) * 1024 + lane * 16;
+    auto stage = [&](int c) {
+#pragma unroll
+        for (int p = 0; p < P; p++)
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                q4_g2lds(xsrc + ((size_t)p * o.steps + c * 4 + j) * 1024, lds + c % 2 * BUF + ((wave * P + p) * 4 + j) * 1024);
+    };
+    int nt[GC];
+#pragma unroll
+    for (int n = 0; n < GC; n++) nt[n] = min(bn * 16 + wn * 4 + n, tiles - 1);
+    u4v code[2][GC];
+    u2v sc[2][GC];
+    auto load = [&](int buf, int c) {
+#pragma unroll
+        for (int n = 0; n < GC; n++) {
+            code[buf][n] = ((const u4v*)w.codes)[((size_t)nt[n] * KC + c) * 64 + lane];
+            const _Float16* p = w.scale + ((size_t)nt[n] * B8 + c * GP / 8) * 128 + r * 8 + c * GP % 8;
+            if (GP == 4) sc[buf][n] = *(const u2v*)p;
+            else if (GP == 2) sc[buf][n][0] = *(const uint32_t*)p;
+            else sc[buf][n][0] = *(const uint16_t*)p;
+        }
+    };
+    stage(0);
+    load(0, 0);
+
+    // the minima's term first, in the units of the codes' sums
+    f32x4 acc[GR][GC];
+#pragma unroll
+    for (int m = 0; m < GR; m++)
+#pragma unroll
+        for (int n = 0; n < GC; n++) acc[m][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const half8* sums = (const half8*)((const unsigned char*)a.X + o.sums_at());
+    for (int b = 0; b < o.blocks; b++) {
+        half8 mn[GC];
+#pragma unroll
+        for (int n = 0; n < GC; n++) mn[n] = *(const half8*)(w.mins + ((size_t)nt[n] * B8 + min(b * 4 + q, B8 - 1)) * 128 + r * 8);
+#pragma unroll
+        for (int m = 0; m < GR; m++)
+#pragma unroll
+            for (int p = 0; p < 2; p++) {
+                const half8 x = sums[(((size_t)min(bm * 8 + wm * 4 + m, xt - 1) * 2 + p) * o.blocks + b) * 64 + lane];
+#pragma unroll
+                for (int n = 0; n < GC; n++) acc[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, mn[n], acc[m][n], 0, 0, 0);
+            }
+    }
+#pragma unroll
+    for (int m = 0; m < GR; m++)
+#pragma unroll
+        for (int n = 0; n < GC; n++) acc[m][n] *= 1.f / kCodeUnit;
+
+    auto step = [&](int buf, int c) {
+        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's pieces of stage c are in LDS
+        lds_barrier();                       // all waves' are, and all have read stage c - 1
+        if (c + 1 < KC) {
+            stage(c + 1);
+            load(buf ^ 1, c + 1);
+        }
+        const unsigned char* x = lds + buf * BUF + wm * 4 * P * 4096 + lane * 16;
+#pragma unroll
+        for (int g = 0; g < GP; g++) {
+            f32x4 p[GR][GC];
+#pragma unroll
+            for (int s = 0; s < SPG; s++) {
+                const int j = g * SPG + s;
+                half8 b[GC];
+#pragma unroll
+                for (int n = 0; n < GC; n++) b[n] = q4_codes(code[buf][n][j]);
+#pragma unroll
+                for (int pt = 0; pt < P; pt++)
+#pragma unroll
+                    for (int m = 0; m < GR; m++) {
+                        const half8 xa = *(const half8*)(x + ((m * P + pt) * 4 + j) * 1024);
+#pragma unroll
+                        for (int n = 0; n < GC; n++)
+                            p[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                                xa, b[n], s == 0 && pt == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : p[m][n], 0, 0, 0);
+                    }
+            }
+#pragma unroll
+            for (int n = 0; n < GC; n++) {
+                const float f = (float)__builtin_bit_cast(_Float16, (uint16_t)(sc[buf][n][g / 2] >> (16 * (g % 2))));
+#pragma unroll
+                for (int m = 0; m < GR; m++) acc[m][n] += p[m][n] * f;
+            }
+            __builtin_amdgcn_sched_barrier(0);  // (one group's sums at a time: registers)
+        }
+    };
+    for (int c = 0; c < KC; c += 2) {
+        step(0, c);
+        if (c + 1 < KC) step(1, c + 1);
+    }
+
+    const int* exps = (const int*)((const unsigned char*)a.X + o.exps_at());
+#pragma unroll
+    for (int m = 0; m < GR; m++) {
+        const int row = bm * GM + (wm * 4 + m) * 16 + 4 * q;
+        const int4 e = *(const int4*)(exps + min(row, xt * 16 - 4));
+        const int es[4] = {18 - e.x, 18 - e.y, 18 - e.z, 18 - e.w};
+#pragma unroll
+        for (int n = 0; n < GC; n++) {
+            const int col = (bn * 16 + wn * 4 + n) * 16 + r;
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (row + i < a.M && col < d.N) {
+                    float* y = a.Y + (size_t)(row + i) * a.ldy + col;
+                    const float v = __builtin_ldexpf(acc[m][n][i], es[i]);
+                    __builtin_nontemporal_store(a.accumulate ? *y + v : v, y);
+                }
+        }
+    }
+}
+
+template <int P, int SPG>
+int launch_gemm(const Q4Args& a, hipStream_t st) {
+    const int tm = (a.M + GM - 1) / GM, tn = (a.d.N + GN - 1) / GN, n = tm * tn, per = (n + 7) / 8;
+    constexpr int lds = 2 * (GM / 16 * P * 4 * 1024);
+    if (lds > 65536)
+        AEG_HIP(hipFuncSetAttribute((const void*)q4_gemm_kernel<P, SPG>, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+    q4_gemm_kernel<P, SPG><<<8 * per, 512, lds, st>>>(a, tm, tn, n, per);
+    return after_launch("linear_q4");
+}
+template <int P>
+int gemm_spg(const Q4Args& a, hipStream_t st) {
+    switch (a.d.G) {
+        case 32: return launch_gemm<P, 1>(a, st);
+        case 64: return launch_gemm<P, 2>(a, st);
+        default: return launch_gemm<P, 4>(a, st);
+    }
+}
+
+// Rows of X and K that the stream takes with X's rows as they are, and as operands (K in blocks of 2048, the minima of
+// all of it in the first).
 bool stream_fits(int M, const Q4Dims& d) { return M <= 16 && d.K <= 4096; }
-bool pre_fits(int M, const Q4Dims& d) { return M <= 4096 && d.K <= 2048; }
+bool pre_fits(int M, const Q4Dims& d) { return M <= 256 && d.K <= 8192; }
 
 int run_stream(const Q4Args& a, int x_dtype, hipStream_t st) {
     if (x_dtype == AEGIST_BF16) return stream_spg<uint16_t, false, 1, 2, 16, false>(a, st);
@@ -433,40 +595,12 @@ int run_rows(Q4Args a, int x_dtype, void* ws, hipStream_t st) {
     int rc = after_launch("linear_q4");
     if (rc) return rc;
     a.X = ws;
-    if (x_dtype == AEGIST_F32) return stream_spg<float, false, 2, 2, 8, true>(a, st);
-    return a.M <= 32 ? stream_spg<uint16_t, false, 2, 2, 8, true>(a, st) : stream_spg<uint16_t, false, 4, 2, 8, true>(a, st);
-}
-
-// ---------------------------------------------------------------------------------------------
-// 16 rows of W x 16 rows of X per workgroup, a product per thread.
-template <typename TX>
-__global__ void __launch_bounds__(256) linear_q4_kernel(const TX* __restrict__ X, long long ldx,
-                                                        const unsigned char* __restrict__ W, float* __restrict__ Y,
-                                                        long long ldy, int M, const Q4Dims d, int accumulate) {
-    const int r = threadIdx.x % 16, n = blockIdx.x * 16 + r;
-    const Q4Ptr w = q4_ptr(W, d);
-    for (int m = blockIdx.y * 16 + threadIdx.x / 16; m < M; m += gridDim.y * 16) {
-        if (n >= d.N) return;
-        const TX* x = X + (size_t)m * ldx;
-        float acc = 0.f;
-        for (int g = 0; g < d.K / d.G; g++) {
-            float p = 0.f, s = 0.f;
-            for (int k = g * d.G; k < (g + 1) * d.G; k += 8) {
-                const int lane = k % 32 / 8 * 16 + r;
-                const uint32_t v = ((const uint32_t*)w.codes)[(((size_t)blockIdx.x * d.chunks() + k / 128) * 64 + lane) * 4 +
-                                                              k % 128 / 32];
-                for (int e = 0; e < 8; e++) {
-                    const float f = Act<TX>::ld(x, k + e);
-                    p = fmaf((float)q4_get(v, e), f, p);
-                    s += f;
-                }
-            }
-            const size_t gi = ((size_t)(n / 16) * d.blocks8() + g / 8) * 128 + (n % 16) * 8 + g % 8;
-            acc = fmaf(p, (float)w.scale[gi], fmaf(s, (float)w.mins[gi], acc));
-        }
-        float* y = Y + (size_t)m * ldy + n;
-        *y = accumulate ? *y + acc : acc;
-    }
+    if (!pre_fits(a.M, a.d)) return x_dtype == AEGIST_F32 ? gemm_spg<2>(a, st) : gemm_spg<1>(a, st);
+    for (a.c0 = 0; a.c0 < a.d.chunks() && !rc; a.c0 += 16, a.accumulate = 1)
+        rc = x_dtype == AEGIST_F32 ? stream_spg<float, false, 2, 2, 8, true>(a, st)
+             : a.M <= 32           ? stream_spg<uint16_t, false, 2, 2, 8, true>(a, st)
+                                   : stream_spg<uint16_t, false, 4, 2, 8, true>(a, st);
+    return rc;
 }
 
 }  // namespace
@@ -475,7 +609,7 @@ namespace aegist {
 
 size_t linear_q4_workspace(int x_dtype, int M, int N, int K, int G) {
     const Q4Dims d{N, K, G};
-    return M == 0 || N == 0 || stream_fits(M, d) || !pre_fits(M, d) ? 0 : XOps(M, x_dtype == AEGIST_F32 ? 2 : 1, d).bytes();
+    return M == 0 || N == 0 || stream_fits(M, d) ? 0 : XOps(M, x_dtype == AEGIST_F32 ? 2 : 1, d).bytes();
 }
 
 int launch_linear_q4(const void* X, int x_dtype, long long ldx, const void* W, float* Y, long long ldy, int M, int N,
@@ -493,16 +627,10 @@ int launch_linear_q4(const void* X, int x_dtype, long long ldx, const void* W, f
     if (ldy < N) return fail(AEGIST_ERR_SHAPE, "linear_q4: ldy < N");
     if ((uintptr_t)W % 16) return fail(AEGIST_ERR_SHAPE, "linear_q4: W must be 16-byte aligned");
     const Q4Dims d{N, K, G};
-    const Q4Args a{X, ldx, (const unsigned char*)W, Y, ldy, M, accumulate, d};
+    const Q4Args a{X, ldx, (const unsigned char*)W, Y, ldy, M, accumulate, d, 0};
     if (stream_fits(M, d)) return run_stream(a, x_dtype, st);
     if ((rc = check_workspace(ws, ws_bytes, linear_q4_workspace(x_dtype, M, N, K, G), "linear_q4"))) return rc;
-    if (pre_fits(M, d)) return run_rows(a, x_dtype, ws, st);
-    const dim3 grid(d.tiles(), std::min((M + 15) / 16, 65535));
-    if (x_dtype == AEGIST_F32)
-        linear_q4_kernel<float><<<grid, 256, 0, st>>>((const float*)X, ldx, (const unsigned char*)W, Y, ldy, M, d, accumulate);
-    else
-        linear_q4_kernel<uint16_t><<<grid, 256, 0, st>>>((const uint16_t*)X, ldx, (const unsigned char*)W, Y, ldy, M, d, accumulate);
-    return after_launch("linear_q4");
+    return run_rows(a, x_dtype, ws, st);
 }
 
 }  // namespace aegist
