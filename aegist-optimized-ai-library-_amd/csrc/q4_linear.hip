@@ -328,6 +328,7 @@ __global__ void __launch_bounds__(MW * WAVE) q4_stream_kernel(const Q4Args a) {
 #pragma unroll
             for (int t = 0; t < RT; t++) {
                 acc[t] += p[t] * sc;
+                asm volatile("" : "+v"(acc[t]));  // (here, not sunk past the tile with p kept till then)
                 p[t] = f32x4{0.f, 0.f, 0.f, 0.f};
             }
             __builtin_amdgcn_sched_barrier(0);  // (codes are unpacked a group at a time: registers)
@@ -419,8 +420,9 @@ int stream_spg(const Q4Args& a, hipStream_t st) {
 
 // ---------------------------------------------------------------------------------------------
 // Many rows: tiles of 128 rows of X x 256 of W, 8 waves of 64 x 64. X's operands go from the workspace straight into
-// LDS (1 KB pieces as they lie there: no bank conflicts, no swizzle), 128 k ahead in a second buffer; codes go from
-// global memory to registers, a piece ahead, and are unpacked in the wave that uses them. The sums of a group join
+// LDS (1 KB pieces as they lie there: no bank conflicts, no swizzle), 128 k to a stage; codes go from global memory to
+// registers and are unpacked in the wave that uses them. Both are requested two stages ahead (fp32 X: one, of
+// twice the products: LDS). The sums of a group join
 // the tile's in fp32 (one FMA per 32 products and lane).
 constexpr int GM = 128, GN = 256, GR = 4, GC = 4;  // tile; a wave's 16 x 16 tiles
 
@@ -431,8 +433,11 @@ __device__ __forceinline__ void q4_g2lds(const void* src, void* lds) {
 
 template <int P, int SPG>
 __global__ void __launch_bounds__(512) q4_gemm_kernel(const Q4Args a, int tiles_m, int tiles_n, int ntiles, int per_xcd) {
-    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];  // [2][8 tiles][P][4 steps][1 KB]
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];  // [NB][8 tiles][P][4 steps][1 KB]
+    constexpr int NB = P == 1 ? 3 : 2;  // stages in LDS and registers
     constexpr int BUF = GM / 16 * P * 4 * 1024, GP = 4 / SPG;
+    // steps whose products are summed before they are scaled: two of one group, where X's operands leave the registers
+    constexpr int U = P == 2 || SPG == 1 ? 1 : 2;
     // consecutive tiles on one XCD: 8 of M beside each other, then along N, so that its workgroups share both in L2
     const int li = (blockIdx.x % 8) * per_xcd + blockIdx.x / 8;
     if (li >= ntiles) return;
@@ -447,18 +452,18 @@ __global__ void __launch_bounds__(512) q4_gemm_kernel(const Q4Args a, int tiles_
 
     // this wave's pieces of X per stage: one tile of 16 rows, all its parts and steps
     const unsigned char* xsrc = (const unsigned char*)a.X + ((size_t)min(bm * 8 + wave, xt - 1) * P * o.steps) * 1024 + lane * 16;
-    auto stage = [&](int c) {
+    auto stage = [&](int buf, int c) {
 #pragma unroll
         for (int p = 0; p < P; p++)
 #pragma unroll
             for (int j = 0; j < 4; j++)
-                q4_g2lds(xsrc + ((size_t)p * o.steps + c * 4 + j) * 1024, lds + c % 2 * BUF + ((wave * P + p) * 4 + j) * 1024);
+                q4_g2lds(xsrc + ((size_t)p * o.steps + c * 4 + j) * 1024, lds + buf * BUF + ((wave * P + p) * 4 + j) * 1024);
     };
     int nt[GC];
 #pragma unroll
     for (int n = 0; n < GC; n++) nt[n] = min(bn * 16 + wn * 4 + n, tiles - 1);
-    u4v code[2][GC];
-    u2v sc[2][GC];
+    u4v code[NB][GC];
+    u2v sc[NB][GC];
     auto load = [&](int buf, int c) {
 #pragma unroll
         for (int n = 0; n < GC; n++) {
@@ -469,8 +474,12 @@ __global__ void __launch_bounds__(512) q4_gemm_kernel(const Q4Args a, int tiles_
             else sc[buf][n][0] = *(const uint16_t*)p;
         }
     };
-    stage(0);
-    load(0, 0);
+#pragma unroll
+    for (int c = 0; c < NB - 1; c++)
+        if (c < KC) {
+            stage(c, c);
+            load(c, c);
+        }
 
     // the minima's term first, in the units of the codes' sums
     f32x4 acc[GR][GC];
@@ -498,45 +507,62 @@ __global__ void __launch_bounds__(512) q4_gemm_kernel(const Q4Args a, int tiles_
         for (int n = 0; n < GC; n++) acc[m][n] *= 1.f / kCodeUnit;
 
     auto step = [&](int buf, int c) {
-        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's pieces of stage c are in LDS
-        lds_barrier();                       // all waves' are, and all have read stage c - 1
-        if (c + 1 < KC) {
-            stage(c + 1);
-            load(buf ^ 1, c + 1);
+        // this wave's pieces of stage c are in LDS once only the later stage's loads are in flight
+        if (NB == 3 && c + 1 < KC) __builtin_amdgcn_s_waitcnt(0x0f70 | (4 * P + 2 * GC));
+        else __builtin_amdgcn_s_waitcnt(0x0f70);
+        lds_barrier();  // all waves' are, and all have read stage c - 1
+        if (c + NB - 1 < KC) {
+            stage((buf + NB - 1) % NB, c + NB - 1);
+            load((buf + NB - 1) % NB, c + NB - 1);
         }
         const unsigned char* x = lds + buf * BUF + wm * 4 * P * 4096 + lane * 16;
+        half8 xa[2][P][U][GR];
+        auto operands = [&](int u) {
 #pragma unroll
-        for (int g = 0; g < GP; g++) {
-            f32x4 p[GR][GC];
+            for (int pt = 0; pt < P; pt++)
 #pragma unroll
-            for (int s = 0; s < SPG; s++) {
-                const int j = g * SPG + s;
-                half8 b[GC];
+                for (int s = 0; s < U; s++)
 #pragma unroll
-                for (int n = 0; n < GC; n++) b[n] = q4_codes(code[buf][n][j]);
+                    for (int m = 0; m < GR; m++) xa[u % 2][pt][s][m] = *(const half8*)(x + ((m * P + pt) * 4 + u * U + s) * 1024);
+        };
+        // unit u, tile n: its products, then the FMAs of the tile before, which run beside them
+        f32x4 p[2][GR];
+        auto join = [&](int i) {
+            const int u = i / GC, n = i % GC, g = u * U / SPG;
+            const float f = (float)__builtin_bit_cast(_Float16, (uint16_t)(sc[buf][n][g / 2] >> (16 * (g % 2))));
 #pragma unroll
-                for (int pt = 0; pt < P; pt++)
-#pragma unroll
-                    for (int m = 0; m < GR; m++) {
-                        const half8 xa = *(const half8*)(x + ((m * P + pt) * 4 + j) * 1024);
-#pragma unroll
-                        for (int n = 0; n < GC; n++)
-                            p[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                                xa, b[n], s == 0 && pt == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : p[m][n], 0, 0, 0);
-                    }
+            for (int m = 0; m < GR; m++) {
+                acc[m][n] += p[i % 2][m] * f;
+                asm volatile("" : "+v"(acc[m][n]));  // (here, not sunk past the stage with p kept till then)
             }
+        };
+        operands(0);
+#pragma unroll
+        for (int u = 0; u < 4 / U; u++) {
+            if (u + 1 < 4 / U) operands(u + 1);
 #pragma unroll
             for (int n = 0; n < GC; n++) {
-                const float f = (float)__builtin_bit_cast(_Float16, (uint16_t)(sc[buf][n][g / 2] >> (16 * (g % 2))));
+                const int i = u * GC + n;
 #pragma unroll
-                for (int m = 0; m < GR; m++) acc[m][n] += p[m][n] * f;
+                for (int s = 0; s < U; s++) {
+                    const half8 b = q4_codes(code[buf][n][u * U + s]);
+#pragma unroll
+                    for (int pt = 0; pt < P; pt++)
+#pragma unroll
+                        for (int m = 0; m < GR; m++)
+                            p[i % 2][m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                                xa[u % 2][pt][s][m], b, s == 0 && pt == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : p[i % 2][m], 0, 0, 0);
+                }
+                if (i > 0) join(i - 1);
+                __builtin_amdgcn_sched_barrier(0);
             }
-            __builtin_amdgcn_sched_barrier(0);  // (one group's sums at a time: registers)
         }
+        join(4 / U * GC - 1);
     };
-    for (int c = 0; c < KC; c += 2) {
-        step(0, c);
-        if (c + 1 < KC) step(1, c + 1);
+    for (int c = 0; c < KC; c += NB) {
+#pragma unroll
+        for (int i = 0; i < NB; i++)
+            if (c + i < KC) step(i, c + i);
     }
 
     const int* exps = (const int*)((const unsigned char*)a.X + o.exps_at());
@@ -562,7 +588,7 @@ __global__ void __launch_bounds__(512) q4_gemm_kernel(const Q4Args a, int tiles_
 template <int P, int SPG>
 int launch_gemm(const Q4Args& a, hipStream_t st) {
     const int tm = (a.M + GM - 1) / GM, tn = (a.d.N + GN - 1) / GN, n = tm * tn, per = (n + 7) / 8;
-    constexpr int lds = 2 * (GM / 16 * P * 4 * 1024);
+    constexpr int lds = (P == 1 ? 3 : 2) * (GM / 16 * P * 4 * 1024);
     if (lds > 65536)
         AEG_HIP(hipFuncSetAttribute((const void*)q4_gemm_kernel<P, SPG>, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
     q4_gemm_kernel<P, SPG><<<8 * per, 512, lds, st>>>(a, tm, tn, n, per);
