@@ -434,7 +434,7 @@ __device__ __forceinline__ void q4_g2lds(const void* src, void* lds) {
 template <int P, int SPG>
 __global__ void __launch_bounds__(512) q4_gemm_kernel(const Q4Args a, int tiles_m, int tiles_n, int ntiles, int per_xcd) {
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];  // [NB][8 tiles][P][4 steps][1 KB]
-    constexpr int NB = P == 1 ? 3 : 2;  // stages in LDS and registers
+    constexpr int NB = 2;  // stages in LDS and registers
     constexpr int BUF = GM / 16 * P * 4 * 1024, GP = 4 / SPG;
     // steps whose products are summed before they are scaled: two of one group, where X's operands leave the registers
     constexpr int U = P == 2 || SPG == 1 ? 1 : 2;
@@ -517,15 +517,16 @@ __global__ void __launch_bounds__(512) q4_gemm_kernel(const Q4Args a, int tiles_
         }
         const unsigned char* x = lds + buf * BUF + wm * 4 * P * 4096 + lane * 16;
         half8 xa[2][P][U][GR];
-        auto operands = [&](int u) {
-#pragma unroll
-            for (int pt = 0; pt < P; pt++)
-#pragma unroll
-                for (int s = 0; s < U; s++)
-#pragma unroll
-                    for (int m = 0; m < GR; m++) xa[u % 2][pt][s][m] = *(const half8*)(x + ((m * P + pt) * 4 + u * U + s) * 1024);
+        constexpr int XF = P * U * GR;  // operands of a unit, products of a unit's tile
+        auto operand = [&](int u, int i) {
+            const int m = i % GR, s = i / GR % U, pt = i / GR / U;
+            xa[u % 2][pt][s][m] = *(const half8*)(x + ((m * P + pt) * 4 + u * U + s) * 1024);
         };
-        // unit u, tile n: its products, then the FMAs of the tile before, which run beside them
+        half8 b[2][U];
+        auto unpack = [&](int i) {
+#pragma unroll
+            for (int s = 0; s < U; s++) b[i % 2][s] = q4_codes(code[buf][i % GC][i / GC * U + s]);
+        };
         f32x4 p[2][GR];
         auto join = [&](int i) {
             const int u = i / GC, n = i % GC, g = u * U / SPG;
@@ -536,28 +537,40 @@ __global__ void __launch_bounds__(512) q4_gemm_kernel(const Q4Args a, int tiles_
                 asm volatile("" : "+v"(acc[m][n]));  // (here, not sunk past the stage with p kept till then)
             }
         };
-        operands(0);
 #pragma unroll
-        for (int u = 0; u < 4 / U; u++) {
-            if (u + 1 < 4 / U) operands(u + 1);
+        for (int i = 0; i < XF; i++) operand(0, i);
+        unpack(0);
+        __builtin_amdgcn_sched_barrier(0);
+        // tile i: its products, and between them the codes of the next one, the FMAs of the one before and a share of the
+        // next unit's operands
+        constexpr int IS = 4 / U * GC;
 #pragma unroll
-            for (int n = 0; n < GC; n++) {
-                const int i = u * GC + n;
+        for (int i = 0; i < IS; i++) {
+            const int u = i / GC;
+            if (u + 1 < 4 / U) {
 #pragma unroll
-                for (int s = 0; s < U; s++) {
-                    const half8 b = q4_codes(code[buf][n][u * U + s]);
-#pragma unroll
-                    for (int pt = 0; pt < P; pt++)
-#pragma unroll
-                        for (int m = 0; m < GR; m++)
-                            p[i % 2][m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                                xa[u % 2][pt][s][m], b, s == 0 && pt == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : p[i % 2][m], 0, 0, 0);
-                }
-                if (i > 0) join(i - 1);
-                __builtin_amdgcn_sched_barrier(0);
+                for (int k = 0; k < XF / GC; k++) operand(u + 1, i % GC * (XF / GC) + k);
             }
+#pragma unroll
+            for (int s = 0; s < U; s++)
+#pragma unroll
+                for (int pt = 0; pt < P; pt++)
+#pragma unroll
+                    for (int m = 0; m < GR; m++)
+                        p[i % 2][m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                            xa[u % 2][pt][s][m], b[i % 2][s], s == 0 && pt == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : p[i % 2][m], 0, 0, 0);
+            if (i + 1 < IS) unpack(i + 1);
+            if (i > 0) join(i - 1);
+            constexpr int VALU = (7 * U + 4 * GR + 2 + XF - 1) / XF;  // per product
+#pragma unroll
+            for (int k = 0; k < XF; k++) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                if (k < XF / GC) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x002, VALU, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
-        join(4 / U * GC - 1);
+        join(IS - 1);
     };
     for (int c = 0; c < KC; c += NB) {
 #pragma unroll
@@ -588,7 +601,7 @@ __global__ void __launch_bounds__(512) q4_gemm_kernel(const Q4Args a, int tiles_
 template <int P, int SPG>
 int launch_gemm(const Q4Args& a, hipStream_t st) {
     const int tm = (a.M + GM - 1) / GM, tn = (a.d.N + GN - 1) / GN, n = tm * tn, per = (n + 7) / 8;
-    constexpr int lds = (P == 1 ? 3 : 2) * (GM / 16 * P * 4 * 1024);
+    constexpr int lds = 2 * (GM / 16 * P * 4 * 1024);
     if (lds > 65536)
         AEG_HIP(hipFuncSetAttribute((const void*)q4_gemm_kernel<P, SPG>, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
     q4_gemm_kernel<P, SPG><<<8 * per, 512, lds, st>>>(a, tm, tn, n, per);
