@@ -18,6 +18,7 @@
 #include "q4.h"
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 using namespace aegist;
@@ -31,6 +32,12 @@ typedef uint32_t u2v __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ half8 q4_codes(uint32_t d) {
     constexpr uint32_t m = 0x03c003c0u;
     return __builtin_bit_cast(half8, u4v{d & m, d << 4 & m, d >> 4 & m, __builtin_amdgcn_alignbit(d, d, 8) & m});
+}
+// The scale in the low half of w as a float in a register of its own (left to the compiler, every FMA converts it again).
+__device__ __forceinline__ float q4_scale(uint32_t w) {
+    float f = (float)__builtin_bit_cast(_Float16, (uint16_t)w);
+    asm("" : "+v"(f));
+    return f;
 }
 // what undoes the units of the code products (2^-18) beside those of the minima (X's sums in units of 2^7)
 constexpr float kCodeUnit = 0x1p11f;
@@ -181,13 +188,20 @@ __global__ void __launch_bounds__(XW * WAVE) q4_rows_kernel(const Q4Args a, unsi
 
 // ---------------------------------------------------------------------------------------------
 // Few rows: the weight as a stream, X in registers. The waves of a workgroup cut K into slices of CPS pieces (128 k
-// each); a wave holds its slice of 16 RT rows of X as matrix operands and takes its pieces of one tile (16 rows of
+// each); a wave holds its slice of 16 rows of X as matrix operands and takes its pieces of one tile (16 rows of
 // W) after the other, the next two in flight; per round of two tiles the waves' sums meet in LDS. So a weight
 // is one contiguous 1 KB load and no more, nothing in the loop reads LDS but the sums, and a slice is
 // scaled by its own largest value, which needs no exchange between waves.
 //
 // Waves that staged X in LDS, once per workgroup, and read it back per piece took 16.5 us at 16 rows of 2048 x 4096,
 // mostly the staging (two rows per wave one after the other).
+
+// Up to kStaged rows are scaled one after the other, 4 values of the slice per lane, and pass through the wave's own LDS
+// into the operands: a lane that makes its operands itself makes those of row r % M, the same as the others of that row
+// (8192 x 2048, one row: 9.0 -> 7 us).
+constexpr int kStaged = 4;
+// per wave: rows [M][parts][256 fp16], sums [M][2][8 fp16], exponents [4]
+__host__ __device__ constexpr int staged_bytes(int M, int parts) { return M * (parts * 512 + 32) + 16; }
 
 template <int SPG, int CPS>
 struct Q4Slice {
@@ -197,28 +211,26 @@ struct Q4Slice {
     u4v scale[SB], mins;
 };
 
-// SPG: steps of 32 k per group. PK: fp32 X of up to 8 rows, its two parts as rows m and m + 8 of one operand.
-// MW: waves at most. PRE: X is there as operands (XOps), else every workgroup makes them of the rows.
-template <typename TX, int SPG, bool PK, int RT, int CPS, int MW, bool PRE>
+// SPG: steps of 32 k per group. MW: waves at most. FEW: up to kStaged rows.
+template <typename TX, int SPG, int CPS, int MW, bool FEW>
 __global__ void __launch_bounds__(MW * WAVE) q4_stream_kernel(const Q4Args a) {
     constexpr bool F32 = std::is_same<TX, float>::value;
+    constexpr bool PK = F32 && FEW;  // the two parts of row m as rows m and m + 8 of one operand
     constexpr int NA = F32 && !PK ? 2 : 1, NS = PK ? 1 : 2, ST = CPS * 4;
-    constexpr int SUMS = RT < 2 ? 2 : RT;  // sums per meeting of the waves
     typedef Q4Slice<SPG, CPS> Slice;
-    constexpr int NB = SUMS / RT;  // tiles of such a meeting
-    extern __shared__ f32x4 red_raw[];  // [2][SUMS][KS][WAVE]
+    extern __shared__ f32x4 red_raw[];  // [2][2 tiles][KS][WAVE]
     const Q4Dims d = a.d;
     const Q4Ptr w = q4_ptr(a.W, d);
     const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
     const int r = lane % 16, q = lane / 16, KS = blockDim.x / WAVE;
     const int KC = d.chunks(), B8 = d.blocks8(), tiles = d.tiles();
     const int c0 = a.c0 + wave * CPS, g0 = c0 * (4 / SPG);  // first piece and first group of the slice
-    const int m0 = blockIdx.y * (16 * RT), M = a.M - m0;  // rows of this workgroup
+    const int m0 = blockIdx.y * 16, M = a.M - m0;  // rows of this workgroup
 
     // tiles blockIdx.x, + gridDim.x, ... Pieces and groups past K repeat the last ones: X is zero there.
     Slice sl[2];
     const int cl = KC - 1 - c0, bl = B8 - 1 - g0 / 8;
-    const int mb = PRE ? min(wave * 4 + q, B8 - 1) : g0 / 8 + min(q, min(Slice::SB - 1, bl));
+    const int mb = g0 / 8 + min(q, min(Slice::SB - 1, bl));
     auto load = [&](Slice& s, int t) {
         if (t >= tiles) return;
         const u4v* cp = (const u4v*)w.codes + ((size_t)t * KC + c0) * 64 + lane;
@@ -233,30 +245,68 @@ __global__ void __launch_bounds__(MW * WAVE) q4_stream_kernel(const Q4Args a) {
     load(sl[1], blockIdx.x + gridDim.x);
 
     // the slice of X: lane (r, q) has k = 32 j + 8 q .. + 7 of the steps j, of row r (PK: of row r % 8)
-    half8 xa[RT][NA][ST], xs[PRE ? 1 : RT][NS];
-    int e4[PRE ? 1 : RT][4];  // exponents of the rows 4 q + i whose sums this lane holds
-    // PRE: the waves' blocks of sums [blocks][RT][2][WAVE], which a tile reads once
-    half8* xsl = (half8*)(red_raw + 2 * SUMS * KS * WAVE);
-    const int nblocks = a.c0 ? 0 : (d.K / d.G + 31) / 32;
+    half8 xa[NA][ST], xs[NS];
+    int e4[4];  // exponents of the rows 4 q + i whose sums this lane holds
+    if constexpr (FEW) {
+        static_assert(CPS == 2, "4 values per lane");
+        constexpr int PARTS = F32 ? 2 : 1;
+        unsigned char* own = (unsigned char*)(red_raw + 4 * KS * WAVE) + wave * staged_bytes(M, PARTS);
+        unsigned char *own_s = own + M * PARTS * 512, *own_e = own_s + M * 32;
+        const int k = c0 * 128 + 4 * lane, kk = min(k, d.K - 4);
+        for (int m = 0; m < M; m++) {
+            float f[4];
+            const TX* x = (const TX*)a.X + (size_t)(m0 + m) * a.ldx + kk;
+            if constexpr (F32) {
+                const f32x4 v = *(const f32x4*)x;
 #pragma unroll
-    for (int t = 0; t < RT; t++) {
-        if constexpr (PRE) {
-            const XOps o(a.M, NA, d);
-            const size_t mt = min((size_t)(m0 / 16 + t), o.tiles - 1);
-            const half8* parts = (const half8*)a.X;
-            const half8* sums = (const half8*)((const unsigned char*)a.X + o.sums_at());
-#pragma unroll
-            for (int n = 0; n < NA; n++)
-#pragma unroll
-                for (int j = 0; j < ST; j++) xa[t][n][j] = parts[((mt * NA + n) * o.steps + c0 * 4 + j) * 64 + lane];
-            if (wave < nblocks) {
-#pragma unroll
-                for (int n = 0; n < 2; n++)
-                    xsl[((wave * RT + t) * 2 + n) * WAVE + lane] = sums[((mt * 2 + n) * o.blocks + wave) * 64 + lane];
+                for (int i = 0; i < 4; i++) f[i] = v[i];
+            } else {
+                const u2v v = *(const u2v*)x;
+                f[0] = bf_lo(v[0]), f[1] = bf_hi(v[0]), f[2] = bf_lo(v[1]), f[3] = bf_hi(v[1]);
             }
-            continue;
+#pragma unroll
+            for (int i = 0; i < 4; i++) f[i] = k < d.K ? f[i] : 0.f;
+            const int e = row_exp(wave_max(fmaxf(fmaxf(fabsf(f[0]), fabsf(f[1])), fmaxf(fabsf(f[2]), fabsf(f[3])))));
+            half4 hi, lo;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float v = __builtin_ldexpf(f[i], e);
+                hi[i] = (_Float16)v;
+                lo[i] = (_Float16)(v - (float)hi[i]);
+            }
+            *(half4*)(own + m * PARTS * 512 + lane * 8) = hi;
+            if (F32) *(half4*)(own + (m * PARTS + 1) * 512 + lane * 8) = lo;
+            // the group's sum, from 8, 16 or 32 lanes, to its place among the 8 of its block
+            float s = (f[0] + f[1]) + (f[2] + f[3]);
+#pragma unroll
+            for (int o = 1; o < 8 * SPG; o *= 2) s += __shfl_xor(s, o, WAVE);
+            s = __builtin_ldexpf(s, e - 7);
+            const _Float16 sh = (_Float16)s;
+            if (lane < 16) ((_Float16*)(own_s + m * 32))[lane] = 0;
+            wave_sync();
+            if (lane % (8 * SPG) == 0) {
+                const int g = (g0 + lane / (8 * SPG)) % 8;
+                ((_Float16*)(own_s + m * 32))[g] = sh;
+                ((_Float16*)(own_s + m * 32))[8 + g] = (_Float16)(s - (float)sh);
+            }
+            if (lane == 0) ((int*)own_e)[m] = e;
         }
-        const int m = min(PK ? r % 8 : 16 * t + r, M - 1);
+        wave_sync();
+        const int m = min(PK ? r % 8 : r, M - 1), part = PK ? r / 8 : 0;
+#pragma unroll
+        for (int n = 0; n < NA; n++)
+#pragma unroll
+            for (int j = 0; j < ST; j++) xa[n][j] = *(const half8*)(own + (m * PARTS + part + n) * 512 + (32 * j + 8 * q) * 2);
+        const half8 none{};
+#pragma unroll
+        for (int n = 0; n < NS; n++) {
+            xs[n] = *(const half8*)(own_s + m * 32 + (part + n) * 16);
+            if (q > 0) xs[n] = none;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) e4[i] = 7 - ((const int*)own_e)[min((4 * q + i) % (PK ? 8 : 16), M - 1)];
+    } else {
+        const int m = min(r, M - 1);
         const TX* x = (const TX*)a.X + (size_t)(m0 + m) * a.ldx;
         X8<TX> f[ST];
         float amax = 0.f;
@@ -273,18 +323,15 @@ __global__ void __launch_bounds__(MW * WAVE) q4_stream_kernel(const Q4Args a) {
         amax = fmaxf(amax, __shfl_xor(amax, 32, WAVE));
         const int e = row_exp(amax);
 #pragma unroll
-        for (int i = 0; i < 4; i++) e4[t][i] = 7 - __shfl(e, (4 * q + i) % (PK ? 8 : 16), WAVE);
+        for (int i = 0; i < 4; i++) e4[i] = 7 - __shfl(e, 4 * q + i, WAVE);
         float s = 0.f;
         half8 hi{}, lo{};
 #pragma unroll
         for (int j = 0; j < ST; j++) {
             half8 l;
             const half8 h = x_parts(f[j], e, F32 ? &l : nullptr);
-            if (PK) xa[t][0][j] = r < 8 ? h : l;
-            else {
-                xa[t][0][j] = h;
-                if (NA == 2) xa[t][NA - 1][j] = l;
-            }
+            xa[0][j] = h;
+            if (F32) xa[NA - 1][j] = l;
             s += ((f[j].get(0) + f[j].get(1)) + (f[j].get(2) + f[j].get(3))) + ((f[j].get(4) + f[j].get(5)) + (f[j].get(6) + f[j].get(7)));
             if (j % SPG < SPG - 1) continue;
             // the group's sum, and its place among the 8 of the block that lanes q read the minima of
@@ -301,130 +348,112 @@ __global__ void __launch_bounds__(MW * WAVE) q4_stream_kernel(const Q4Args a) {
             }
             s = 0.f;
         }
-        if (PK) xs[t][0] = r < 8 ? hi : lo;
-        else xs[t][0] = hi, xs[t][NS - 1] = lo;
+        xs[0] = hi, xs[NS - 1] = lo;
     }
 
     // a tile: this wave's share of its sums, in units of Y
-    auto product = [&](const Slice& s, f32x4 (&v)[RT]) {
-        f32x4 acc[RT], p[RT];
-#pragma unroll
-        for (int t = 0; t < RT; t++) acc[t] = p[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto product = [&](const Slice& s) {
+        f32x4 acc{0.f, 0.f, 0.f, 0.f}, p{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int j = 0; j < ST; j++) {
             const half8 b = q4_codes(s.code[j / 4][j % 4]);
 #pragma unroll
-            for (int n = 0; n < NA; n++)
-#pragma unroll
-                for (int t = 0; t < RT; t++) p[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xa[t][n][j], b, p[t], 0, 0, 0);
+            for (int n = 0; n < NA; n++) p = __builtin_amdgcn_mfma_f32_16x16x32_f16(xa[n][j], b, p, 0, 0, 0);
             if (j % SPG < SPG - 1) continue;
             const int g = j / SPG;
             uint32_t sw;  // (a slice of 4 or 2 groups begins in the middle of its block)
             if (Slice::GROUPS >= 8) sw = s.scale[g / 8][g % 8 / 2];
             else if (Slice::GROUPS == 4) sw = g0 % 8 ? s.scale[0][2 + g / 2] : s.scale[0][g / 2];
-            else if (Slice::GROUPS == 2) sw = s.scale[0][g0 / 2 % 4];
-            else sw = s.scale[0][g0 / 2 % 4] >> (16 * (g0 % 2));
-            const float sc = (float)__builtin_bit_cast(_Float16, (uint16_t)(Slice::GROUPS > 1 ? sw >> (16 * (g % 2)) : sw));
-#pragma unroll
-            for (int t = 0; t < RT; t++) {
-                acc[t] += p[t] * sc;
-                asm volatile("" : "+v"(acc[t]));  // (here, not sunk past the tile with p kept till then)
-                p[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-            }
+            else sw = s.scale[0][g0 / 2 % 4];
+            acc += p * q4_scale(sw >> (16 * (g % 2)));
+            asm volatile("" : "+v"(acc));  // (here, not sunk past the tile with p kept till then)
+            p = f32x4{0.f, 0.f, 0.f, 0.f};
             __builtin_amdgcn_sched_barrier(0);  // (codes are unpacked a group at a time: registers)
         }
-        const half8 mn = __builtin_bit_cast(half8, s.mins);
+        f32x4 v = acc * kCodeUnit;
 #pragma unroll
-        for (int t = 0; t < RT; t++) {
-            f32x4 am = acc[t] * kCodeUnit;
-            if constexpr (PRE) {
-                if (wave < nblocks) {
+        for (int n = 0; n < NS; n++) v = __builtin_amdgcn_mfma_f32_16x16x32_f16(xs[n], __builtin_bit_cast(half8, s.mins), v, 0, 0, 0);
 #pragma unroll
-                    for (int n = 0; n < 2; n++)
-                        am = __builtin_amdgcn_mfma_f32_16x16x32_f16(xsl[((wave * RT + t) * 2 + n) * WAVE + lane], mn, am, 0, 0, 0);
-                }
-                v[t] = am;
-            } else {
-#pragma unroll
-                for (int n = 0; n < NS; n++) am = __builtin_amdgcn_mfma_f32_16x16x32_f16(xs[t][n], mn, am, 0, 0, 0);
-#pragma unroll
-                for (int i = 0; i < 4; i++) v[t][i] = __builtin_ldexpf(PK ? pair_sum32(am[i]) : am[i], e4[t][i]);
-            }
-        }
+        for (int i = 0; i < 4; i++) v[i] = __builtin_ldexpf(PK ? pair_sum32(v[i]) : v[i], e4[i]);
+        return v;
     };
 
-    auto red = [&](int buf, int i, int k) -> f32x4& { return red_raw[((buf * SUMS + i) * KS + k) * WAVE + lane]; };
+    auto red = [&](int buf, int i, int k) -> f32x4& { return red_raw[((buf * 2 + i) * KS + k) * WAVE + lane]; };
     int buf = 0;
-    for (int t0 = blockIdx.x; t0 < tiles; t0 += 2 * gridDim.x) {
+    for (int t0 = blockIdx.x; t0 < tiles; t0 += 2 * gridDim.x, buf ^= 1) {
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             const int ct = t0 + h * gridDim.x;  // (the same for all waves)
-            if (ct < tiles) {
-                f32x4 v[RT];
-                product(sl[h], v);
-                load(sl[h], ct + 2 * gridDim.x);
+            if (ct >= tiles) break;
+            red(buf, h, wave) = product(sl[h]);
+            load(sl[h], ct + 2 * gridDim.x);
+        }
+        lds_barrier();  // (the other buffer's readers are past it when they reach the next one)
+        // the sums over the waves: lane (r, q) has rows 4 q .. 4 q + 3 of Y's column 16 ct + r
+        for (int h = wave; h < 2; h += KS) {
+            const int ct = t0 + h * gridDim.x, n = ct * 16 + r;
+            if (ct >= tiles) break;
+            f32x4 v = red(buf, h, 0);
+            for (int k = 1; k < KS; k++) v += red(buf, h, k);
+            if (n >= d.N) continue;
 #pragma unroll
-                for (int t = 0; t < RT; t++) red(buf, h % NB + t, wave) = v[t];
-            }
-            if (h % NB < NB - 1) continue;
-            lds_barrier();  // (the other buffer's readers are past it when they reach the next one)
-            // the sums over the waves: lane (r, q) has rows 4 q .. 4 q + 3 of Y's column 16 ct + r
-            for (int i = wave; i < SUMS; i += KS) {
-                const int t = RT == 1 ? 0 : i, tt = RT == 1 ? t0 + i * gridDim.x : ct, n = tt * 16 + r;
-                if (tt >= tiles) break;
-                f32x4 v = red(buf, i, 0);
-                for (int k = 1; k < KS; k++) v += red(buf, i, k);
-                if constexpr (PRE) {  // (one power of two for all slices of a row)
-                    const XOps o(a.M, NA, d);
-                    const int4 e = *((const int4*)((const unsigned char*)a.X + o.exps_at()) + min((size_t)(m0 / 16 + t), o.tiles - 1) * 4 + q);
-                    v = f32x4{__builtin_ldexpf(v[0], 7 - e.x), __builtin_ldexpf(v[1], 7 - e.y), __builtin_ldexpf(v[2], 7 - e.z),
-                              __builtin_ldexpf(v[3], 7 - e.w)};
-                }
-                if (n >= d.N) continue;
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const int m = 16 * t + 4 * q + j;
-                    if (m < M) {
-                        float* y = a.Y + (size_t)(m0 + m) * a.ldy + n;
-                        *y = a.accumulate ? *y + v[j] : v[j];
-                    }
+            for (int j = 0; j < 4; j++) {
+                const int m = 4 * q + j;
+                if (m < M) {
+                    float* y = a.Y + (size_t)(m0 + m) * a.ldy + n;
+                    *y = a.accumulate ? *y + v[j] : v[j];
                 }
             }
-            buf ^= 1;
         }
     }
 }
 
-template <typename TX, int SPG, bool PK, int RT, int CPS, int MW, bool PRE>
+// Tiles that each workgroup takes, one after the other, where a CU holds `per` workgroups and gy of them share a tile: as
+// many as fill the chip, every one as many tiles as the others.
+int stream_rounds(int tiles, int gy, int per) {
+    const int most = std::max(1, 256 * per / gy);
+    return (tiles + most - 1) / most;
+}
+
+template <typename TX, int SPG, int CPS, int MW, bool FEW>
 int launch_stream(const Q4Args& a, hipStream_t st) {
-    const int ks = std::min(MW, (a.d.chunks() - a.c0 + CPS - 1) / CPS), tiles = a.d.tiles(), gy = (a.M + 16 * RT - 1) / (16 * RT);
-    // 16 waves per CU, or 8 with X's operands in twice the registers; every workgroup as many tiles as the others
-    const int cu = PRE ? 8 : 16, most = std::max(1, 256 * std::max(1, cu / ks) / gy), rounds = (tiles + most - 1) / most;
-    const int lds = ((RT < 2 ? 4 : 2 * RT) * ks + (PRE ? (a.d.K / a.d.G + 31) / 32 * 2 * RT : 0)) * 1024;
+    const int ks = std::min(MW, (a.d.chunks() - a.c0 + CPS - 1) / CPS), tiles = a.d.tiles(), gy = (a.M + 15) / 16;
+    const int rounds = stream_rounds(tiles, gy, MW / ks);
+    const int lds = 4 * ks * 1024 + (FEW ? ks * staged_bytes(a.M, std::is_same<TX, float>::value ? 2 : 1) : 0);
     if (lds > 65536)
-        AEG_HIP(hipFuncSetAttribute((const void*)q4_stream_kernel<TX, SPG, PK, RT, CPS, MW, PRE>,
+        AEG_HIP(hipFuncSetAttribute((const void*)q4_stream_kernel<TX, SPG, CPS, MW, FEW>,
                                     hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-    q4_stream_kernel<TX, SPG, PK, RT, CPS, MW, PRE><<<dim3((tiles + rounds - 1) / rounds, gy), ks * WAVE,
-                                                      lds, st>>>(a);
+    q4_stream_kernel<TX, SPG, CPS, MW, FEW><<<dim3((tiles + rounds - 1) / rounds, gy), ks * WAVE, lds, st>>>(a);
     return after_launch("linear_q4");
 }
 
-template <typename TX, bool PK, int RT, int CPS, int MW, bool PRE>
-int stream_spg(const Q4Args& a, hipStream_t st) {
-    switch (a.d.G) {
-        case 32: return launch_stream<TX, 1, PK, RT, CPS, MW, PRE>(a, st);
-        case 64: return launch_stream<TX, 2, PK, RT, CPS, MW, PRE>(a, st);
-        default: return launch_stream<TX, 4, PK, RT, CPS, MW, PRE>(a, st);
-    }
+// K in blocks that the waves' slices hold
+template <typename TX, int CPS, int MW, bool FEW = false>
+int run_stream(Q4Args a, hipStream_t st) {
+    int rc = 0;
+    for (a.c0 = 0; a.c0 < a.d.chunks() && !rc; a.c0 += CPS * MW, a.accumulate = 1) switch (a.d.G) {
+            case 32: rc = launch_stream<TX, 1, CPS, MW, FEW>(a, st); break;
+            case 64: rc = launch_stream<TX, 2, CPS, MW, FEW>(a, st); break;
+            default: rc = launch_stream<TX, 4, CPS, MW, FEW>(a, st);
+        }
+    return rc;
+}
+
+int run_stream(const Q4Args& a, int x_dtype, hipStream_t st) {
+    const bool few = a.M <= kStaged;
+    if (x_dtype == AEGIST_BF16) return few ? run_stream<uint16_t, 2, 16, true>(a, st) : run_stream<uint16_t, 2, 16>(a, st);
+    if (few) return run_stream<float, 2, 16, true>(a, st);
+    // twice the registers per row: 8 waves
+    return a.d.K > 2048 ? run_stream<float, 4, 8>(a, st) : run_stream<float, 2, 8>(a, st);
 }
 
 // ---------------------------------------------------------------------------------------------
-// Many rows: tiles of 128 rows of X x 256 of W, 8 waves of 64 x 64. X's operands go from the workspace straight into
+// Many rows: tiles of 128 rows of X x 256 of W, 8 waves of 128 x 32 (so that no two unpack the same codes). X's operands go from the workspace straight into
 // LDS (1 KB pieces as they lie there: no bank conflicts, no swizzle), 128 k to a stage; codes go from global memory to
 // registers and are unpacked in the wave that uses them. Both are requested two stages ahead (fp32 X: one, of
 // twice the products: LDS). The sums of a group join
 // the tile's in fp32 (one FMA per 32 products and lane).
-constexpr int GM = 128, GN = 256, GR = 4, GC = 4;  // tile; a wave's 16 x 16 tiles
+constexpr int GM = 128, GN = 256, GR = 8, GC = 2;  // tile; a wave's 16 x 16 tiles
 
 // 16 bytes per lane straight from global memory into LDS at lds + 16 lane (lds uniform)
 __device__ __forceinline__ void q4_g2lds(const void* src, void* lds) {
@@ -447,7 +476,7 @@ __global__ void __launch_bounds__(512) q4_gemm_kernel(const Q4Args a, int tiles_
     const Q4Ptr w = q4_ptr(a.W, d);
     const XOps o(a.M, P, d);
     const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
-    const int r = lane % 16, q = lane / 16, wm = wave % 2, wn = wave / 2;
+    const int r = lane % 16, q = lane / 16;
     const int KC = d.chunks(), B8 = d.blocks8(), tiles = d.tiles(), xt = (int)o.tiles;
 
     // this wave's pieces of X per stage: one tile of 16 rows, all its parts and steps
@@ -461,7 +490,7 @@ __global__ void __launch_bounds__(512) q4_gemm_kernel(const Q4Args a, int tiles_
     };
     int nt[GC];
 #pragma unroll
-    for (int n = 0; n < GC; n++) nt[n] = min(bn * 16 + wn * 4 + n, tiles - 1);
+    for (int n = 0; n < GC; n++) nt[n] = min(bn * 16 + wave * GC + n, tiles - 1);
     u4v code[NB][GC];
     u2v sc[NB][GC];
     auto load = [&](int buf, int c) {
@@ -496,7 +525,7 @@ __global__ void __launch_bounds__(512) q4_gemm_kernel(const Q4Args a, int tiles_
         for (int m = 0; m < GR; m++)
 #pragma unroll
             for (int p = 0; p < 2; p++) {
-                const half8 x = sums[(((size_t)min(bm * 8 + wm * 4 + m, xt - 1) * 2 + p) * o.blocks + b) * 64 + lane];
+                const half8 x = sums[(((size_t)min(bm * 8 + m, xt - 1) * 2 + p) * o.blocks + b) * 64 + lane];
 #pragma unroll
                 for (int n = 0; n < GC; n++) acc[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, mn[n], acc[m][n], 0, 0, 0);
             }
@@ -515,12 +544,11 @@ __global__ void __launch_bounds__(512) q4_gemm_kernel(const Q4Args a, int tiles_
             stage((buf + NB - 1) % NB, c + NB - 1);
             load((buf + NB - 1) % NB, c + NB - 1);
         }
-        const unsigned char* x = lds + buf * BUF + wm * 4 * P * 4096 + lane * 16;
-        half8 xa[2][P][U][GR];
+        const unsigned char* x = lds + buf * BUF + lane * 16;
+        half8 xa[P][U][GR];
         constexpr int XF = P * U * GR;  // operands of a unit, products of a unit's tile
-        auto operand = [&](int u, int i) {
-            const int m = i % GR, s = i / GR % U, pt = i / GR / U;
-            xa[u % 2][pt][s][m] = *(const half8*)(x + ((m * P + pt) * 4 + u * U + s) * 1024);
+        auto operand = [&](int u, int s, int pt, int m) {
+            xa[pt][s][m] = *(const half8*)(x + ((m * P + pt) * 4 + u * U + s) * 1024);
         };
         half8 b[2][U];
         auto unpack = [&](int i) {
@@ -530,7 +558,7 @@ __global__ void __launch_bounds__(512) q4_gemm_kernel(const Q4Args a, int tiles_
         f32x4 p[2][GR];
         auto join = [&](int i) {
             const int u = i / GC, n = i % GC, g = u * U / SPG;
-            const float f = (float)__builtin_bit_cast(_Float16, (uint16_t)(sc[buf][n][g / 2] >> (16 * (g % 2))));
+            const float f = q4_scale(sc[buf][n][g / 2] >> (16 * (g % 2)));
 #pragma unroll
             for (int m = 0; m < GR; m++) {
                 acc[m][n] += p[i % 2][m] * f;
@@ -538,34 +566,37 @@ __global__ void __launch_bounds__(512) q4_gemm_kernel(const Q4Args a, int tiles_
             }
         };
 #pragma unroll
-        for (int i = 0; i < XF; i++) operand(0, i);
+        for (int s = 0; s < U; s++)
+#pragma unroll
+            for (int pt = 0; pt < P; pt++)
+#pragma unroll
+                for (int m = 0; m < GR; m++) operand(0, s, pt, m);
         unpack(0);
         __builtin_amdgcn_sched_barrier(0);
-        // tile i: its products, and between them the codes of the next one, the FMAs of the one before and a share of the
-        // next unit's operands
+        // tile i: its products, and between them the codes of the next one, the FMAs of the one before and, in a unit's
+        // last tile, the next unit's operands in the place of those just used
         constexpr int IS = 4 / U * GC;
 #pragma unroll
         for (int i = 0; i < IS; i++) {
             const int u = i / GC;
-            if (u + 1 < 4 / U) {
-#pragma unroll
-                for (int k = 0; k < XF / GC; k++) operand(u + 1, i % GC * (XF / GC) + k);
-            }
+            const bool last = i % GC == GC - 1 && u + 1 < 4 / U;
 #pragma unroll
             for (int s = 0; s < U; s++)
 #pragma unroll
                 for (int pt = 0; pt < P; pt++)
 #pragma unroll
-                    for (int m = 0; m < GR; m++)
+                    for (int m = 0; m < GR; m++) {
                         p[i % 2][m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                            xa[u % 2][pt][s][m], b[i % 2][s], s == 0 && pt == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : p[i % 2][m], 0, 0, 0);
+                            xa[pt][s][m], b[i % 2][s], s == 0 && pt == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : p[i % 2][m], 0, 0, 0);
+                        if (last) operand(u + 1, s, pt, m);
+                    }
             if (i + 1 < IS) unpack(i + 1);
             if (i > 0) join(i - 1);
             constexpr int VALU = (7 * U + 4 * GR + 2 + XF - 1) / XF;  // per product
 #pragma unroll
             for (int k = 0; k < XF; k++) {
                 __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                if (k < XF / GC) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                if (last) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
                 __builtin_amdgcn_sched_group_barrier(0x002, VALU, 0);
             }
             __builtin_amdgcn_sched_barrier(0);
@@ -581,12 +612,12 @@ __global__ void __launch_bounds__(512) q4_gemm_kernel(const Q4Args a, int tiles_
     const int* exps = (const int*)((const unsigned char*)a.X + o.exps_at());
 #pragma unroll
     for (int m = 0; m < GR; m++) {
-        const int row = bm * GM + (wm * 4 + m) * 16 + 4 * q;
+        const int row = bm * GM + m * 16 + 4 * q;
         const int4 e = *(const int4*)(exps + min(row, xt * 16 - 4));
         const int es[4] = {18 - e.x, 18 - e.y, 18 - e.z, 18 - e.w};
 #pragma unroll
         for (int n = 0; n < GC; n++) {
-            const int col = (bn * 16 + wn * 4 + n) * 16 + r;
+            const int col = (bn * 16 + wave * GC + n) * 16 + r;
 #pragma unroll
             for (int i = 0; i < 4; i++)
                 if (row + i < a.M && col < d.N) {
@@ -616,30 +647,33 @@ int gemm_spg(const Q4Args& a, hipStream_t st) {
     }
 }
 
-// Rows of X and K that the stream takes with X's rows as they are, and as operands (K in blocks of 2048, the minima of
-// all of it in the first).
-bool stream_fits(int M, const Q4Dims& d) { return M <= 16 && d.K <= 4096; }
-bool pre_fits(int M, const Q4Dims& d) { return M <= 256 && d.K <= 8192; }
-
-int run_stream(const Q4Args& a, int x_dtype, hipStream_t st) {
-    if (x_dtype == AEGIST_BF16) return stream_spg<uint16_t, false, 1, 2, 16, false>(a, st);
-    if (a.M <= 8) return stream_spg<float, true, 1, 2, 16, false>(a, st);
-    return a.d.K > 2048 ? stream_spg<float, false, 1, 4, 8, false>(a, st) : stream_spg<float, false, 1, 2, 8, false>(a, st);
+// Whether the stream takes M rows, or the 128 x 256 tiles: the shorter by these estimates (us, fitted to M 200 to 2000,
+// N 512 to 32768, K 512 to 4096, where the choice is at most 8% above the faster). The stream: 1.2 per round of tiles
+// (fp32 X 0.95, 1.4 in slices of 512), all rows of X at once; 1000 rows of 8192 x 2048, bf16: 81, tiles 54; of 512 x
+// 2048: 13, tiles 43. The tiles: rounds of 256 workgroups, each a walk along K.
+bool use_stream(int x_dtype, int M, const Q4Dims& d) {
+    if (M <= 16) return true;
+    const bool f32 = x_dtype == AEGIST_F32;
+    const int gy = (M + 15) / 16, KC = d.chunks(), cps = f32 && d.K > 2048 ? 4 : 2, mw = f32 ? 8 : 16;
+    if (gy > 65535) return false;
+    double stream = 7, gemm = 4;
+    for (int c = 0; c < KC; c += cps * mw) {
+        const int per = mw / std::min(mw, (KC - c + cps - 1) / cps), slots = 256 * per;
+        stream += (double)stream_rounds(d.tiles(), gy, per) * ((gy + slots - 1) / slots) * (f32 ? cps == 4 ? 1.4 : 0.95 : 1.2);
+    }
+    const double groups = (double)((M + GM - 1) / GM) * ((d.N + GN - 1) / GN);
+    gemm += std::ceil(groups / 256) * (f32 ? 13 + 28.0 / 8 * KC : 8 + 17.5 / 8 * KC);
+    return stream <= gemm;
 }
 
-int run_rows(Q4Args a, int x_dtype, void* ws, hipStream_t st) {
+int run_gemm(Q4Args a, int x_dtype, void* ws, hipStream_t st) {
     const int tiles = (a.M + 15) / 16;
     if (x_dtype == AEGIST_F32) q4_rows_kernel<float><<<tiles, XW * WAVE, 0, st>>>(a, (unsigned char*)ws);
     else q4_rows_kernel<uint16_t><<<tiles, XW * WAVE, 0, st>>>(a, (unsigned char*)ws);
     int rc = after_launch("linear_q4");
     if (rc) return rc;
     a.X = ws;
-    if (!pre_fits(a.M, a.d)) return x_dtype == AEGIST_F32 ? gemm_spg<2>(a, st) : gemm_spg<1>(a, st);
-    for (a.c0 = 0; a.c0 < a.d.chunks() && !rc; a.c0 += 16, a.accumulate = 1)
-        rc = x_dtype == AEGIST_F32 ? stream_spg<float, false, 2, 2, 8, true>(a, st)
-             : a.M <= 32           ? stream_spg<uint16_t, false, 2, 2, 8, true>(a, st)
-                                   : stream_spg<uint16_t, false, 4, 2, 8, true>(a, st);
-    return rc;
+    return x_dtype == AEGIST_F32 ? gemm_spg<2>(a, st) : gemm_spg<1>(a, st);
 }
 
 }  // namespace
@@ -648,7 +682,11 @@ namespace aegist {
 
 size_t linear_q4_workspace(int x_dtype, int M, int N, int K, int G) {
     const Q4Dims d{N, K, G};
-    return M == 0 || N == 0 || stream_fits(M, d) ? 0 : XOps(M, x_dtype == AEGIST_F32 ? 2 : 1, d).bytes();
+    if (N == 0) return 0;
+    // (what the choice of any smaller M needs is enough for it)
+    for (long long m = 32; m < M + 16; m += 16)
+        if (!use_stream(x_dtype, (int)std::min<long long>(m, M), d)) return XOps(M, x_dtype == AEGIST_F32 ? 2 : 1, d).bytes();
+    return 0;
 }
 
 int launch_linear_q4(const void* X, int x_dtype, long long ldx, const void* W, float* Y, long long ldy, int M, int N,
@@ -667,9 +705,10 @@ int launch_linear_q4(const void* X, int x_dtype, long long ldx, const void* W, f
     if ((uintptr_t)W % 16) return fail(AEGIST_ERR_SHAPE, "linear_q4: W must be 16-byte aligned");
     const Q4Dims d{N, K, G};
     const Q4Args a{X, ldx, (const unsigned char*)W, Y, ldy, M, accumulate, d, 0};
-    if (stream_fits(M, d)) return run_stream(a, x_dtype, st);
-    if ((rc = check_workspace(ws, ws_bytes, linear_q4_workspace(x_dtype, M, N, K, G), "linear_q4"))) return rc;
-    return run_rows(a, x_dtype, ws, st);
+    if (use_stream(x_dtype, M, d)) return run_stream(a, x_dtype, st);
+    rc = check_workspace(ws, ws_bytes, XOps(M, x_dtype == AEGIST_F32 ? 2 : 1, d).bytes(), "linear_q4");
+    if (rc) return rc;
+    return run_gemm(a, x_dtype, ws, st);
 }
 
 }  // namespace aegist
