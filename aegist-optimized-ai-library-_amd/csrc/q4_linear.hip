@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(XW * WAVE) q4_rows_kernel(const Q4Args a, unsi
 // Up to kStaged rows are scaled one after the other, 4 values of the slice per lane, and pass through the wave's own LDS
 // into the operands: a lane that makes its operands itself makes those of row r % M, the same as the others of that row
 // (8192 x 2048, one row: 9.0 -> 7 us).
-constexpr int kStaged = 4;
+constexpr int kStaged = 2;
 // per wave: rows [M][parts][256 fp16], sums [M][2][8 fp16], exponents [4]
 __host__ __device__ constexpr int staged_bytes(int M, int parts) { return M * (parts * 512 + 32) + 16; }
 
@@ -253,37 +253,42 @@ __global__ void __launch_bounds__(MW * WAVE) q4_stream_kernel(const Q4Args a) {
         unsigned char* own = (unsigned char*)(red_raw + 4 * KS * WAVE) + wave * staged_bytes(M, PARTS);
         unsigned char *own_s = own + M * PARTS * 512, *own_e = own_s + M * 32;
         const int k = c0 * 128 + 4 * lane, kk = min(k, d.K - 4);
-        for (int m = 0; m < M; m++) {
-            float f[4];
-            const TX* x = (const TX*)a.X + (size_t)(m0 + m) * a.ldx + kk;
+        float f[kStaged][4];
+#pragma unroll
+        for (int m = 0; m < kStaged; m++) {
+            const TX* x = (const TX*)a.X + (size_t)(m0 + min(m, M - 1)) * a.ldx + kk;
             if constexpr (F32) {
                 const f32x4 v = *(const f32x4*)x;
 #pragma unroll
-                for (int i = 0; i < 4; i++) f[i] = v[i];
+                for (int i = 0; i < 4; i++) f[m][i] = v[i];
             } else {
                 const u2v v = *(const u2v*)x;
-                f[0] = bf_lo(v[0]), f[1] = bf_hi(v[0]), f[2] = bf_lo(v[1]), f[3] = bf_hi(v[1]);
+                f[m][0] = bf_lo(v[0]), f[m][1] = bf_hi(v[0]), f[m][2] = bf_lo(v[1]), f[m][3] = bf_hi(v[1]);
             }
+        }
+        if (lane < 8 * M) ((uint32_t*)own_s)[lane] = 0;
+        wave_sync();
 #pragma unroll
-            for (int i = 0; i < 4; i++) f[i] = k < d.K ? f[i] : 0.f;
-            const int e = row_exp(wave_max(fmaxf(fmaxf(fabsf(f[0]), fabsf(f[1])), fmaxf(fabsf(f[2]), fabsf(f[3])))));
+        for (int m = 0; m < kStaged; m++) {
+            if (m >= M) break;  // (the same for all lanes)
+#pragma unroll
+            for (int i = 0; i < 4; i++) f[m][i] = k < d.K ? f[m][i] : 0.f;
+            const int e = row_exp(wave_max(fmaxf(fmaxf(fabsf(f[m][0]), fabsf(f[m][1])), fmaxf(fabsf(f[m][2]), fabsf(f[m][3])))));
             half4 hi, lo;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const float v = __builtin_ldexpf(f[i], e);
+                const float v = __builtin_ldexpf(f[m][i], e);
                 hi[i] = (_Float16)v;
                 lo[i] = (_Float16)(v - (float)hi[i]);
             }
             *(half4*)(own + m * PARTS * 512 + lane * 8) = hi;
             if (F32) *(half4*)(own + (m * PARTS + 1) * 512 + lane * 8) = lo;
             // the group's sum, from 8, 16 or 32 lanes, to its place among the 8 of its block
-            float s = (f[0] + f[1]) + (f[2] + f[3]);
+            float s = (f[m][0] + f[m][1]) + (f[m][2] + f[m][3]);
 #pragma unroll
             for (int o = 1; o < 8 * SPG; o *= 2) s += __shfl_xor(s, o, WAVE);
             s = __builtin_ldexpf(s, e - 7);
             const _Float16 sh = (_Float16)s;
-            if (lane < 16) ((_Float16*)(own_s + m * 32))[lane] = 0;
-            wave_sync();
             if (lane % (8 * SPG) == 0) {
                 const int g = (g0 + lane / (8 * SPG)) % 8;
                 ((_Float16*)(own_s + m * 32))[g] = sh;
