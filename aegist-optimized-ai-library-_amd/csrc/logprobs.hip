@@ -27,7 +27,6 @@ constexpr int MAX_TOP = 64;
 constexpr int NT = 256, NW = NT / WAVE;  // threads, waves
 constexpr int CAP = 512;                 // candidates that are ranked at once
 
-typedef uint32_t u4v __attribute__((ext_vector_type(4)));
 typedef unsigned long long u64;
 
 // Order of the alternatives as one number: the larger value first (NaN before all, -0 as +0), then the lower
@@ -121,6 +120,19 @@ struct Lds {
     u64 list[MAX_TOP];         // the alternatives so far, descending
 };
 
+// Largest value of the wave by DPP steps (as wave_sum_dpp), in every lane
+__device__ __forceinline__ float wave_max_dpp(float v) {
+#define AEG_DPP_MAX(CTRL, ROWS) \
+    v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(v), __float_as_int(v), CTRL, ROWS, 0xF, false)))
+    AEG_DPP_MAX(0x111, 0xF);  // row_shr:1
+    AEG_DPP_MAX(0x112, 0xF);
+    AEG_DPP_MAX(0x114, 0xF);
+    AEG_DPP_MAX(0x118, 0xF);
+    AEG_DPP_MAX(0x142, 0xA);  // row_bcast:15 to rows 1 and 3
+    AEG_DPP_MAX(0x143, 0xC);  // row_bcast:31 to rows 2 and 3
+#undef AEG_DPP_MAX
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), WAVE - 1));
+}
 __device__ __forceinline__ float lane_value(float v, int j) {
     return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), j));
 }
@@ -131,7 +143,7 @@ __device__ __forceinline__ float nth_value(float v, int top) {
     int r = 0;
 #pragma unroll 16
     for (int j = 0; j < WAVE; j++) r += lane_value(v, j) > v;
-    return -wave_max(r < top ? -v : -INFINITY);
+    return -wave_max_dpp(r < top ? -v : -INFINITY);
 }
 // The same of 64 different keys, or 0 for lanes without one; 0 if there are too few.
 __device__ __forceinline__ u64 nth_key(u64 k, int top) {
@@ -247,11 +259,12 @@ __global__ void __launch_bounds__(NT) logprobs_kernel(const T* __restrict__ L, l
                         v[i].set(e, ce < c1 ? Act<T>::ld(x, ce) : -INFINITY);
                     }
             }
+            if (b == c0 && tok >= c0 && tok < c1) p.tok = Act<T>::ld(x, tok);  // (with the segment's, not after it)
             float mt = -INFINITY;  // the thread's largest (NaN apart)
 #pragma unroll
             for (int i = 0; i < VPT; i++)
                 mt = fmaxf(fmaxf(fmaxf(mt, v[i].get(0)), fmaxf(v[i].get(1), v[i].get(2))), v[i].get(3));
-            const float mw = wave_max(mt);
+            const float mw = wave_max_dpp(mt);
             // the alternatives' lower bound: from the first segment's lanes, then from the list
             const float nth = top && have < top ? nth_value(mt, top) : 0.f;
             if (lane == 0) {
@@ -278,8 +291,8 @@ __global__ void __launch_bounds__(NT) logprobs_kernel(const T* __restrict__ L, l
                 q.z = z[0] + z[1];
                 q.s = (y2[0] + y2[1]) * LN2;
             }
-            q.z = wave_sum(q.z);
-            q.s = wave_sum(q.s);
+            q.z = wave_sum_dpp(q.z);
+            q.s = wave_sum_dpp(q.s);
             if (lane == 0) s.red[1][wave] = q.z, s.red[2][wave] = q.s;
             bool few = true;
             if (top) {
@@ -334,7 +347,6 @@ __global__ void __launch_bounds__(NT) logprobs_kernel(const T* __restrict__ L, l
             __syncthreads();
             join(p, q);
         }
-        if (tok >= c0 && tok < c1) p.tok = Act<T>::ld(x, tok);
         if (all_splits == 1) {
             if (threadIdx.x == 0) finish(o, t, V, p);
             if ((int)threadIdx.x < top) finish_top(o, t, threadIdx.x, p, s.list[threadIdx.x]);
@@ -361,10 +373,10 @@ __global__ void __launch_bounds__(NT) logprobs_join_kernel(const Part* __restric
         for (int i = 0; i < N; i++) k[i] = (int)threadIdx.x + NT * i < n ? keys[threadIdx.x + NT * i] : 0;
         Part p{-INFINITY, 0.f, 0.f, -INFINITY, 0, {}};
         for (int i = threadIdx.x; i < splits; i += NT) join(p, parts[(size_t)t * splits + i]);
-        const float m = wave_max(p.m), f = p.m == -INFINITY ? 0.f : p.m == m ? 1.f : expf(p.m - m);
-        p.s = wave_sum(f > 0.f ? f * fmaf(p.m - m, p.z, p.s) : 0.f);
-        p.z = wave_sum(f * p.z);
-        p.tok = wave_max(p.tok);
+        const float m = wave_max_dpp(p.m), f = p.m == -INFINITY ? 0.f : p.m == m ? 1.f : expf(p.m - m);
+        p.s = wave_sum_dpp(f > 0.f ? f * fmaf(p.m - m, p.z, p.s) : 0.f);
+        p.z = wave_sum_dpp(f * p.z);
+        p.tok = wave_max_dpp(p.tok);
         p.bad = __any(p.bad);
         p.m = m;
         if (splits > WAVE) {
@@ -401,9 +413,9 @@ int check_out(const char* who, int T, int V, const LogprobOut& o) {
     return 0;
 }
 
-// Logits of a split: few rows are cut so that about 1024 workgroups share them.
+// Logits of a split: few rows are cut so that about 1536 workgroups share them (6 per CU at once).
 int split_span(int T, int cols, int* small) {
-    const long long want = std::max(1LL, 1024LL / std::max(T, 1));
+    const long long want = std::max(1LL, 1536LL / std::max(T, 1));
     const int seg = 4 * 4 * NT;  // a segment of the small form
     long long span = (cols + want - 1) / want;
     *small = span <= 2 * seg;

@@ -44,6 +44,30 @@ __host__ __device__ inline Q4Ptr q4_ptr(const void* w, const Q4Dims& d) {
     return {p, (const _Float16*)(p + d.code_bytes()), (const _Float16*)(p + d.code_bytes() + d.scale_bytes())};
 }
 
+typedef uint32_t u4v __attribute__((ext_vector_type(4)));
+
+// 8 consecutive values of a row (k a multiple of 8; rows 16-byte aligned)
+template <typename T> struct X8;
+template <> struct X8<float> {
+    f32x4 v[2];
+    // zeros where k is past the row's K (a multiple of 8)
+    __device__ __forceinline__ void load(const float* row, int k, int K) {
+        const f32x4* p = (const f32x4*)(row + min(k, K - 8));
+        const f32x4 a = p[0], b = p[1];
+        v[0] = k < K ? a : f32x4{0, 0, 0, 0};
+        v[1] = k < K ? b : f32x4{0, 0, 0, 0};
+    }
+    __device__ __forceinline__ float get(int i) const { return v[i / 4][i % 4]; }
+};
+template <> struct X8<uint16_t> {
+    u4v v;
+    __device__ __forceinline__ void load(const uint16_t* row, int k, int K) {
+        const u4v a = *(const u4v*)(row + min(k, K - 8));
+        v = k < K ? a : u4v{0, 0, 0, 0};
+    }
+    __device__ __forceinline__ float get(int i) const { return i % 2 ? bf_hi(v[i / 2]) : bf_lo(v[i / 2]); }
+};
+
 // AEGIST_OK, or the error of sizes that no Q4 weight has.
 int check_q4(const char* who, int N, int K, int G);
 size_t linear_q4_workspace(int x_dtype, int M, int N, int K, int G);

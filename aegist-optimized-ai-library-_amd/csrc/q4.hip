@@ -7,16 +7,23 @@ using namespace aegist;
 
 namespace {
 
-typedef uint32_t u4v __attribute__((ext_vector_type(4)));
-
 // index of (row n, group g) in the scale and min sections
 __device__ __forceinline__ size_t q4_group(const Q4Dims& d, int n, int g) {
     return ((size_t)(n / 16) * d.blocks8() + g / 8) * 128 + (n % 16) * 8 + g % 8;
 }
 
+// (w - mn) / sc rounded to the nearest, ties to even, in 0..15, as doubles decide it. In fp32 the quotient is off by at
+// most 15.5 * 3 * 2^-24 < 2^-18, so only within 2^-16 of a half can doubles say otherwise: 1 value in 30000, and the
+// division in doubles is left to those (8 M values: 28 us with it for all, bf16, 9 so).
+__device__ __forceinline__ uint32_t q4_code(float w, _Float16 mn, _Float16 sc, float inv) {
+    const float q = (w - (float)mn) * inv, f = q - floorf(q);
+    float c = __builtin_rintf(q);
+    if (fabsf(f - 0.5f) < 0x1p-16f) c = (float)rint(((double)w - (double)mn) / (double)sc);
+    return (uint32_t)fminf(fmaxf(c, 0.f), 15.f);
+}
+
 // One wave per 16 rows x 128 k. Lane 16 q + r holds the runs k = 32 j + 8 q .. + 7 of row r, so a group's extremes
-// are its own values' and, over the four q, two exchanges'. The code is decided in doubles: w - min and its
-// quotient by the scale next to a half would round either way in fp32.
+// are its own values' and, over the four q, two exchanges'.
 template <typename TW>
 __global__ void __launch_bounds__(256) q4_quantize_kernel(const TW* __restrict__ W, long long ldw, unsigned char* out,
                                                           const Q4Dims d) {
@@ -25,24 +32,20 @@ __global__ void __launch_bounds__(256) q4_quantize_kernel(const TW* __restrict__
     if (c >= d.chunks() || nt >= d.tiles()) return;
     const int n = nt * 16 + r;
     const bool row = n < d.N;
-    float w[4][8];
+    X8<TW> w[4];
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-        const int k = c * 128 + 32 * j + 8 * q;
-#pragma unroll
-        for (int e = 0; e < 8; e++) w[j][e] = row && k < d.K ? Act<TW>::ld(W, (size_t)n * ldw + k + e) : 0.f;
-    }
+    for (int j = 0; j < 4; j++) w[j].load(W + (size_t)min(n, d.N - 1) * ldw, c * 128 + 32 * j + 8 * q, d.K);
     float lo[4], hi[4];
     bool bad[4];
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-        lo[j] = hi[j] = w[j][0];
+        lo[j] = hi[j] = w[j].get(0);
         bad[j] = false;
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            lo[j] = fminf(lo[j], w[j][e]);
-            hi[j] = fmaxf(hi[j], w[j][e]);
-            bad[j] |= !(fabsf(w[j][e]) <= 65504.f);
+            lo[j] = fminf(lo[j], w[j].get(e));
+            hi[j] = fmaxf(hi[j], w[j].get(e));
+            bad[j] |= !(fabsf(w[j].get(e)) <= 65504.f);
         }
     }
     const int span = d.G / 32;  // runs of 32 k per group
@@ -77,19 +80,23 @@ __global__ void __launch_bounds__(256) q4_quantize_kernel(const TW* __restrict__
         const _Float16 mn = bad[j] ? (_Float16)__builtin_nanf("") : (_Float16)lo[j];
         const double range = ((double)hi[j] - (double)mn) / 15.0;
         const _Float16 sc = range > 0.0 ? (_Float16)range : (_Float16)0.f;
-        uint32_t p = 0;
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const double v = sc > (_Float16)0.f ? rint(((double)w[j][e] - (double)mn) / (double)sc) : 0.0;
-            p |= q4_put((uint32_t)(int)fmin(fmax(v, 0.0), 15.0), e);
-        }
         const int k = c * 128 + 32 * j;
-        codes[j] = row && k < d.K ? p : 0;
-        if (q == 0 && row && k < d.K && k % d.G == 0) {
-            scale[q4_group(d, n, k / d.G)] = sc;
-            mins[q4_group(d, n, k / d.G)] = mn;
+        const bool in = row && k < d.K;
+        uint32_t p = 0;
+        if (sc > (_Float16)0.f) {
+            const float inv = 1.f / (float)sc;
+#pragma unroll
+            for (int e = 0; e < 8; e++) p |= q4_put(q4_code(w[j].get(e), mn, sc, inv), e);
+        }
+        codes[j] = in ? p : 0;
+        // (the rows past N and the groups past K too: zeros)
+        if (q == 0 && k % d.G == 0 && k / d.G < d.blocks8() * 8) {
+            scale[q4_group(d, n, k / d.G)] = in ? sc : (_Float16)0.f;
+            mins[q4_group(d, n, k / d.G)] = in ? mn : (_Float16)0.f;
         }
     }
+    if (c == d.chunks() - 1 && q == 0)
+        for (int g = d.chunks() * (128 / d.G); g < d.blocks8() * 8; g++) scale[q4_group(d, n, g)] = mins[q4_group(d, n, g)] = 0;
     ((u4v*)out)[((size_t)nt * d.chunks() + c) * 64 + lane] = codes;
 }
 
@@ -114,17 +121,15 @@ __global__ void __launch_bounds__(256) q4_pack_kernel(const unsigned char* __res
     ((u4v*)out)[((size_t)nt * d.chunks() + c) * 64 + lane] = v;
 }
 
-// Scales and minima from rows [N, K / G], or (src null) zeros in the places that no group has.
+// Scales and minima from rows [N, K / G], with zeros in the places that no group has.
 __global__ void __launch_bounds__(256) q4_pack_groups_kernel(const _Float16* __restrict__ scale,
                                                              const _Float16* __restrict__ mins, unsigned char* out,
-                                                             const Q4Dims d, bool fill) {
+                                                             const Q4Dims d) {
     const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x, all = d.scale_bytes() / 2;
     if (i >= all) return;
     const int g = (int)(i / 128 % d.blocks8()) * 8 + i % 8, n = (int)(i / 128 / d.blocks8()) * 16 + i / 8 % 16;
-    const bool in = n < d.N && g < d.K / d.G;
-    if (!fill && in) return;
     _Float16 s = 0, m = 0;
-    if (in) {
+    if (n < d.N && g < d.K / d.G) {
         s = scale[(size_t)n * (d.K / d.G) + g];
         m = mins ? mins[(size_t)n * (d.K / d.G) + g] : (_Float16)(-8.f * (float)s);
     }
@@ -192,11 +197,6 @@ extern "C" int aegist_q4_quantize(const void* W, int w_dtype, long long ldw, voi
         return fail(AEGIST_ERR_SHAPE, "q4_quantize: W needs 16-byte aligned rows (ldw >= K)");
     const Q4Dims d{N, K, group};
     const hipStream_t st = AEG_STREAM(stream);
-    if (N % 16 || K / group % 8) {
-        q4_pack_groups_kernel<<<(unsigned)((d.scale_bytes() / 2 + 255) / 256), 256, 0, st>>>(nullptr, nullptr,
-                                                                                             (unsigned char*)q4, d, false);
-        if ((rc = after_launch("q4_quantize"))) return rc;
-    }
     if (w_dtype == AEGIST_F32)
         q4_quantize_kernel<float><<<q4_grid(d), 256, 0, st>>>((const float*)W, ldw, (unsigned char*)q4, d);
     else
@@ -216,7 +216,7 @@ extern "C" int aegist_q4_pack(const void* codes, const uint16_t* scale, const ui
     q4_pack_kernel<<<q4_grid(d), 256, 0, st>>>((const unsigned char*)codes, (unsigned char*)q4, d);
     if ((rc = after_launch("q4_pack"))) return rc;
     q4_pack_groups_kernel<<<(unsigned)((d.scale_bytes() / 2 + 255) / 256), 256, 0, st>>>(
-        (const _Float16*)scale, (const _Float16*)mins, (unsigned char*)q4, d, true);
+        (const _Float16*)scale, (const _Float16*)mins, (unsigned char*)q4, d);
     return after_launch("q4_pack");
 }
 

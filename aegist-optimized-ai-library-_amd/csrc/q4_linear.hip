@@ -25,7 +25,6 @@ using namespace aegist;
 
 namespace {
 
-typedef uint32_t u4v __attribute__((ext_vector_type(4)));
 typedef uint32_t u2v __attribute__((ext_vector_type(2)));
 
 // the four fp16 pairs of eight codes, in units of 2^-18
@@ -49,28 +48,6 @@ __device__ __forceinline__ int row_exp(float amax) {
                                                         : -118 - __builtin_clz(__float_as_uint(amax))))
                                          : 0;
 }
-
-// 8 consecutive values of X
-template <typename TX> struct X8;
-template <> struct X8<float> {
-    f32x4 v[2];
-    // zeros where k is past the row's K (a multiple of 8)
-    __device__ __forceinline__ void load(const float* row, int k, int K) {
-        const f32x4* p = (const f32x4*)(row + min(k, K - 8));
-        const f32x4 a = p[0], b = p[1];
-        v[0] = k < K ? a : f32x4{0, 0, 0, 0};
-        v[1] = k < K ? b : f32x4{0, 0, 0, 0};
-    }
-    __device__ __forceinline__ float get(int i) const { return v[i / 4][i % 4]; }
-};
-template <> struct X8<uint16_t> {
-    u4v v;
-    __device__ __forceinline__ void load(const uint16_t* row, int k, int K) {
-        const u4v a = *(const u4v*)(row + min(k, K - 8));
-        v = k < K ? a : u4v{0, 0, 0, 0};
-    }
-    __device__ __forceinline__ float get(int i) const { return i % 2 ? bf_hi(v[i / 2]) : bf_lo(v[i / 2]); }
-};
 
 // 8 scaled values as fp16; `lo` gets the remainders
 template <typename TX>
