@@ -46,14 +46,15 @@ __host__ __device__ inline Q4Ptr q4_ptr(const void* w, const Q4Dims& d) {
 
 typedef uint32_t u4v __attribute__((ext_vector_type(4)));
 
-// 8 consecutive values of a row (k a multiple of 8; rows 16-byte aligned)
+// 8 consecutive values of a row (k a multiple of 8; rows 16-byte aligned). ONCE: read past the caches
 template <typename T> struct X8;
 template <> struct X8<float> {
     f32x4 v[2];
     // zeros where k is past the row's K (a multiple of 8)
+    template <bool ONCE = false>
     __device__ __forceinline__ void load(const float* row, int k, int K) {
         const f32x4* p = (const f32x4*)(row + min(k, K - 8));
-        const f32x4 a = p[0], b = p[1];
+        const f32x4 a = ONCE ? __builtin_nontemporal_load(p) : p[0], b = ONCE ? __builtin_nontemporal_load(p + 1) : p[1];
         v[0] = k < K ? a : f32x4{0, 0, 0, 0};
         v[1] = k < K ? b : f32x4{0, 0, 0, 0};
     }
@@ -61,8 +62,10 @@ template <> struct X8<float> {
 };
 template <> struct X8<uint16_t> {
     u4v v;
+    template <bool ONCE = false>
     __device__ __forceinline__ void load(const uint16_t* row, int k, int K) {
-        const u4v a = *(const u4v*)(row + min(k, K - 8));
+        const u4v* p = (const u4v*)(row + min(k, K - 8));
+        const u4v a = ONCE ? __builtin_nontemporal_load(p) : *p;
         v = k < K ? a : u4v{0, 0, 0, 0};
     }
     __device__ __forceinline__ float get(int i) const { return i % 2 ? bf_hi(v[i / 2]) : bf_lo(v[i / 2]); }

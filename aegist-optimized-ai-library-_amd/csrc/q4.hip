@@ -12,6 +12,14 @@ __device__ __forceinline__ size_t q4_group(const Q4Dims& d, int n, int g) {
     return ((size_t)(n / 16) * d.blocks8() + g / 8) * 128 + (n % 16) * 8 + g % 8;
 }
 
+// largest of the lanes l, l ^ 16, l ^ 32 and l ^ 48
+__device__ __forceinline__ float quad_max(float x) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
 // (w - mn) / sc rounded to the nearest, ties to even, in 0..15, as doubles decide it. In fp32 the quotient is off by at
 // most 15.5 * 3 * 2^-24 < 2^-18, so only within 2^-16 of a half can doubles say otherwise: 1 value in 30000, and the
 // division in doubles is left to those (8 M values: 28 us with it for all, bf16, 9 so).
@@ -34,50 +42,39 @@ __global__ void __launch_bounds__(256) q4_quantize_kernel(const TW* __restrict__
     const bool row = n < d.N;
     X8<TW> w[4];
 #pragma unroll
-    for (int j = 0; j < 4; j++) w[j].load(W + (size_t)min(n, d.N - 1) * ldw, c * 128 + 32 * j + 8 * q, d.K);
-    float lo[4], hi[4];
-    bool bad[4];
+    for (int j = 0; j < 4; j++) w[j].template load<true>(W + (size_t)min(n, d.N - 1) * ldw, c * 128 + 32 * j + 8 * q, d.K);
+    float lo[4], hi[4];  // (hi is infinite where a value has no place in the format)
 #pragma unroll
     for (int j = 0; j < 4; j++) {
         lo[j] = hi[j] = w[j].get(0);
-        bad[j] = false;
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            lo[j] = fminf(lo[j], w[j].get(e));
-            hi[j] = fmaxf(hi[j], w[j].get(e));
-            bad[j] |= !(fabsf(w[j].get(e)) <= 65504.f);
+            const float f = w[j].get(e);
+            lo[j] = fminf(lo[j], f);
+            hi[j] = fmaxf(hi[j], fabsf(f) <= 65504.f ? f : INFINITY);
         }
+        lo[j] = -quad_max(-lo[j]);
+        hi[j] = quad_max(hi[j]);
     }
     const int span = d.G / 32;  // runs of 32 k per group
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-#pragma unroll
-        for (int o = 16; o < 64; o *= 2) {
-            lo[j] = fminf(lo[j], __shfl_xor(lo[j], o, WAVE));
-            hi[j] = fmaxf(hi[j], __shfl_xor(hi[j], o, WAVE));
-            bad[j] |= __shfl_xor((int)bad[j], o, WAVE) != 0;
-        }
-    }
 #pragma unroll
     for (int s = 1; s < 4; s *= 2)
         if (s < span) {
             float l2[4], h2[4];
-            bool b2[4];
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 l2[j] = fminf(lo[j], lo[j ^ s]);
                 h2[j] = fmaxf(hi[j], hi[j ^ s]);
-                b2[j] = bad[j] | bad[j ^ s];
             }
 #pragma unroll
-            for (int j = 0; j < 4; j++) lo[j] = l2[j], hi[j] = h2[j], bad[j] = b2[j];
+            for (int j = 0; j < 4; j++) lo[j] = l2[j], hi[j] = h2[j];
         }
     u4v codes;
     _Float16* scale = (_Float16*)(out + d.code_bytes());
     _Float16* mins = (_Float16*)(out + d.code_bytes() + d.scale_bytes());
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-        const _Float16 mn = bad[j] ? (_Float16)__builtin_nanf("") : (_Float16)lo[j];
+        const _Float16 mn = hi[j] == INFINITY ? (_Float16)__builtin_nanf("") : (_Float16)lo[j];
         const double range = ((double)hi[j] - (double)mn) / 15.0;
         const _Float16 sc = range > 0.0 ? (_Float16)range : (_Float16)0.f;
         const int k = c * 128 + 32 * j;
