@@ -391,21 +391,27 @@ __global__ void __launch_bounds__(MW * WAVE) q4_stream_kernel(const Q4Args a) {
 }
 
 // Tiles that each workgroup takes, one after the other, where a CU holds `per` workgroups and gy of them share a tile: as
-// many as fill the chip, every one as many tiles as the others.
-int stream_rounds(int tiles, int gy, int per) {
-    const int most = std::max(1, 256 * per / gy);
-    return (tiles + most - 1) / most;
+// many as fill the chip, every one as many tiles as the others. Workgroups go round the 8 XCDs, so with a multiple of 8
+// of them side by side those that share a tile share it in one L2 (160 rows of 8192 x 2048: 26.4 us without).
+int stream_rounds(int tiles, int gy, int per, int* gx = nullptr) {
+    int most = std::max(1, 256 * per / gy);
+    const bool whole = gy > 1 && most >= 8;
+    if (whole) most = most / 8 * 8;
+    const int rounds = (tiles + most - 1) / most, x = (tiles + rounds - 1) / rounds;
+    if (gx) *gx = whole ? (x + 7) / 8 * 8 : x;
+    return rounds;
 }
 
 template <typename TX, int SPG, int CPS, int MW, bool FEW>
 int launch_stream(const Q4Args& a, hipStream_t st) {
     const int ks = std::min(MW, (a.d.chunks() - a.c0 + CPS - 1) / CPS), tiles = a.d.tiles(), gy = (a.M + 15) / 16;
-    const int rounds = stream_rounds(tiles, gy, MW / ks);
+    int gx;
+    stream_rounds(tiles, gy, MW / ks, &gx);
     const int lds = 4 * ks * 1024 + (FEW ? ks * staged_bytes(a.M, std::is_same<TX, float>::value ? 2 : 1) : 0);
     if (lds > 65536)
         AEG_HIP(hipFuncSetAttribute((const void*)q4_stream_kernel<TX, SPG, CPS, MW, FEW>,
                                     hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-    q4_stream_kernel<TX, SPG, CPS, MW, FEW><<<dim3((tiles + rounds - 1) / rounds, gy), ks * WAVE, lds, st>>>(a);
+    q4_stream_kernel<TX, SPG, CPS, MW, FEW><<<dim3(gx, gy), ks * WAVE, lds, st>>>(a);
     return after_launch("linear_q4");
 }
 
@@ -430,23 +436,24 @@ int run_stream(const Q4Args& a, int x_dtype, hipStream_t st) {
 }
 
 // ---------------------------------------------------------------------------------------------
-// Many rows: tiles of 128 rows of X x 256 of W, 8 waves of 128 x 32 (so that no two unpack the same codes). X's operands go from the workspace straight into
+// Many rows: tiles of 32, 64 or 128 rows of X x 256 of W, 8 waves of 32 columns (so that no two unpack the same codes). X's operands go from the workspace straight into
 // LDS (1 KB pieces as they lie there: no bank conflicts, no swizzle), 128 k to a stage; codes go from global memory to
 // registers and are unpacked in the wave that uses them. Both are requested two stages ahead (fp32 X: one, of
 // twice the products: LDS). The sums of a group join
 // the tile's in fp32 (one FMA per 32 products and lane).
-constexpr int GM = 128, GN = 256, GR = 8, GC = 2;  // tile; a wave's 16 x 16 tiles
+constexpr int GN = 256, GC = 2;  // columns of a tile; a wave's 16-column tiles of them
 
 // 16 bytes per lane straight from global memory into LDS at lds + 16 lane (lds uniform)
 __device__ __forceinline__ void q4_g2lds(const void* src, void* lds) {
     __builtin_amdgcn_global_load_lds(src, (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
 }
 
-template <int P, int SPG>
+// GR: 16-row tiles, of the workgroup and of each wave.
+template <int P, int SPG, int GR>
 __global__ void __launch_bounds__(512) q4_gemm_kernel(const Q4Args a, int tiles_m, int tiles_n, int ntiles, int per_xcd) {
-    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];  // [NB][8 tiles][P][4 steps][1 KB]
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];  // [NB][GR][P][4 steps][1 KB]
     constexpr int NB = 2;  // stages in LDS and registers
-    constexpr int BUF = GM / 16 * P * 4 * 1024, GP = 4 / SPG;
+    constexpr int GM = 16 * GR, BUF = GR * P * 4 * 1024, GP = 4 / SPG;
     // steps whose products are summed before they are scaled: two of one group, where X's operands leave the registers
     constexpr int U = P == 2 || SPG == 1 ? 1 : 2;
     // consecutive tiles on one XCD: 8 of M beside each other, then along N, so that its workgroups share both in L2
@@ -461,14 +468,17 @@ __global__ void __launch_bounds__(512) q4_gemm_kernel(const Q4Args a, int tiles_
     const int r = lane % 16, q = lane / 16;
     const int KC = d.chunks(), B8 = d.blocks8(), tiles = d.tiles(), xt = (int)o.tiles;
 
-    // this wave's pieces of X per stage: one tile of 16 rows, all its parts and steps
-    const unsigned char* xsrc = (const unsigned char*)a.X + ((size_t)min(bm * 8 + wave, xt - 1) * P * o.steps) * 1024 + lane * 16;
+    // this wave's pieces of X per stage
+    constexpr int XP = GR * P * 4 / 8;
+    const unsigned char* xsrc[XP];
+#pragma unroll
+    for (int i = 0; i < XP; i++) {
+        const int j = wave * XP + i;  // (tile, part, step)
+        xsrc[i] = (const unsigned char*)a.X + (((size_t)min(bm * GR + j / (4 * P), xt - 1) * P + j / 4 % P) * o.steps + j % 4) * 1024 + lane * 16;
+    }
     auto stage = [&](int buf, int c) {
 #pragma unroll
-        for (int p = 0; p < P; p++)
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-                q4_g2lds(xsrc + ((size_t)p * o.steps + c * 4 + j) * 1024, lds + buf * BUF + ((wave * P + p) * 4 + j) * 1024);
+        for (int i = 0; i < XP; i++) q4_g2lds(xsrc[i] + (size_t)c * 4096, lds + buf * BUF + (wave * XP + i) * 1024);
     };
     int nt[GC];
 #pragma unroll
@@ -507,7 +517,7 @@ __global__ void __launch_bounds__(512) q4_gemm_kernel(const Q4Args a, int tiles_
         for (int m = 0; m < GR; m++)
 #pragma unroll
             for (int p = 0; p < 2; p++) {
-                const half8 x = sums[(((size_t)min(bm * 8 + m, xt - 1) * 2 + p) * o.blocks + b) * 64 + lane];
+                const half8 x = sums[(((size_t)min(bm * GR + m, xt - 1) * 2 + p) * o.blocks + b) * 64 + lane];
 #pragma unroll
                 for (int n = 0; n < GC; n++) acc[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, mn[n], acc[m][n], 0, 0, 0);
             }
@@ -611,51 +621,66 @@ __global__ void __launch_bounds__(512) q4_gemm_kernel(const Q4Args a, int tiles_
     }
 }
 
-template <int P, int SPG>
+template <int P, int SPG, int GR>
 int launch_gemm(const Q4Args& a, hipStream_t st) {
-    const int tm = (a.M + GM - 1) / GM, tn = (a.d.N + GN - 1) / GN, n = tm * tn, per = (n + 7) / 8;
-    constexpr int lds = 2 * (GM / 16 * P * 4 * 1024);
+    const int tm = (a.M + 16 * GR - 1) / (16 * GR), tn = (a.d.N + GN - 1) / GN, n = tm * tn, per = (n + 7) / 8;
+    constexpr int lds = 2 * (GR * P * 4 * 1024);
     if (lds > 65536)
-        AEG_HIP(hipFuncSetAttribute((const void*)q4_gemm_kernel<P, SPG>, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-    q4_gemm_kernel<P, SPG><<<8 * per, 512, lds, st>>>(a, tm, tn, n, per);
+        AEG_HIP(hipFuncSetAttribute((const void*)q4_gemm_kernel<P, SPG, GR>, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+    q4_gemm_kernel<P, SPG, GR><<<8 * per, 512, lds, st>>>(a, tm, tn, n, per);
     return after_launch("linear_q4");
 }
-template <int P>
+template <int P, int GR>
 int gemm_spg(const Q4Args& a, hipStream_t st) {
     switch (a.d.G) {
-        case 32: return launch_gemm<P, 1>(a, st);
-        case 64: return launch_gemm<P, 2>(a, st);
-        default: return launch_gemm<P, 4>(a, st);
+        case 32: return launch_gemm<P, 1, GR>(a, st);
+        case 64: return launch_gemm<P, 2, GR>(a, st);
+        default: return launch_gemm<P, 4, GR>(a, st);
     }
 }
 
-// Whether the stream takes M rows, or the 128 x 256 tiles: the shorter by these estimates (us, fitted to M 200 to 2000,
-// N 512 to 32768, K 512 to 4096, where the choice is at most 8% above the faster). The stream: 1.2 per round of tiles
-// (fp32 X 0.95, 1.4 in slices of 512), all rows of X at once; 1000 rows of 8192 x 2048, bf16: 81, tiles 54; of 512 x
-// 2048: 13, tiles 43. The tiles: rounds of 256 workgroups, each a walk along K.
-bool use_stream(int x_dtype, int M, const Q4Dims& d) {
-    if (M <= 16) return true;
+// The kernel of M rows: 0 for the stream, else the GR of the tiles (32, 64 or 128 rows of X x 256 of W), whichever the
+// estimate is shortest for (us; fitted to M 64 to 4000, N 512 to 32768, K 512 to 4096; over 176 other sizes of these
+// ranges the choice is at most 9% above the fastest). The stream: 1.2 per round of tiles (fp32 X 0.95, 1.4 in slices of 512), all rows of X at once. The
+// tiles: rounds of 256 workgroups, each a walk along K; of the small ones, two of a CU overlap. Measured (bf16, K =
+// 2048; stream, 32, 64, 128 rows): 1000 rows x 512 12.9, 22.6, 28.8, 43.6; 1000 x 4096 46.9, 33.9, 32.9, 45.3; 200 x
+// 8192 31.6, 24.2, 28.6, 41.2; 4000 x 8192 300, 195, 188, 172.
+int q4_form(int x_dtype, int M, const Q4Dims& d) {
+    if (M <= 16) return 0;
     const bool f32 = x_dtype == AEGIST_F32;
     const int gy = (M + 15) / 16, KC = d.chunks(), cps = f32 && d.K > 2048 ? 4 : 2, mw = f32 ? 8 : 16;
-    if (gy > 65535) return false;
-    double stream = 7, gemm = 4;
+    double best = 7;
     for (int c = 0; c < KC; c += cps * mw) {
         const int per = mw / std::min(mw, (KC - c + cps - 1) / cps), slots = 256 * per;
-        stream += (double)stream_rounds(d.tiles(), gy, per) * ((gy + slots - 1) / slots) * (f32 ? cps == 4 ? 1.4 : 0.95 : 1.2);
+        best += (double)stream_rounds(d.tiles(), gy, per) * ((gy + slots - 1) / slots) * (f32 ? cps == 4 ? 1.4 : 0.95 : 1.2);
     }
-    const double groups = (double)((M + GM - 1) / GM) * ((d.N + GN - 1) / GN);
-    gemm += std::ceil(groups / 256) * (f32 ? 13 + 28.0 / 8 * KC : 8 + 17.5 / 8 * KC);
-    return stream <= gemm;
+    int form = 0;
+    if (gy > 65535) best = 1e30;  // (rows of the stream's grid)
+    // {before the rounds, per round, per round and 128 k, a further round's share of the first}
+    struct Cost { int gr; double base, round, k, more; };
+    static constexpr Cost kBf16[3] = {{2, 8, 0.8, 6.9 / 8, 0.8}, {4, 8.5, 2, 10.3 / 8, 1}, {8, 4, 8, 17.5 / 8, 1}};
+    static constexpr Cost kF32[3] = {{2, 10, 2, 9.8 / 8, 0.85}, {4, 10, 1, 17.3 / 8, 1}, {8, 4, 13, 28.0 / 8, 1}};
+    for (const Cost& c : f32 ? kF32 : kBf16) {
+        const double groups = std::ceil(M / (16.0 * c.gr)) * ((d.N + GN - 1) / GN), rounds = std::ceil(groups / 256);
+        const double us = c.base + (c.round + c.k * KC) * (1 + c.more * (rounds - 1));
+        if (us < best) best = us, form = c.gr;
+    }
+    return form;
 }
 
-int run_gemm(Q4Args a, int x_dtype, void* ws, hipStream_t st) {
+int run_gemm(int form, Q4Args a, int x_dtype, void* ws, hipStream_t st) {
     const int tiles = (a.M + 15) / 16;
     if (x_dtype == AEGIST_F32) q4_rows_kernel<float><<<tiles, XW * WAVE, 0, st>>>(a, (unsigned char*)ws);
     else q4_rows_kernel<uint16_t><<<tiles, XW * WAVE, 0, st>>>(a, (unsigned char*)ws);
     int rc = after_launch("linear_q4");
     if (rc) return rc;
     a.X = ws;
-    return x_dtype == AEGIST_F32 ? gemm_spg<2>(a, st) : gemm_spg<1>(a, st);
+    const bool f32 = x_dtype == AEGIST_F32;
+    switch (form) {
+        case 2: return f32 ? gemm_spg<2, 2>(a, st) : gemm_spg<1, 2>(a, st);
+        case 4: return f32 ? gemm_spg<2, 4>(a, st) : gemm_spg<1, 4>(a, st);
+        default: return f32 ? gemm_spg<2, 8>(a, st) : gemm_spg<1, 8>(a, st);
+    }
 }
 
 }  // namespace
@@ -667,7 +692,7 @@ size_t linear_q4_workspace(int x_dtype, int M, int N, int K, int G) {
     if (N == 0) return 0;
     // (what the choice of any smaller M needs is enough for it)
     for (long long m = 32; m < M + 16; m += 16)
-        if (!use_stream(x_dtype, (int)std::min<long long>(m, M), d)) return XOps(M, x_dtype == AEGIST_F32 ? 2 : 1, d).bytes();
+        if (q4_form(x_dtype, (int)std::min<long long>(m, M), d)) return XOps(M, x_dtype == AEGIST_F32 ? 2 : 1, d).bytes();
     return 0;
 }
 
@@ -687,10 +712,11 @@ int launch_linear_q4(const void* X, int x_dtype, long long ldx, const void* W, f
     if ((uintptr_t)W % 16) return fail(AEGIST_ERR_SHAPE, "linear_q4: W must be 16-byte aligned");
     const Q4Dims d{N, K, G};
     const Q4Args a{X, ldx, (const unsigned char*)W, Y, ldy, M, accumulate, d, 0};
-    if (use_stream(x_dtype, M, d)) return run_stream(a, x_dtype, st);
+    const int form = q4_form(x_dtype, M, d);
+    if (!form) return run_stream(a, x_dtype, st);
     rc = check_workspace(ws, ws_bytes, XOps(M, x_dtype == AEGIST_F32 ? 2 : 1, d).bytes(), "linear_q4");
     if (rc) return rc;
-    return run_gemm(a, x_dtype, ws, st);
+    return run_gemm(form, a, x_dtype, ws, st);
 }
 
 }  // namespace aegist
