@@ -24,6 +24,7 @@ int launch_proj(const void* X, int x_dtype, long long ldx, const void* W, int w_
 namespace {
 
 constexpr int MAX_TOP = 64;
+constexpr int MAX_V = 1 << 30;           // (a logit's index plus a segment stays an int)
 constexpr int NT = 256, NW = NT / WAVE;  // threads, waves
 constexpr int CAP = 512;                 // candidates that are ranked at once
 
@@ -226,21 +227,21 @@ __device__ __forceinline__ int select_keys(Lds& s, int have, int top, Key key) {
     return have;
 }
 
-// A workgroup's items: rows x splits, each `span` logits (the last fewer) in segments of 4 VPT NT. `base` is
-// the first token of these logits, V the whole vocabulary's. With one split the outputs are written here.
+// A workgroup's items: rows x splits, each `span` logits (the last fewer) in segments of 4 VPT NT. With one split the
+// outputs are written here.
 template <typename T, int VPT>
-__global__ void __launch_bounds__(NT) logprobs_kernel(const T* __restrict__ L, long long ld, int rows, int cols, int base,
-                                                      int V, int span, int split0, int splits, int all_splits,
-                                                      Part* __restrict__ parts, u64* __restrict__ tops, const LogprobOut o) {
+__global__ void __launch_bounds__(NT) logprobs_kernel(const T* __restrict__ L, long long ld, int rows, int V, int span,
+                                                      int splits, Part* __restrict__ parts, u64* __restrict__ tops,
+                                                      const LogprobOut o) {
     __shared__ Lds s;
     const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE, top = o.top;
     constexpr int SEG = 4 * VPT * NT;
     constexpr float LOG2E = 1.44269504f, LN2 = 0.693147181f;
     for (long long item = blockIdx.x; item < (long long)rows * splits; item += gridDim.x) {
         const int t = (int)(item / splits), sp = (int)(item % splits);
-        const int c0 = sp * span, c1 = min(cols, c0 + span);
+        const int c0 = sp * span, c1 = min(V, c0 + span);
         const T* x = L + (size_t)t * ld;
-        const int tok = o.tokens[t] - base;
+        const int tok = o.tokens[t];
         Part p{-INFINITY, 0.f, 0.f, -INFINITY, 0, {}};
         int have = 0;  // alternatives so far (the same in all threads)
         for (int b = c0; b < c1; b += SEG) {
@@ -311,7 +312,7 @@ __global__ void __launch_bounds__(NT) logprobs_kernel(const T* __restrict__ L, l
 #pragma unroll
                     for (int e = 0; e < 4; e++)
                         if (4 * (int)threadIdx.x + e < 2 * top && c + e < c1 && v[0].get(e) == -INFINITY)
-                            add_candidate(s, lp_key(-INFINITY, base + c + e));
+                            add_candidate(s, lp_key(-INFINITY, c + e));
                 }
                 if (strict ? mt > thr : mt >= thr) {
 #pragma unroll
@@ -321,7 +322,7 @@ __global__ void __launch_bounds__(NT) logprobs_kernel(const T* __restrict__ L, l
                             const float f = v[i].get(e);
                             if (strict ? f > thr : f >= thr) {
                                 const int ce = c + 4 * NT * i + e;
-                                if (ce < c1) add_candidate(s, lp_key(f, base + ce));
+                                if (ce < c1) add_candidate(s, lp_key(f, ce));
                             }
                         }
                 }
@@ -340,18 +341,18 @@ __global__ void __launch_bounds__(NT) logprobs_kernel(const T* __restrict__ L, l
                     // (read again: keys of a whole segment would take two registers per logit)
                     have = select_keys<4 * VPT, 1>(s, have, top, [&](int i) {
                         const int ce = c + 4 * NT * (i / 4) + i % 4;
-                        return ce < c1 ? lp_key(Act<T>::ld(x, ce), base + ce) : 0;
+                        return ce < c1 ? lp_key(Act<T>::ld(x, ce), ce) : 0;
                     });
                 }
             }
             __syncthreads();
             join(p, q);
         }
-        if (all_splits == 1) {
+        if (splits == 1) {
             if (threadIdx.x == 0) finish(o, t, V, p);
             if ((int)threadIdx.x < top) finish_top(o, t, threadIdx.x, p, s.list[threadIdx.x]);
         } else {
-            const size_t at = (size_t)t * all_splits + split0 + sp;
+            const size_t at = (size_t)item;
             if (threadIdx.x == 0) parts[at] = p;
             if ((int)threadIdx.x < top) tops[at * top + threadIdx.x] = (int)threadIdx.x < have ? s.list[threadIdx.x] : 0;
         }
@@ -404,7 +405,8 @@ __global__ void __launch_bounds__(NT) logprobs_join_kernel(const Part* __restric
 
 int check_out(const char* who, int T, int V, const LogprobOut& o) {
     const std::string w(who);
-    if (T < 0 || V < 1) return fail(AEGIST_ERR_SHAPE, w + ": negative size or empty vocabulary");
+    if (T < 0 || V < 1 || V > MAX_V)
+        return fail(AEGIST_ERR_SHAPE, w + ": negative size, or a vocabulary of none or more than 2^30 tokens");
     if (o.top < 0 || o.top > MAX_TOP || o.top > V)
         return fail(AEGIST_ERR_SHAPE, w + ": 0 to 64 alternatives, no more than the vocabulary has");
     if (T == 0) return 0;
@@ -420,7 +422,7 @@ int split_span(int T, int cols, int* small) {
     long long span = (cols + want - 1) / want;
     *small = span <= 2 * seg;
     const int unit = *small ? seg : 4 * seg;
-    return (int)std::min<long long>((span + unit - 1) / unit * unit, 1 << 30);
+    return (int)((span + unit - 1) / unit * unit);
 }
 int split_count(int T, int cols) {
     int small;
@@ -428,16 +430,18 @@ int split_count(int T, int cols) {
     return (cols + span - 1) / span;
 }
 
-// logits [T, cols] of the tokens base .. base + cols - 1, as splits split0 .. of all_splits
-int run_splits(const void* L, int dtype, long long ld, int T, int cols, int base, int V, int split0, int all_splits, void* ws,
-               const LogprobOut& o, hipStream_t st) {
+size_t splits_bytes(int T, int V, int top) {
+    const int n = split_count(T, V);
+    return n > 1 ? parts_bytes(T, n, top) : 0;
+}
+
+int run_logprobs(const void* L, int dtype, long long ld, int T, int V, void* ws, const LogprobOut& o, hipStream_t st) {
     int small;
-    const int span = split_span(T, cols, &small), splits = (cols + span - 1) / span;
+    const int span = split_span(T, V, &small), splits = (V + span - 1) / span;
     Part* parts = (Part*)ws;
-    u64* tops = (u64*)(parts + (size_t)T * all_splits);
+    u64* tops = (u64*)(parts + (size_t)T * splits);
     const int grid = (int)std::min<long long>((long long)T * splits, 1 << 20);
-#define AEG_LP(TY, VPT) \
-    logprobs_kernel<TY, VPT><<<grid, NT, 0, st>>>((const TY*)L, ld, T, cols, base, V, span, split0, splits, all_splits, parts, tops, o)
+#define AEG_LP(TY, VPT) logprobs_kernel<TY, VPT><<<grid, NT, 0, st>>>((const TY*)L, ld, T, V, span, splits, parts, tops, o)
     if (dtype == AEGIST_F32) {
         if (small) AEG_LP(float, 4);
         else AEG_LP(float, 16);
@@ -446,12 +450,9 @@ int run_splits(const void* L, int dtype, long long ld, int T, int cols, int base
         else AEG_LP(uint16_t, 16);
     }
 #undef AEG_LP
-    return after_launch("token_logprobs");
-}
-
-int run_join(int T, int V, int splits, const void* ws, const LogprobOut& o, hipStream_t st) {
-    const Part* parts = (const Part*)ws;
-    logprobs_join_kernel<<<std::min(T, 1 << 20), NT, 0, st>>>(parts, (const u64*)(parts + (size_t)T * splits), T, V, splits, o);
+    int rc = after_launch("token_logprobs");
+    if (rc || splits == 1) return rc;
+    logprobs_join_kernel<<<std::min(T, 1 << 20), NT, 0, st>>>(parts, tops, T, V, splits, o);
     return after_launch("token_logprobs");
 }
 
@@ -463,9 +464,11 @@ size_t head_logits_bytes(int T, int V) { return ((size_t)head_rows(T, V) * V * 4
 }  // namespace
 
 extern "C" size_t aegist_token_logprobs_workspace_bytes(int T, int V, int top) {
-    if (T < 1 || V < 1 || top < 0 || top > MAX_TOP) return 0;
-    const int n = split_count(T, V);
-    return n > 1 ? parts_bytes(T, n, top) : 0;
+    if (T < 1 || V < 1 || V > MAX_V || top < 0 || top > MAX_TOP) return 0;
+    // what any T up to this needs: few rows are cut into the most splits, more than 768 into none
+    size_t need = 0;
+    for (int t = 1; t <= std::min(T, 768); t++) need = std::max(need, splits_bytes(t, V, top));
+    return need;
 }
 
 extern "C" int aegist_token_logprobs(const void* logits, int dtype, long long ld, const int* tokens, float* logprob,
@@ -478,16 +481,12 @@ extern "C" int aegist_token_logprobs(const void* logits, int dtype, long long ld
         return fail(AEGIST_ERR_DTYPE, "token_logprobs: logits must be AEGIST_F32 or AEGIST_BF16");
     if (T == 0) return 0;
     if (!logits || ld < V) return fail(AEGIST_ERR_SHAPE, "token_logprobs: null logits, or ld < V");
-    rc = check_workspace(ws, ws_bytes, aegist_token_logprobs_workspace_bytes(T, V, top), "token_logprobs");
-    if (rc) return rc;
-    const hipStream_t st = AEG_STREAM(stream);
-    const int n = split_count(T, V);
-    rc = run_splits(logits, dtype, ld, T, V, 0, V, 0, n, ws, o, st);
-    return rc || n == 1 ? rc : run_join(T, V, n, ws, o, st);
+    rc = check_workspace(ws, ws_bytes, splits_bytes(T, V, top), "token_logprobs");
+    return rc ? rc : run_logprobs(logits, dtype, ld, T, V, ws, o, AEG_STREAM(stream));
 }
 
 extern "C" size_t aegist_head_logprobs_workspace_bytes(int x_dtype, int w_dtype, int T, int V, int K, int group, int top) {
-    if (T < 1 || V < 1 || K < 1) return 0;
+    if (T < 1 || V < 1 || V > MAX_V || K < 1) return 0;
     const int rows = head_rows(T, V);
     return head_logits_bytes(T, V) + aegist_token_logprobs_workspace_bytes(rows, V, top) +
            (w_dtype == AEGIST_Q4 ? aegist_linear_q4_workspace_bytes(x_dtype, rows, V, K, group) : 0);
@@ -523,9 +522,7 @@ extern "C" int aegist_head_logprobs(const void* X, int x_dtype, long long ldx, c
         if (rc) return rc;
         const LogprobOut part{tokens + t, logprob + t, entropy + t, top_ids ? top_ids + (size_t)t * top : nullptr,
                               top_logprobs ? top_logprobs + (size_t)t * top : nullptr, top};
-        const int n = split_count(m, V);
-        if ((rc = run_splits(logits, AEGIST_F32, V, m, V, 0, V, 0, n, pws, part, st))) return rc;
-        if (n > 1 && (rc = run_join(m, V, n, pws, part, st))) return rc;
+        if ((rc = run_logprobs(logits, AEGIST_F32, V, m, V, pws, part, st))) return rc;
     }
     return 0;
 }

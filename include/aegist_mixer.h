@@ -439,7 +439,7 @@ int aegist_linear_q4(const void* X, int x_dtype, long long ldx, const void* q4, 
                      int K, int group, int accumulate, void* ws, size_t ws_bytes, void* stream);
 
 /* -------------------------------------------------------------------------------------
- * Log probabilities of given tokens under logits [T, V], with the entropy of each row and its
+ * Log probabilities of given tokens under logits [T, V] (V at most 2^30), with the entropy of each row and its
  * `top` (0 to 64, at most V) most probable tokens. No counterpart in the reference, whose engine
  * copies the logits to the host.
  *   tokens       [T] int32. A negative one has logprob 0 (no token there), one past the vocabulary NaN
@@ -450,7 +450,8 @@ int aegist_linear_q4(const void* X, int x_dtype, long long ldx, const void* q4, 
  * Logits of -inf have no probability. A row of nothing else has logprob -inf for every token and
  * entropy 0. A row with a NaN or +inf has NaN for all of them (top_ids: NaN first). Deterministic.
  * ------------------------------------------------------------------------------------- */
-/* logits AEGIST_F32 | AEGIST_BF16, row stride ld elements, aligned to the element. */
+/* logits AEGIST_F32 | AEGIST_BF16, row stride ld elements, aligned to the element. A workspace for T rows
+ * serves every smaller batch. */
 size_t aegist_token_logprobs_workspace_bytes(int T, int V, int top);
 int aegist_token_logprobs(const void* logits, int dtype, long long ld, const int* tokens, float* logprob,
                           float* entropy, int* top_ids, float* top_logprobs, int T, int V, int top, void* ws,

@@ -179,6 +179,30 @@ def test_head_logprobs(dev, kind, T, V, K, top, dtype):
     assert ((r.top_logprobs.cpu().double() - lps[:, :top]).abs() <= 2 * off.unsqueeze(1) + 2.0 ** -15).all()
 
 
+@pytest.mark.parametrize("V,T", [(65537, 1024), (131073, 513), (131073, 1535)])
+@pytest.mark.parametrize("top", [0, 3])
+def test_head_logprobs_in_blocks(dev, V, T, top):
+    """More rows than 256 MiB of logits have: the last block, of one row, two or three, is cut into other splits than the
+    blocks before it. Against the logits of bf16 products, exact in fp32 but for the order of 64 sums (the bounds
+    of the test above, rows of bf16 values)."""
+    K = 64
+    w, _, wd = _head("bf16", V, K, 1, dev)
+    g = torch.Generator().manual_seed(T)
+    x = torch.randn(T, K, generator=g).bfloat16()
+    tok = torch.randint(0, V, (T,), generator=g, dtype=torch.int32)
+    r = ops.head_logprobs(x.to(dev), w, tok.to(dev), top)
+    for t in (slice(0, 3), slice(T // 2, T // 2 + 2), slice(T - 4, T)):  # (rows of every block)
+        xs = x[t].double()
+        off = (K * 2.0 ** -23 * (xs.abs() @ wd.abs().t())).amax(1)
+        lp, ent, _, lps, _ = _ref(xs @ wd.t(), tok[t], top)
+        assert ((r.logprob[t].cpu().double() - lp).abs() <= 2 * off + 2.0 ** -15).all()
+        assert ((r.entropy[t].cpu().double() - ent).abs() <= 40 * off + 30 * 2.0 ** -16).all()
+        if top:
+            assert ((r.top_logprobs[t].cpu().double() - lps).abs() <= 2 * off.unsqueeze(1) + 2.0 ** -15).all()
+    one = ops.head_logprobs(x[T // 3:T // 3 + 1].to(dev), w, tok[T // 3:T // 3 + 1].to(dev), top)
+    assert (one.logprob - r.logprob[T // 3:T // 3 + 1]).abs().max() < 1e-3
+
+
 @pytest.mark.parametrize("T", [1, 20, 300])
 def test_quantize_project_score_together(dev, T):
     """A head quantised, multiplied and scored: the head's answers are those of the logits that linear_q4 makes of

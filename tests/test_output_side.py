@@ -187,3 +187,28 @@ def test_call_is_made_on_the_tensors_device(monkeypatch, launches):
 def test_tensors_of_two_devices_are_refused():
     with pytest.raises(ops.AegistError, match="one device"):
         ops._one_device(torch.empty(1), None, torch.empty(1, device="meta"))
+
+
+@pytest.mark.parametrize("V", [1, 1000, 4097, 50257, 131072, 2 ** 20 + 1, 2 ** 27, 2 ** 30])
+def test_logprob_workspace_serves_every_smaller_batch(V):
+    """Few rows are cut into more splits than many, which need no workspace at all: what is asked for T rows covers
+    every smaller batch, so also the last block of a head's rows."""
+    L = _lib.lib()
+    for top in (0, 1, min(V, 64)):
+        sizes = [L.aegist_token_logprobs_workspace_bytes(T, V, top) for T in list(range(1, 800, 7)) + [1536, 1537, 2 ** 20]]
+        assert sizes == sorted(sizes)
+        if V >= 50257:
+            assert sizes[0] > 0
+        # the logits of a block of 256 MiB (at least one row) and behind them what any number of its rows needs
+        rows = max(1, 2 ** 28 // (4 * V))
+        logits = -(-rows * V * 4 // 256) * 256
+        blocks = L.aegist_head_logprobs_workspace_bytes(1, 1, 3 * rows + 1, V, 64, 0, top) - logits
+        assert blocks >= max(L.aegist_token_logprobs_workspace_bytes(m, V, top) for m in (1, (rows + 1) // 2, rows))
+
+
+def test_logprobs_refuse_a_vocabulary_past_the_index(launches):
+    L = _lib.lib()
+    V = 2 ** 30 + 1
+    assert L.aegist_token_logprobs(64, 0, V, 64, 64, 64, 64, 64, 1, V, 1, None, 0, None) == -1 and "2^30" in _lib.last_error()
+    assert L.aegist_head_logprobs(64, 0, 64, 64, 1, None, 64, 64, 64, 64, 64, 1, V, 64, 0, 1, None, 0, None) == -1
+    assert L.aegist_token_logprobs_workspace_bytes(1, V, 1) == 0
