@@ -38,8 +38,9 @@ __device__ __forceinline__ float q4_scale(uint32_t w) {
     asm("" : "+v"(f));
     return f;
 }
-// what undoes the units of the code products (2^-18) beside those of the minima (X's sums in units of 2^7)
-constexpr float kCodeUnit = 0x1p11f;
+// what undoes the units of the code products (2^-18) beside those of the minima (X's sums in units of 2^7, in which the
+// 128 values of a group stay within fp16)
+constexpr float kCodeUnit = 0x1p11f, kSumUnit = 0x1p-7f;
 
 // power of two by which a row of X is scaled; 0 for rows without a finite largest value (their outputs are not)
 __device__ __forceinline__ int row_exp(float amax) {
@@ -144,13 +145,14 @@ __global__ void __launch_bounds__(XW * WAVE) q4_rows_kernel(const Q4Args a, unsi
         for (int j = 0; j < XJ; j++) {
             half8 lo;
             const half8 hi = x_parts(f[j], e, F32 ? &lo : nullptr);
+#pragma unroll
+            for (int i = 0; i < 8; i++) s += __builtin_ldexpf(f[j].get(i), e);  // (scaled: it cannot overflow)
             parts[(mt * o.parts * o.steps + j0 + j) * 64 + lane] = hi;
             if (F32) parts[((mt * o.parts + 1) * o.steps + j0 + j) * 64 + lane] = lo;
-            s += ((f[j].get(0) + f[j].get(1)) + (f[j].get(2) + f[j].get(3))) + ((f[j].get(4) + f[j].get(5)) + (f[j].get(6) + f[j].get(7)));
             if ((j + 1) % spg) continue;
             s += __shfl_xor(s, 16, WAVE);
             s += __shfl_xor(s, 32, WAVE);
-            s = __builtin_ldexpf(s, e - 7);
+            s *= kSumUnit;
             const int g = (j0 + j) / spg;
             const _Float16 hs = (_Float16)s;
             if (q < 2 && g < NG)  // lane 16 q + r writes part q
@@ -254,9 +256,9 @@ __global__ void __launch_bounds__(MW * WAVE) q4_stream_kernel(const Q4Args a) {
             half4 hi, lo;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const float v = __builtin_ldexpf(f[m][i], e);
-                hi[i] = (_Float16)v;
-                lo[i] = (_Float16)(v - (float)hi[i]);
+                f[m][i] = __builtin_ldexpf(f[m][i], e);
+                hi[i] = (_Float16)f[m][i];
+                lo[i] = (_Float16)(f[m][i] - (float)hi[i]);
             }
             *(half4*)(own + m * PARTS * 512 + lane * 8) = hi;
             if (F32) *(half4*)(own + (m * PARTS + 1) * 512 + lane * 8) = lo;
@@ -264,7 +266,7 @@ __global__ void __launch_bounds__(MW * WAVE) q4_stream_kernel(const Q4Args a) {
             float s = (f[m][0] + f[m][1]) + (f[m][2] + f[m][3]);
 #pragma unroll
             for (int o = 1; o < 8 * SPG; o *= 2) s += __shfl_xor(s, o, WAVE);
-            s = __builtin_ldexpf(s, e - 7);
+            s *= kSumUnit;
             const _Float16 sh = (_Float16)s;
             if (lane % (8 * SPG) == 0) {
                 const int g = (g0 + lane / (8 * SPG)) % 8;
@@ -306,31 +308,29 @@ __global__ void __launch_bounds__(MW * WAVE) q4_stream_kernel(const Q4Args a) {
         const int e = row_exp(amax);
 #pragma unroll
         for (int i = 0; i < 4; i++) e4[i] = 7 - __shfl(e, 4 * q + i, WAVE);
-        float s = 0.f;
-        half8 hi{}, lo{};
+        // the groups' sums as products with rows of ones: group g of row r in lane (r, g / 8), the value g % 4 of
+        // sums[g % 8 / 4], which is the place that the product with the minima reads it from (a slice of 2 or 4 groups
+        // begins within its block of 8)
+        constexpr bool WHOLE = Slice::GROUPS >= 8;
+        f32x4 sums[2]{};
 #pragma unroll
         for (int j = 0; j < ST; j++) {
-            half8 l;
-            const half8 h = x_parts(f[j], e, F32 ? &l : nullptr);
-            xa[0][j] = h;
-            if (F32) xa[NA - 1][j] = l;
-            s += ((f[j].get(0) + f[j].get(1)) + (f[j].get(2) + f[j].get(3))) + ((f[j].get(4) + f[j].get(5)) + (f[j].get(6) + f[j].get(7)));
-            if (j % SPG < SPG - 1) continue;
-            // the group's sum, and its place among the 8 of the block that lanes q read the minima of
-            s += __shfl_xor(s, 16, WAVE);
-            s += __shfl_xor(s, 32, WAVE);
-            s = __builtin_ldexpf(s, e - 7);
-            const _Float16 sh = (_Float16)s, slo = (_Float16)(s - (float)sh);
+            half8 lo;
+            xa[0][j] = x_parts(f[j], e, F32 ? &lo : nullptr);
+            if (F32) xa[NA - 1][j] = lo;
             const int g = j / SPG;
+            const uint32_t one = r == (WHOLE ? 4 * (g / 8) + g % 4 : (g0 + g) % 4) ? 0x3c003c00u : 0;
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const bool here = Slice::GROUPS >= 8 ? g % 8 == i && q == g / 8 : q == 0 && (g0 + g) % 8 == i;
-                hi[i] = here ? sh : hi[i];
-                lo[i] = here ? slo : lo[i];
-            }
-            s = 0.f;
+            for (int n = 0; n < NA; n++)
+                sums[WHOLE ? g % 8 / 4 : 0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                    __builtin_bit_cast(half8, u4v{one, one, one, one}), xa[n][j], sums[WHOLE ? g % 8 / 4 : 0], 0, 0, 0);
         }
-        xs[0] = hi, xs[NS - 1] = lo;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float s = kSumUnit * (WHOLE ? sums[i / 4][i % 4] : i / 4 == g0 % 8 / 4 ? sums[0][i % 4] : 0.f);
+            xs[0][i] = (_Float16)s;
+            xs[NS - 1][i] = (_Float16)(s - (float)xs[0][i]);
+        }
     }
 
     // a tile: this wave's share of its sums, in units of Y

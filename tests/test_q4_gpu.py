@@ -108,6 +108,20 @@ def test_linear_q4_rows_of_any_size(dev, M):
     _check(x.bfloat16(), w4, wt, dev)
 
 
+@pytest.mark.parametrize("M", [1, 2, 7, 40, 700])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("G", [32, 64, 128])
+def test_linear_q4_sums_of_large_rows(dev, M, dtype, G):
+    """Rows whose groups sum to more than fp32 holds, although every output is far inside it."""
+    N, K = 40, 256
+    codes, scale, mn, _ = _weight(N, K, G, 16)
+    scale, mn = (scale.float() / 64).half(), (mn.float() / 64).half()
+    wt = (codes, scale, mn, R.q4_dequantize(codes, scale, mn, G))
+    x = 1e38 * (1 + torch.rand(M, K, generator=torch.Generator().manual_seed(5))).to(dtype)
+    assert torch.isinf(x.float()[:, :G].sum(1)).all() and (x.double() @ wt[3].t()).abs().max() < 1e38
+    _check(x.to(dtype), _pack(*wt[:3], dev), wt, dev)
+
+
 @pytest.mark.parametrize("M", [2, 9, 33, 140])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_linear_q4_keeps_bad_rows_apart(dev, M, dtype):
