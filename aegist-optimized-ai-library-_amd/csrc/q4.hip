@@ -122,16 +122,17 @@ __global__ void __launch_bounds__(256) q4_pack_kernel(const unsigned char* __res
 __global__ void __launch_bounds__(256) q4_pack_groups_kernel(const _Float16* __restrict__ scale,
                                                              const _Float16* __restrict__ mins, unsigned char* out,
                                                              const Q4Dims d) {
-    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x, all = d.scale_bytes() / 2;
-    if (i >= all) return;
-    const int g = (int)(i / 128 % d.blocks8()) * 8 + i % 8, n = (int)(i / 128 / d.blocks8()) * 16 + i / 8 % 16;
-    _Float16 s = 0, m = 0;
-    if (n < d.N && g < d.K / d.G) {
-        s = scale[(size_t)n * (d.K / d.G) + g];
-        m = mins ? mins[(size_t)n * (d.K / d.G) + g] : (_Float16)(-8.f * (float)s);
+    const size_t all = d.scale_bytes() / 2;
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (size_t)gridDim.x * 256) {
+        const int g = (int)(i / 128 % d.blocks8()) * 8 + i % 8, n = (int)(i / 128 / d.blocks8()) * 16 + i / 8 % 16;
+        _Float16 s = 0, m = 0;
+        if (n < d.N && g < d.K / d.G) {
+            s = scale[(size_t)n * (d.K / d.G) + g];
+            m = mins ? mins[(size_t)n * (d.K / d.G) + g] : (_Float16)(-8.f * (float)s);
+        }
+        ((_Float16*)(out + d.code_bytes()))[i] = s;
+        ((_Float16*)(out + d.code_bytes() + d.scale_bytes()))[i] = m;
     }
-    ((_Float16*)(out + d.code_bytes()))[i] = s;
-    ((_Float16*)(out + d.code_bytes() + d.scale_bytes()))[i] = m;
 }
 
 __global__ void __launch_bounds__(256) q4_dequantize_kernel(const unsigned char* __restrict__ W, float* __restrict__ out,
@@ -171,6 +172,7 @@ int check_q4(const char* who, int N, int K, int G) {
     const std::string w(who);
     if (G != 32 && G != 64 && G != 128) return fail(AEGIST_ERR_SHAPE, w + ": groups of 32, 64 or 128 values");
     if (N < 0 || K <= 0 || K % G) return fail(AEGIST_ERR_SHAPE, w + ": K must be a positive multiple of the group");
+    if (N > 1 << 28 || K > 1 << 28) return fail(AEGIST_ERR_SHAPE, w + ": N and K are at most 2^28");
     return 0;
 }
 
@@ -212,7 +214,7 @@ extern "C" int aegist_q4_pack(const void* codes, const uint16_t* scale, const ui
     const hipStream_t st = AEG_STREAM(stream);
     q4_pack_kernel<<<q4_grid(d), 256, 0, st>>>((const unsigned char*)codes, (unsigned char*)q4, d);
     if ((rc = after_launch("q4_pack"))) return rc;
-    q4_pack_groups_kernel<<<(unsigned)((d.scale_bytes() / 2 + 255) / 256), 256, 0, st>>>(
+    q4_pack_groups_kernel<<<(unsigned)std::min<size_t>((d.scale_bytes() / 2 + 255) / 256, 1 << 20), 256, 0, st>>>(
         (const _Float16*)scale, (const _Float16*)mins, (unsigned char*)q4, d);
     return after_launch("q4_pack");
 }

@@ -63,6 +63,10 @@ __device__ __forceinline__ half8 x_parts(const X8<TX>& x, int e, half8* lo) {
     return hi;
 }
 
+// Rows of a launch (of more, blocks of so many): their 16-row tiles fit a grid's second dimension, and their operands'
+// workspace does not grow further.
+constexpr int kMaxRows = 1 << 19;
+
 struct Q4Args {
     const void* X;  // rows, or the operands made of them (XOps)
     long long ldx;
@@ -78,14 +82,14 @@ struct Q4Args {
 // More than a few rows: X is made into matrix operands once, in the workspace, in the order in which waves load
 // them (1 KB for 16 rows x 32 k):
 //   parts [M / 16][parts][K / 32][64 lanes][8 fp16]: lane 16 q + r has k = 32 j + 8 q .. + 7 of row r, with zeros
-//         from K to a multiple of 256
+//         from K to a multiple of 128
 //   sums  [M / 16][2 parts][K / G / 32][64 lanes][8 fp16]: the sums of the groups 32 b + 8 q .. + 7
 //   exps  [M] int: the power of two each row was scaled by
 struct XOps {
     int parts, steps, blocks;  // 32 k each, 32 groups each
     size_t tiles;
     __host__ __device__ XOps(int M, int parts, const Q4Dims& d)
-        : parts(parts), steps((d.K + 255) / 256 * 8), blocks((d.K / d.G + 31) / 32), tiles((M + 15) / 16) {}
+        : parts(parts), steps(d.chunks() * 4), blocks((d.K / d.G + 31) / 32), tiles((M + 15) / 16) {}
     __host__ __device__ size_t sums_at() const { return tiles * parts * steps * 1024; }
     __host__ __device__ size_t exps_at() const { return sums_at() + tiles * 2 * blocks * 1024; }
     __host__ __device__ size_t bytes() const { return exps_at() + (tiles * 64 + 255) / 256 * 256; }
@@ -176,8 +180,8 @@ __global__ void __launch_bounds__(XW * WAVE) q4_rows_kernel(const Q4Args a, unsi
 // mostly the staging (two rows per wave one after the other).
 
 // Up to kStaged rows are scaled one after the other, 4 values of the slice per lane, and pass through the wave's own LDS
-// into the operands: a lane that makes its operands itself makes those of row r % M, the same as the others of that row
-// (8192 x 2048, one row: 9.0 -> 7 us).
+// into the operands: a lane that makes its operands itself makes those of row min(r, M - 1), the same as the others of that
+// row (8192 x 2048, one row: 7.0 us so, 5.7 staged; three rows: no difference).
 constexpr int kStaged = 2;
 // per wave: rows [M][parts][256 fp16], sums [M][2][8 fp16], exponents [4]
 __host__ __device__ constexpr int staged_bytes(int M, int parts) { return M * (parts * 512 + 32) + 16; }
@@ -436,11 +440,10 @@ int run_stream(const Q4Args& a, int x_dtype, hipStream_t st) {
 }
 
 // ---------------------------------------------------------------------------------------------
-// Many rows: tiles of 32, 64 or 128 rows of X x 256 of W, 8 waves of 32 columns (so that no two unpack the same codes). X's operands go from the workspace straight into
-// LDS (1 KB pieces as they lie there: no bank conflicts, no swizzle), 128 k to a stage; codes go from global memory to
-// registers and are unpacked in the wave that uses them. Both are requested two stages ahead (fp32 X: one, of
-// twice the products: LDS). The sums of a group join
-// the tile's in fp32 (one FMA per 32 products and lane).
+// Many rows: tiles of 32, 64 or 128 rows of X x 256 of W, 8 waves of 32 columns (so that no two unpack the same codes).
+// X's operands go from the workspace straight into LDS (1 KB pieces as they lie there: no bank conflicts, no swizzle),
+// 128 k to a stage; codes go from global memory to registers and are unpacked in the wave that uses them. Both are
+// requested a stage ahead. The sums of a group join the tile's in fp32 (one FMA per 32 products and lane).
 constexpr int GN = 256, GC = 2;  // columns of a tile; a wave's 16-column tiles of them
 
 // 16 bytes per lane straight from global memory into LDS at lds + 16 lane (lds uniform)
@@ -451,8 +454,7 @@ __device__ __forceinline__ void q4_g2lds(const void* src, void* lds) {
 // GR: 16-row tiles, of the workgroup and of each wave.
 template <int P, int SPG, int GR>
 __global__ void __launch_bounds__(512) q4_gemm_kernel(const Q4Args a, int tiles_m, int tiles_n, int ntiles, int per_xcd) {
-    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];  // [NB][GR][P][4 steps][1 KB]
-    constexpr int NB = 2;  // stages in LDS and registers
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];  // [2 stages][GR][P][4 steps][1 KB]
     constexpr int GM = 16 * GR, BUF = GR * P * 4 * 1024, GP = 4 / SPG;
     // steps whose products are summed before they are scaled: two of one group, where X's operands leave the registers
     constexpr int U = P == 2 || SPG == 1 ? 1 : 2;
@@ -483,8 +485,8 @@ __global__ void __launch_bounds__(512) q4_gemm_kernel(const Q4Args a, int tiles_
     int nt[GC];
 #pragma unroll
     for (int n = 0; n < GC; n++) nt[n] = min(bn * 16 + wave * GC + n, tiles - 1);
-    u4v code[NB][GC];
-    u2v sc[NB][GC];
+    u4v code[2][GC];
+    u2v sc[2][GC];
     auto load = [&](int buf, int c) {
 #pragma unroll
         for (int n = 0; n < GC; n++) {
@@ -495,12 +497,8 @@ __global__ void __launch_bounds__(512) q4_gemm_kernel(const Q4Args a, int tiles_
             else sc[buf][n][0] = *(const uint16_t*)p;
         }
     };
-#pragma unroll
-    for (int c = 0; c < NB - 1; c++)
-        if (c < KC) {
-            stage(c, c);
-            load(c, c);
-        }
+    stage(0, 0);
+    load(0, 0);
 
     // the minima's term first, in the units of the codes' sums
     f32x4 acc[GR][GC];
@@ -528,13 +526,11 @@ __global__ void __launch_bounds__(512) q4_gemm_kernel(const Q4Args a, int tiles_
         for (int n = 0; n < GC; n++) acc[m][n] *= 1.f / kCodeUnit;
 
     auto step = [&](int buf, int c) {
-        // this wave's pieces of stage c are in LDS once only the later stage's loads are in flight
-        if (NB == 3 && c + 1 < KC) __builtin_amdgcn_s_waitcnt(0x0f70 | (4 * P + 2 * GC));
-        else __builtin_amdgcn_s_waitcnt(0x0f70);
-        lds_barrier();  // all waves' are, and all have read stage c - 1
-        if (c + NB - 1 < KC) {
-            stage((buf + NB - 1) % NB, c + NB - 1);
-            load((buf + NB - 1) % NB, c + NB - 1);
+        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's pieces of stage c are in LDS
+        lds_barrier();                       // all waves' are, and all have read stage c - 1
+        if (c + 1 < KC) {
+            stage(1 - buf, c + 1);
+            load(1 - buf, c + 1);
         }
         const unsigned char* x = lds + buf * BUF + lane * 16;
         half8 xa[P][U][GR];
@@ -595,10 +591,9 @@ __global__ void __launch_bounds__(512) q4_gemm_kernel(const Q4Args a, int tiles_
         }
         join(IS - 1);
     };
-    for (int c = 0; c < KC; c += NB) {
-#pragma unroll
-        for (int i = 0; i < NB; i++)
-            if (c + i < KC) step(i, c + i);
+    for (int c = 0; c < KC; c += 2) {
+        step(0, c);
+        if (c + 1 < KC) step(1, c + 1);
     }
 
     const int* exps = (const int*)((const unsigned char*)a.X + o.exps_at());
@@ -655,7 +650,6 @@ int q4_form(int x_dtype, int M, const Q4Dims& d) {
         best += (double)stream_rounds(d.tiles(), gy, per) * ((gy + slots - 1) / slots) * (f32 ? cps == 4 ? 1.4 : 0.95 : 1.2);
     }
     int form = 0;
-    if (gy > 65535) best = 1e30;  // (rows of the stream's grid)
     // {before the rounds, per round, per round and 128 k, a further round's share of the first}
     struct Cost { int gr; double base, round, k, more; };
     static constexpr Cost kBf16[3] = {{2, 8, 0.8, 6.9 / 8, 0.8}, {4, 8.5, 2, 10.3 / 8, 1}, {8, 4, 8, 17.5 / 8, 1}};
@@ -690,9 +684,10 @@ namespace aegist {
 size_t linear_q4_workspace(int x_dtype, int M, int N, int K, int G) {
     const Q4Dims d{N, K, G};
     if (N == 0) return 0;
+    M = std::min(M, kMaxRows);
     // (what the choice of any smaller M needs is enough for it)
-    for (long long m = 32; m < M + 16; m += 16)
-        if (q4_form(x_dtype, (int)std::min<long long>(m, M), d)) return XOps(M, x_dtype == AEGIST_F32 ? 2 : 1, d).bytes();
+    for (int m = 32; m < M + 16; m += 16)
+        if (q4_form(x_dtype, std::min(m, M), d)) return XOps(M, x_dtype == AEGIST_F32 ? 2 : 1, d).bytes();
     return 0;
 }
 
@@ -711,12 +706,15 @@ int launch_linear_q4(const void* X, int x_dtype, long long ldx, const void* W, f
     if (ldy < N) return fail(AEGIST_ERR_SHAPE, "linear_q4: ldy < N");
     if ((uintptr_t)W % 16) return fail(AEGIST_ERR_SHAPE, "linear_q4: W must be 16-byte aligned");
     const Q4Dims d{N, K, G};
-    const Q4Args a{X, ldx, (const unsigned char*)W, Y, ldy, M, accumulate, d, 0};
-    const int form = q4_form(x_dtype, M, d);
-    if (!form) return run_stream(a, x_dtype, st);
-    rc = check_workspace(ws, ws_bytes, XOps(M, x_dtype == AEGIST_F32 ? 2 : 1, d).bytes(), "linear_q4");
-    if (rc) return rc;
-    return run_gemm(form, a, x_dtype, ws, st);
+    for (int m = 0; m < M && !rc; m += std::min(kMaxRows, M - m)) {
+        const Q4Args a{(const char*)X + (size_t)m * ldx * xs, ldx, (const unsigned char*)W, Y + (size_t)m * ldy, ldy,
+                       std::min(kMaxRows, M - m), accumulate, d, 0};
+        const int form = q4_form(x_dtype, a.M, d);
+        if (!form) rc = run_stream(a, x_dtype, st);
+        else if (!(rc = check_workspace(ws, ws_bytes, XOps(a.M, x_dtype == AEGIST_F32 ? 2 : 1, d).bytes(), "linear_q4")))
+            rc = run_gemm(form, a, x_dtype, ws, st);
+    }
+    return rc;
 }
 
 }  // namespace aegist

@@ -412,7 +412,7 @@ int aegist_silu_mul(const float* g, const float* u, float* out, long long n, voi
  * consecutive k, w = code * scale + min, codes 0..15, scale and min fp16: the format of the
  * experts above, packed into one block of device memory ("q4", 16-byte aligned,
  * aegist_q4_bytes(N, K, group) bytes) in the order in which the matrix cores take it. K is a
- * positive multiple of the group. No counterpart in the reference, whose projections are int8.
+ * positive multiple of the group, N and K at most 2^28. No counterpart in the reference, whose projections are int8.
  * ------------------------------------------------------------------------------------- */
 /* Bytes of a packed weight; 0 for sizes that none has. */
 size_t aegist_q4_bytes(int N, int K, int group);
@@ -430,10 +430,10 @@ int aegist_q4_pack(const void* codes, const uint16_t* scale, const uint16_t* min
 /* out [N, K] fp32 (16-byte aligned) = code * scale + min. */
 int aegist_q4_dequantize(const void* q4, float* out, int N, int K, int group, void* stream);
 /* Y[m, n] (+)= sum_k X[m, k] w[n, k], Y fp32 with row stride ldy; X AEGIST_F32 | AEGIST_BF16 with row
- * stride ldx elements, rows 16-byte aligned. Deterministic. Every value of X counts with 22 bits
- * below the largest of its row; a row of X with an infinity or NaN has no finite output. Needs
- * aegist_linear_q4_workspace_bytes(x_dtype, M, N, K, group) bytes (256-byte aligned; 0 at few
- * rows). */
+ * stride ldx elements, rows 16-byte aligned. Deterministic. A value of X counts with 22 bits (bf16: all),
+ * as far as they reach 2^-39 of the largest of its row; a row with an infinity or NaN has no finite
+ * output. Needs aegist_linear_q4_workspace_bytes(x_dtype, M, N, K, group) bytes (256-byte aligned; 0 at
+ * few rows), which serve every smaller M too. */
 size_t aegist_linear_q4_workspace_bytes(int x_dtype, int M, int N, int K, int group);
 int aegist_linear_q4(const void* X, int x_dtype, long long ldx, const void* q4, float* Y, long long ldy, int M, int N,
                      int K, int group, int accumulate, void* ws, size_t ws_bytes, void* stream);

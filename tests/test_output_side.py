@@ -212,3 +212,13 @@ def test_logprobs_refuse_a_vocabulary_past_the_index(launches):
     assert L.aegist_token_logprobs(64, 0, V, 64, 64, 64, 64, 64, 1, V, 1, None, 0, None) == -1 and "2^30" in _lib.last_error()
     assert L.aegist_head_logprobs(64, 0, 64, 64, 1, None, 64, 64, 64, 64, 64, 1, V, 64, 0, 1, None, 0, None) == -1
     assert L.aegist_token_logprobs_workspace_bytes(1, V, 1) == 0
+
+
+def test_q4_sizes_past_the_index_are_refused():
+    L = _lib.lib()
+    for N, K in ((2 ** 28 + 1, 64), (8, 2 ** 28 + 64), (2 ** 31 - 1, 2 ** 31 - 64)):
+        assert L.aegist_q4_bytes(N, K, 64) == 0 and "2^28" in _lib.last_error()
+        assert L.aegist_linear_q4_workspace_bytes(1, 8, N, K, 64) == 0
+        assert L.aegist_linear_q4(64, 0, K, 64, 64, N, 1, N, K, 64, 0, None, 0, None) == -1
+    # rows go in blocks: the workspace of a projection is no larger for 2^31 of them than for 2^19
+    assert L.aegist_linear_q4_workspace_bytes(1, 2 ** 31 - 1, 64, 64, 64) == L.aegist_linear_q4_workspace_bytes(1, 2 ** 19, 64, 64, 64)

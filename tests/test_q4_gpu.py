@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 import torch
 
-from aegist_mixer import ops
+from aegist_mixer import _lib, ops
 from oracle import mixer_ref as R
 
 pytestmark = pytest.mark.gpu
@@ -141,6 +141,60 @@ def test_linear_q4_keeps_bad_rows_apart(dev, M, dtype):
     y = ops.linear_q4(x.to(dev), _pack(codes, sb, mb, dev))
     keep = (torch.arange(N) != 3) & (torch.arange(N) != 31)
     assert not torch.isfinite(y[:, ~keep]).any() and torch.equal(y[:, keep], good[:, keep])
+
+
+def test_linear_q4_of_more_rows_than_a_launch(dev):
+    """2^19 rows and some: blocks of rows, accumulating into the output's strides; offsets of X past 2^32 bytes."""
+    M, N, K, G = 2 ** 19 + 21, 24, 4608, 128
+    wt = _weight(N, K, G, 10)
+    w4 = _pack(*wt[:3], dev)
+    x = torch.randn(2 ** 16, K, device=dev).bfloat16().repeat(9, 1)[:M]
+    out = torch.full((M, N + 8), 2.0, device=dev)
+    need = _lib.lib().aegist_linear_q4_workspace_bytes(_lib.BF16, M, N, K, G)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    # (the library's own call: columns 3 to 3 + N of a wider output)
+    _lib.call("aegist_linear_q4", x.data_ptr(), _lib.BF16, K, w4.data.data_ptr(), out.data_ptr() + 12, N + 8, M, N, K, G, 1,
+              ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream)
+    assert (out[:, :3] == 2).all() and (out[:, 3 + N:] == 2).all()
+    for t in (0, 2 ** 18 - 5, 2 ** 19 - 8, 2 ** 19, M - 16):
+        xs = x[t:t + 16].cpu()
+        off = (out[t:t + 16, 3:3 + N].cpu().double() - 2 - xs.double() @ wt[3].t()).abs()
+        # (the sum with 2 rounds once more)
+        assert (off <= _bound(xs, wt[0], wt[1], wt[2], G) + 2.0 ** -24 * (off + 2 + (xs.double() @ wt[3].t()).abs())).all()
+
+
+@pytest.mark.parametrize("M", [1, 3, 40, 140])
+def test_linear_q4_of_a_weight_past_32_bits(dev, M):
+    """Codes of more than 4 GiB, scales and minima behind them: the first and the last rows' outputs."""
+    N, K, G = 2 ** 20 + 40, 8448, 64
+    g = torch.Generator(dev).manual_seed(11)
+    codes = torch.randint(0, 256, (N, K // 2), generator=g, dtype=torch.uint8, device=dev)
+    scale = (0.007 * (0.5 + torch.rand(N, K // G, generator=g, device=dev))).half()
+    mn = (-7.5 * scale.float()).half()
+    w4 = ops.q4_pack(codes, scale, mn)
+    x = torch.randn(M, K, generator=torch.Generator().manual_seed(1)).bfloat16()
+    y = ops.linear_q4(x.to(dev), w4)
+    for n in (0, N // 2, N - 24):
+        c, s, m = (t[n:n + 24].cpu() for t in (codes, scale, mn))
+        ref = x.double() @ R.q4_dequantize(c, s, m, G).t()
+        assert ((y[:, n:n + 24].cpu().double() - ref).abs() <= _bound(x, c, s, m, G)).all()
+
+
+@pytest.mark.parametrize("M", [2, 5, 17, 150])
+@pytest.mark.parametrize("K", [4224, 8192 + 64])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_linear_q4_long_rows(dev, M, K, dtype):
+    """K past what a workgroup's waves hold at a time, where later parts add to the earlier ones' output."""
+    N, G = 150, 32
+    wt = _weight(N, K, G, K)
+    w4 = _pack(*wt[:3], dev)
+    x = torch.randn(M, K, generator=torch.Generator().manual_seed(M)).to(dtype)
+    y = _check(x, w4, wt, dev)
+    res = torch.randn(M, N, generator=torch.Generator().manual_seed(2))
+    both = ops.linear_q4(x.to(dev), w4, out=res.to(dev), accumulate=True)
+    # a rounding of the sum per part of K (at most 5 of them), of what is there then
+    size = res.abs().double() + x.abs().double() @ wt[3].abs().t()
+    assert ((both - y).cpu().double() - res.double()).abs().le(6 * 2.0 ** -24 * 2 * size).all()
 
 
 def test_linear_q4_empty(dev):
