@@ -243,3 +243,85 @@ def test_same_bits_again_and_in_graphs(dev, T):
             torch.cuda.synchronize()
             for a, b in zip(o[0] + o[1], ops.head_logprobs(xi, w4, tok, top) + ops.token_logprobs(xi, tok % K, top)):
                 assert torch.equal(a, b)
+
+
+def test_more_rows_than_a_grid(dev):
+    """2^20 rows and some, and tokens at the ends of their type."""
+    T, V = 2 ** 20 + 7, 5
+    x = torch.randn(T, V, device=dev)
+    tok = torch.randint(0, V, (T,), device=dev, dtype=torch.int32)
+    tok[::1000] = -2 ** 31
+    tok[1::1000] = 2 ** 31 - 1
+    r = ops.token_logprobs(x, tok, 2)
+    assert (r.logprob[::1000] == 0).all() and torch.isnan(r.logprob[1::1000]).all()
+    for t in (slice(2, 900), slice(T - 20, T)):
+        ok = (tok[t] >= 0) & (tok[t] < V)
+        keep = torch.where(ok, tok[t], 0)
+        _check(x[t].cpu()[ok.cpu()], keep.cpu()[ok.cpu()], 2, type(r)(*(f[t][ok] for f in r)))
+
+
+@pytest.mark.parametrize("top", [0, 5])
+def test_logits_past_32_bits(dev, top):
+    """More than 2^31 logits: the rows on both sides of the offsets 2^31 and 2^32 bytes, and the last."""
+    V, T = 131072 + 3, 16500
+    x = torch.empty(T, V, device=dev, dtype=torch.bfloat16)
+    x[:64].normal_()
+    for t in range(64, T, 64):
+        x[t:t + 64] = x[:min(64, T - t)]
+    tok = torch.randint(0, V, (T,), device=dev, dtype=torch.int32)
+    r = ops.token_logprobs(x, tok, top)
+    for t in (0, 2 ** 30 // V, 2 ** 31 // V, T - 2):
+        t = slice(t, t + 2)
+        _check(x[t].cpu(), tok[t].cpu(), top, type(r)(*(f if f is None else f[t] for f in r)))
+
+
+@pytest.mark.parametrize("T", [1, 40])
+def test_two_calls_at_once(dev, T):
+    """Calls on two streams, each with a workspace of its own, do not disturb each other."""
+    V, K, top = 60001, 256, 9
+    w4 = ops.q4_quantize(0.05 * torch.randn(V, K, device=dev))
+    xs = [torch.randn(T, K, device=dev) for _ in range(2)]
+    tok = torch.randint(0, V, (T,), device=dev, dtype=torch.int32)
+    want = [ops.head_logprobs(x, w4, tok, top) + (ops.linear_q4(x, w4),) for x in xs]
+    streams = [torch.cuda.Stream() for _ in xs]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(ops.head_logprobs(xs[i], w4, tok, top) + (ops.linear_q4(xs[i], w4),))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for g in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(g, want[i]))
+
+
+@pytest.mark.parametrize("kind", ["q4", "bf16", "int8"])
+def test_head_takes_strides_and_leading_dimensions(dev, kind):
+    """Rows of a wider matrix, a batch of sequences padded with -1, and the same answers as packed rows."""
+    V, K, top = 3001, 128, 4
+    w, s, _ = _head(kind, V, K, 3, dev)
+    wide = torch.randn(2, 9, K + 64, device=dev).bfloat16()
+    x = wide[..., 64:]
+    tok = torch.randint(0, V, (2, 9), device=dev, dtype=torch.int32)
+    tok[0, 5:] = -1
+    r = ops.head_logprobs(x, w, tok, top, scale=s)
+    flat = ops.head_logprobs(x.reshape(18, K).contiguous(), w, tok.flatten(), top, scale=s)
+    assert r.logprob.shape == (2, 9) and r.top_ids.shape == (2, 9, top)
+    assert all(torch.equal(a.flatten(), b.flatten()) for a, b in zip(r, flat))
+    assert (r.logprob[0, 5:] == 0).all() and (r.logprob[0, :5] < 0).all() and torch.isfinite(r.entropy).all()
+
+
+def test_head_scales_bf16_rows(dev):
+    """A bf16 head with a scale per row, as the projections take it."""
+    V, K, T = 2003, 64, 5
+    w, _, wd = _head("bf16", V, K, 4, dev)
+    sc = (0.5 + torch.rand(V, generator=torch.Generator().manual_seed(1))).bfloat16()
+    x = torch.randn(T, K, generator=torch.Generator().manual_seed(2))
+    tok = torch.arange(T, dtype=torch.int32) * 400
+    r = ops.head_logprobs(x.to(dev), w, tok.to(dev), scale=sc.to(dev))
+    wd = wd * sc.double().unsqueeze(1)
+    off = ((2.0 ** -16 + K * 2.0 ** -24) * 2 * (x.abs().double() @ wd.abs().t())).amax(1)
+    lp, ent, _, _, _ = _ref(x.double() @ wd.t(), tok, 0)
+    assert ((r.logprob.cpu().double() - lp).abs() <= 2 * off + 2.0 ** -15).all()
+    assert ((r.entropy.cpu().double() - ent).abs() <= 40 * off + 30 * 2.0 ** -16).all()
