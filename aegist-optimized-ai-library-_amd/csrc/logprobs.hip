@@ -8,8 +8,12 @@
 // +inf anywhere in a row makes its logprobs and entropy NaN.
 //
 // One pass: a workgroup holds a segment of a row in registers, so the maximum, the sums relative to it and the
-// selection of the alternatives read it from there. Segments of a row (and, for a head, blocks of the vocabulary)
-// are joined by their maxima in fixed order; few rows are cut into many splits, which a second launch joins.
+// selection of the alternatives read it from there. Segments of a row are joined by their maxima in fixed order; few
+// long rows are cut into splits, which a second launch joins.
+//
+// Bound by HBM for many rows (2000 x 131072 fp32, 8 alternatives: 162 us, 6.5 TB/s with part of it in the last-level
+// cache; without alternatives 156), by the latency of a launch or two for few: 61 rows of 100003 in bf16 with 5 take
+// 16.5 us, the first 9 of them without any alternatives.
 #include "q4.h"
 
 #include <algorithm>
@@ -95,7 +99,8 @@ __device__ __forceinline__ void finish_top(const LogprobOut& o, int t, int j, co
                                                                : lp_key_value(key) - p.m - logf(p.z);
 }
 
-// 4 consecutive logits
+// 4 consecutive logits. again(): what follows takes them from these registers anew (bf16 values would be kept unpacked as
+// floats beside them, twice the registers)
 template <typename T> struct L4;
 template <> struct L4<float> {
     typedef float v __attribute__((ext_vector_type(4), aligned(4)));
@@ -103,19 +108,25 @@ template <> struct L4<float> {
     __device__ __forceinline__ void load(const float* p) { x = __builtin_nontemporal_load((const v*)p); }
     __device__ __forceinline__ float get(int i) const { return x[i]; }
     __device__ __forceinline__ void set(int i, float f) { x[i] = f; }
+    __device__ __forceinline__ void again() {}
 };
 template <> struct L4<uint16_t> {
-    typedef uint16_t v __attribute__((ext_vector_type(4), aligned(2)));
+    typedef uint32_t v __attribute__((ext_vector_type(2), aligned(2)));
     v x;
     __device__ __forceinline__ void load(const uint16_t* p) { x = __builtin_nontemporal_load((const v*)p); }
-    __device__ __forceinline__ float get(int i) const { return bf2f(x[i]); }
-    __device__ __forceinline__ void set(int i, float f) { x[i] = f2bf(f); }
+    __device__ __forceinline__ float get(int i) const { return i % 2 ? bf_hi(x[i / 2]) : bf_lo(x[i / 2]); }
+    __device__ __forceinline__ void set(int i, float f) {
+        const uint32_t h = __float_as_uint(f) >> 16;  // (a bf16 value)
+        x[i / 2] = i % 2 ? (x[i / 2] & 0xffffu) | h << 16 : (x[i / 2] & 0xffff0000u) | h;
+    }
+    __device__ __forceinline__ void again() { asm volatile("" : "+v"(x)); }
 };
 
 struct Lds {
     float red[3][NW];
     Part part[NW];
-    u64 thr[NW];
+    u64 key[NW];
+    uint32_t thr[2][NW];
     int count;
     u64 cand[CAP + MAX_TOP];   // candidates, after the alternatives so far
     u64 list[MAX_TOP];         // the alternatives so far, descending
@@ -134,31 +145,95 @@ __device__ __forceinline__ float wave_max_dpp(float v) {
 #undef AEG_DPP_MAX
     return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), WAVE - 1));
 }
-__device__ __forceinline__ float lane_value(float v, int j) {
-    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), j));
+// The same of unsigned values
+__device__ __forceinline__ uint32_t wave_umax_dpp(uint32_t v) {
+#define AEG_DPP_MAX(CTRL, ROWS) v = max(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, ROWS, 0xF, false))
+    AEG_DPP_MAX(0x111, 0xF);
+    AEG_DPP_MAX(0x112, 0xF);
+    AEG_DPP_MAX(0x114, 0xF);
+    AEG_DPP_MAX(0x118, 0xF);
+    AEG_DPP_MAX(0x142, 0xA);
+    AEG_DPP_MAX(0x143, 0xC);
+#undef AEG_DPP_MAX
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, WAVE - 1);
 }
 
-// The `top`-th largest of the wave's 64 values; so many of the wave's logits, where a lane's is the largest of its
-// own, are at or above it.
-__device__ __forceinline__ float nth_value(float v, int top) {
+// Bounds from below of the `top`-th largest of a workgroup's values, where v is the largest of a lane's, as the upper
+// halves of keys (0: below all). A wave's top-th largest lane is one: so many values of the wave are at or above it. The
+// smallest, over the waves, of their (top / NW)-th largest is another, closer one where values are spread evenly
+// (one row of 4000, 20 alternatives: 30 candidates are left instead of 80). Each wave leaves both in LDS.
+__device__ __forceinline__ void bound_part(Lds& s, uint32_t v, int top, int lane, int wave) {
     int r = 0;
 #pragma unroll 16
-    for (int j = 0; j < WAVE; j++) r += lane_value(v, j) > v;
-    return -wave_max_dpp(r < top ? -v : -INFINITY);
+    for (int j = 0; j < WAVE; j++) r += (uint32_t)__builtin_amdgcn_readlane((int)v, j) > v;
+    const uint32_t nth = ~wave_umax_dpp(r < top ? ~v : 0), part = ~wave_umax_dpp(r < (top + NW - 1) / NW ? ~v : 0);
+    if (lane == 0) s.thr[0][wave] = nth, s.thr[1][wave] = part;
 }
-// The same of 64 different keys, or 0 for lanes without one; 0 if there are too few.
-__device__ __forceinline__ u64 nth_key(u64 k, int top) {
-    int r = 0;
-#pragma unroll 8
-    for (int j = 0; j < WAVE; j++)
-        r += ((u64)(uint32_t)__builtin_amdgcn_readlane((int)(k >> 32), j) << 32 |
-              (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)k, j)) > k;
-    return wave_max64(r == top - 1 ? k : 0);
+__device__ __forceinline__ uint32_t bound(const Lds& s) {
+    uint32_t a = s.thr[0][0], b = s.thr[1][0];
+#pragma unroll
+    for (int w = 1; w < NW; w++) a = max(a, s.thr[0][w]), b = min(b, s.thr[1][w]);
+    return max(a, b);
 }
 
 __device__ __forceinline__ void add_candidate(Lds& s, u64 k) {
-    const int at = atomicAdd(&s.count, 1);  // (their order does not matter: they are ranked)
+    const int at = atomicAdd(&s.count, 1);
     if (at < CAP + MAX_TOP) s.cand[at] = k;
+}
+
+// Places for a wave's n candidates, behind the ones that are there already, in any order (they are ranked). -1 if there are
+// more than are ranked (the count says so).
+__device__ __forceinline__ int candidate_places(Lds& s, int n, int lane) {
+    int at = 0;
+    if (lane == 0) at = atomicAdd(&s.count, n);
+    at = __builtin_amdgcn_readfirstlane(at);
+    return at + n <= CAP + MAX_TOP ? at : -1;
+}
+__device__ __forceinline__ int lanes_below(u64 b) {
+    return __builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0));
+}
+
+// The candidates among a segment's logits: those at or above thr. Few lanes hold any. Up to HITS of those
+// at a time lay all their logits down in LDS, and the wave looks at 64 of them at once: a test and a branch per
+// register would be paid by every wave that holds a single one.
+template <int VPT>
+struct alignas(16) Hits {
+    static constexpr int LANES = 32 / VPT, EACH = 4 * VPT, ROW = EACH + 4;  // (rows 16 bytes apart in the banks)
+    float x[LANES][ROW];
+    int c[LANES];
+};
+template <int VPT, typename V>
+__device__ __forceinline__ void add_candidates(Lds& s, Hits<VPT>& hits, const V (&v)[VPT], float mt, float thr, int c, int c1,
+                                               int lane) {
+    typedef Hits<VPT> H;
+    u64 todo = __ballot(mt >= thr);
+    while (todo) {
+        const int at = lanes_below(todo), cnt = min((int)__popcll(todo), H::LANES);
+        const bool mine = (todo >> lane & 1) && at < H::LANES;
+        if (mine) {
+#pragma unroll
+            for (int i = 0; i < VPT; i++)
+                *(f32x4*)&hits.x[at][4 * i] = f32x4{v[i].get(0), v[i].get(1), v[i].get(2), v[i].get(3)};
+            hits.c[at] = c;
+        }
+        todo &= ~__ballot(mine);
+        wave_sync();
+        u64 key[2], is[2];
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const int id = lane + WAVE * j, h = id / H::EACH, k = id % H::EACH;
+            const float f = hits.x[h][k];
+            const int ce = hits.c[h] + 4 * NT * (k / 4) + k % 4;
+            key[j] = lp_key(f, ce);
+            is[j] = __ballot(h < cnt && ce < c1 && f >= thr);
+        }
+        int to = candidate_places(s, (int)__popcll(is[0]) + (int)__popcll(is[1]), lane);
+        if (to < 0) return;
+        if (is[0] >> lane & 1) s.cand[to + lanes_below(is[0])] = key[0];
+        to += (int)__popcll(is[0]);
+        if (is[1] >> lane & 1) s.cand[to + lanes_below(is[1])] = key[1];
+        wave_sync();  // (the next ones' logits go where these were read)
+    }
 }
 
 // the `top` largest of n <= CAP + MAX_TOP keys (all different, or 0) into the list, descending
@@ -173,23 +248,20 @@ __device__ __forceinline__ void rank_keys(Lds& s, int n, int top) {
 }
 
 // The `top` largest of the list's `have` keys and the N keys that each thread gives (0: none), into the list. All
-// threads call it; returns how many there are. Keys are different, so from the largest bound that the waves' lanes
-// give there are few to rank; where they are not (values in order), the largest is taken one after the other.
+// threads call it; returns how many there are. Where the bound leaves too many (values all alike or in order), the
+// largest is taken one after the other.
 template <int N, int UNROLL, typename Key>
 __device__ __forceinline__ int select_keys(Lds& s, int have, int top, Key key) {
     const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE;
     u64 k = 0;
 #pragma unroll UNROLL
     for (int i = 0; i < N; i++) k = max64(k, key(i));
-    const u64 nth = nth_key(k, top);
     __syncthreads();
-    if (lane == 0) s.thr[wave] = nth;
+    bound_part(s, (uint32_t)(k >> 32), top, lane, wave);
     if ((int)threadIdx.x < have) s.cand[threadIdx.x] = s.list[threadIdx.x];
     if (threadIdx.x == 0) s.count = have;
     __syncthreads();
-    u64 thr = have == top ? max64(s.list[top - 1], 1) : 1;
-#pragma unroll
-    for (int w = 0; w < NW; w++) thr = max64(thr, s.thr[w]);
+    u64 thr = max64((u64)bound(s) << 32, have == top ? max64(s.list[top - 1], 1) : 1);
     if (k >= thr) {
 #pragma unroll UNROLL
         for (int i = 0; i < N; i++) {
@@ -214,10 +286,10 @@ __device__ __forceinline__ int select_keys(Lds& s, int have, int top, Key key) {
             }
             best = wave_max64(best);
             __syncthreads();
-            if (lane == 0) s.thr[wave] = best;
+            if (lane == 0) s.key[wave] = best;
             __syncthreads();
 #pragma unroll
-            for (int w = 0; w < NW; w++) best = max64(best, s.thr[w]);
+            for (int w = 0; w < NW; w++) best = max64(best, s.key[w]);
             if (threadIdx.x == 0) s.list[j] = best;
             last = best;
         }
@@ -231,9 +303,10 @@ __device__ __forceinline__ int select_keys(Lds& s, int have, int top, Key key) {
 // outputs are written here.
 template <typename T, int VPT>
 __global__ void __launch_bounds__(NT) logprobs_kernel(const T* __restrict__ L, long long ld, int rows, int V, int span,
-                                                      int splits, Part* __restrict__ parts, u64* __restrict__ tops,
-                                                      const LogprobOut o) {
+                                                         int splits, Part* __restrict__ parts, u64* __restrict__ tops,
+                                                         const LogprobOut o) {
     __shared__ Lds s;
+    __shared__ Hits<VPT> hits[NW];
     const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE, top = o.top;
     constexpr int SEG = 4 * VPT * NT;
     constexpr float LOG2E = 1.44269504f, LN2 = 0.693147181f;
@@ -247,32 +320,37 @@ __global__ void __launch_bounds__(NT) logprobs_kernel(const T* __restrict__ L, l
         for (int b = c0; b < c1; b += SEG) {
             L4<T> v[VPT];
             // the thread's logits: b + 4 (NT i + thread) ..
-            const int c = b + 4 * (int)threadIdx.x;
+            const T* xb = x + b;
+            uint32_t at = 4 * threadIdx.x;
+            asm volatile("" : "+v"(at));  // (VPT offsets are not worth registers for the whole loop)
+            const int c = b + (int)at;
             if (b + SEG <= c1) {
 #pragma unroll
-                for (int i = 0; i < VPT; i++) v[i].load(x + c + 4 * NT * i);
+                for (int i = 0; i < VPT; i++) v[i].load(xb + 4 * NT * i + at);
             } else {
+                // the last segment: whole fours as above, then the one that the end cuts, -inf past it
+                const uint32_t n = c1 - b, whole = n & ~3u;
+                L4<T> rest;
 #pragma unroll
-                for (int i = 0; i < VPT; i++)
+                for (int e = 0; e < 4; e++) rest.set(e, whole + e < n ? Act<T>::ld(xb, min(whole + e, n - 1)) : -INFINITY);
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const int ce = c + 4 * NT * i + e;
-                        v[i].set(e, ce < c1 ? Act<T>::ld(x, ce) : -INFINITY);
-                    }
+                for (int i = 0; i < VPT; i++) {
+                    const uint32_t k = at + 4 * NT * i;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) v[i].set(e, -INFINITY);
+                    if (k < whole) v[i].load(xb + 4 * NT * i + at);
+                    else if (k == whole) v[i] = rest;
+                }
             }
             if (b == c0 && tok >= c0 && tok < c1) p.tok = Act<T>::ld(x, tok);  // (with the segment's, not after it)
             float mt = -INFINITY;  // the thread's largest (NaN apart)
 #pragma unroll
             for (int i = 0; i < VPT; i++)
                 mt = fmaxf(fmaxf(fmaxf(mt, v[i].get(0)), fmaxf(v[i].get(1), v[i].get(2))), v[i].get(3));
+#pragma unroll
+            for (int i = 0; i < VPT; i++) v[i].again();
             const float mw = wave_max_dpp(mt);
-            // the alternatives' lower bound: from the first segment's lanes, then from the list
-            const float nth = top && have < top ? nth_value(mt, top) : 0.f;
-            if (lane == 0) {
-                s.red[0][wave] = mw;
-                s.thr[wave] = __float_as_uint(nth);
-            }
-            if (threadIdx.x == 0) s.count = have;
+            if (lane == 0) s.red[0][wave] = mw;
             __syncthreads();
             const float m = fmaxf(fmaxf(s.red[0][0], s.red[0][1]), fmaxf(s.red[0][2], s.red[0][3]));
             // e^(x - m) = 2^y. The entropy's y is held at -200, so that a masked logit's term is 0, not 0 times -inf;
@@ -291,22 +369,27 @@ __global__ void __launch_bounds__(NT) logprobs_kernel(const T* __restrict__ L, l
                     }
                 q.z = z[0] + z[1];
                 q.s = (y2[0] + y2[1]) * LN2;
+#pragma unroll
+                for (int i = 0; i < VPT; i++) v[i].again();
             }
             q.z = wave_sum_dpp(q.z);
             q.s = wave_sum_dpp(q.s);
             if (lane == 0) s.red[1][wave] = q.z, s.red[2][wave] = q.s;
-            bool few = true;
+            if (threadIdx.x == 0) s.count = have;
+            // the alternatives' lower bound: from the first segment's lanes, then from the list
+            if (top && have < top) bound_part(s, (uint32_t)(lp_key(mt, 0) >> 32), top, lane, wave);
+            __syncthreads();
+            q.z = (s.red[1][0] + s.red[1][1]) + (s.red[1][2] + s.red[1][3]);
+            q.s = (s.red[2][0] + s.red[2][1]) + (s.red[2][2] + s.red[2][3]);
+            if (!(q.z < INFINITY)) q.bad = 1;
             if (top) {
-                float thr = -INFINITY;
-                if (have == top) {
-                    thr = lp_key_value(s.list[top - 1]);  // (NaN: nothing is above it)
-                } else {
-#pragma unroll
-                    for (int w = 0; w < NW; w++) thr = fmaxf(thr, __uint_as_float((uint32_t)s.thr[w]));
-                }
-                // later tokens lose ties with the list's. Where fewer logits than asked for are not masked, those are
-                // all of them and masked ones of the lowest tokens: of the first 2 top, at least top are
-                const bool masked = have < top && thr == -INFINITY, strict = have == top || masked;
+                // later tokens lose ties with the list's, so after it come values above its last. Where fewer logits than
+                // asked for are not masked, those are all of them and masked ones of the lowest tokens: of the first 2
+                // top, at least top are
+                uint32_t low = have == top ? (uint32_t)(s.list[top - 1] >> 32) : bound(s);
+                const bool masked = have < top && low == (uint32_t)(lp_key(-INFINITY, 0) >> 32);
+                if (have == top || masked) low++;
+                const float thr = lp_key_value((u64)low << 32);  // (past +inf: NaN, which nothing is above)
                 if ((int)threadIdx.x < have) s.cand[threadIdx.x] = s.list[threadIdx.x];
                 if (masked) {
 #pragma unroll
@@ -314,27 +397,10 @@ __global__ void __launch_bounds__(NT) logprobs_kernel(const T* __restrict__ L, l
                         if (4 * (int)threadIdx.x + e < 2 * top && c + e < c1 && v[0].get(e) == -INFINITY)
                             add_candidate(s, lp_key(-INFINITY, c + e));
                 }
-                if (strict ? mt > thr : mt >= thr) {
-#pragma unroll
-                    for (int i = 0; i < VPT; i++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            const float f = v[i].get(e);
-                            if (strict ? f > thr : f >= thr) {
-                                const int ce = c + 4 * NT * i + e;
-                                if (ce < c1) add_candidate(s, lp_key(f, ce));
-                            }
-                        }
-                }
-            }
-            __syncthreads();
-            q.z = (s.red[1][0] + s.red[1][1]) + (s.red[1][2] + s.red[1][3]);
-            q.s = (s.red[2][0] + s.red[2][1]) + (s.red[2][2] + s.red[2][3]);
-            if (!(q.z < INFINITY)) q.bad = 1;
-            if (top) {
+                add_candidates(s, hits[wave], v, mt, thr, c, c1, lane);
+                __syncthreads();
                 const int n = s.count;
-                few = n <= CAP + MAX_TOP && !q.bad;  // (NaN comes first, and no float comparison finds it)
-                if (few) {
+                if (n <= CAP + MAX_TOP && !q.bad) {  // (NaN comes first, and no float comparison finds it)
                     if (n > have) rank_keys(s, n, top);
                     have = min(top, n);
                 } else {
@@ -345,9 +411,9 @@ __global__ void __launch_bounds__(NT) logprobs_kernel(const T* __restrict__ L, l
                     });
                 }
             }
-            __syncthreads();
             join(p, q);
         }
+        if (top) __syncthreads();
         if (splits == 1) {
             if (threadIdx.x == 0) finish(o, t, V, p);
             if ((int)threadIdx.x < top) finish_top(o, t, threadIdx.x, p, s.list[threadIdx.x]);
@@ -356,7 +422,6 @@ __global__ void __launch_bounds__(NT) logprobs_kernel(const T* __restrict__ L, l
             if (threadIdx.x == 0) parts[at] = p;
             if ((int)threadIdx.x < top) tops[at * top + threadIdx.x] = (int)threadIdx.x < have ? s.list[threadIdx.x] : 0;
         }
-        __syncthreads();
     }
 }
 
@@ -415,44 +480,53 @@ int check_out(const char* who, int T, int V, const LogprobOut& o) {
     return 0;
 }
 
-// Logits of a split: few rows are cut so that about 1536 workgroups share them (6 per CU at once).
-int split_span(int T, int cols, int* small) {
-    const long long want = std::max(1LL, 1536LL / std::max(T, 1));
-    const int seg = 4 * 4 * NT;  // a segment of the small form
-    long long span = (cols + want - 1) / want;
-    *small = span <= 2 * seg;
-    const int unit = *small ? seg : 4 * seg;
-    return (int)((span + unit - 1) / unit * unit);
-}
-int split_count(int T, int cols) {
-    int small;
-    const int span = split_span(T, cols, &small);
-    return (cols + span - 1) / span;
+// How T rows are taken: segments of 1024 vpt logits, `splits` of `span` logits.
+//   - up to 8192 logits: one workgroup per row, small segments (1 row of 8000, 20 alternatives: 8.4 us, large segments
+//     10.2, two splits 10.0; 1000 rows with 5: 14, 16, 21);
+//   - up to 16384, and 32768 from 128 rows on: one workgroup per row, large segments (1 row of 16000 with 20: 10.7 us and one
+//     launch, four splits 10.9 and two launches; 200 rows of 32768 with 5: 14.2, in 7 splits 17.8. But 1 row of 32000
+//     with 20: 16, in 8 splits 10.7);
+//   - longer rows, fewer than 384: so many splits that about 1536 workgroups share them (6 per CU); of the small
+//     segments if those are up to 8192 logits (1 row of 131072 with 20: 11.6 us, in 8 large splits 16.7);
+//   - more rows: one workgroup each (500 rows of 100000 with 5: 43 us, in 3 splits 49).
+struct Form {
+    int vpt, span, splits;
+};
+Form form_of(int T, int V) {
+    auto cut = [&](int vpt, long long want) {
+        const int seg = 4 * vpt * NT;
+        const long long span = ((V + want - 1) / want + seg - 1) / seg * seg;
+        return Form{vpt, (int)span, (int)((V + span - 1) / span)};
+    };
+    if (V <= 8192) return cut(4, 1);
+    if (V <= (T < 128 ? 16384 : 32768) || T >= 384) return cut(16, 1);
+    const long long want = 1536 / T;
+    const Form f = cut(4, want);
+    return f.span <= 8192 ? f : cut(16, want);
 }
 
 size_t splits_bytes(int T, int V, int top) {
-    const int n = split_count(T, V);
-    return n > 1 ? parts_bytes(T, n, top) : 0;
+    const Form f = form_of(T, V);
+    return f.splits > 1 ? parts_bytes(T, f.splits, top) : 0;
 }
 
 int run_logprobs(const void* L, int dtype, long long ld, int T, int V, void* ws, const LogprobOut& o, hipStream_t st) {
-    int small;
-    const int span = split_span(T, V, &small), splits = (V + span - 1) / span;
+    const Form f = form_of(T, V);
     Part* parts = (Part*)ws;
-    u64* tops = (u64*)(parts + (size_t)T * splits);
-    const int grid = (int)std::min<long long>((long long)T * splits, 1 << 20);
-#define AEG_LP(TY, VPT) logprobs_kernel<TY, VPT><<<grid, NT, 0, st>>>((const TY*)L, ld, T, V, span, splits, parts, tops, o)
+    u64* tops = (u64*)(parts + (size_t)T * f.splits);
+    const int grid = (int)std::min<long long>((long long)T * f.splits, 1 << 20);
+#define AEG_LP(TY, VPT) logprobs_kernel<TY, VPT><<<grid, NT, 0, st>>>((const TY*)L, ld, T, V, f.span, f.splits, parts, tops, o)
     if (dtype == AEGIST_F32) {
-        if (small) AEG_LP(float, 4);
+        if (f.vpt == 4) AEG_LP(float, 4);
         else AEG_LP(float, 16);
     } else {
-        if (small) AEG_LP(uint16_t, 4);
+        if (f.vpt == 4) AEG_LP(uint16_t, 4);
         else AEG_LP(uint16_t, 16);
     }
 #undef AEG_LP
     int rc = after_launch("token_logprobs");
-    if (rc || splits == 1) return rc;
-    logprobs_join_kernel<<<std::min(T, 1 << 20), NT, 0, st>>>(parts, tops, T, V, splits, o);
+    if (rc || f.splits == 1) return rc;
+    logprobs_join_kernel<<<std::min(T, 1 << 20), NT, 0, st>>>(parts, tops, T, V, f.splits, o);
     return after_launch("token_logprobs");
 }
 
@@ -465,9 +539,9 @@ size_t head_logits_bytes(int T, int V) { return ((size_t)head_rows(T, V) * V * 4
 
 extern "C" size_t aegist_token_logprobs_workspace_bytes(int T, int V, int top) {
     if (T < 1 || V < 1 || V > MAX_V || top < 0 || top > MAX_TOP) return 0;
-    // what any T up to this needs: few rows are cut into the most splits, more than 768 into none
+    // what any T up to this needs: few rows are cut into the most splits, from 384 on none
     size_t need = 0;
-    for (int t = 1; t <= std::min(T, 768); t++) need = std::max(need, splits_bytes(t, V, top));
+    for (int t = 1; t < std::min(T + 1LL, 384LL); t++) need = std::max(need, splits_bytes(t, V, top));
     return need;
 }
 

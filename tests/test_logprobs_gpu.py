@@ -83,6 +83,27 @@ def test_ties_order_and_extremes(dev, T, V):
     _check(xb, tok, top, ops.token_logprobs(xb.to(dev), tok.to(dev), top))
 
 
+@pytest.mark.parametrize("T,V", [(127, 16385), (128, 30001), (383, 32769), (384, 33001), (3, 8192), (3, 8193), (5, 16384)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_where_the_cutting_changes(dev, T, V, dtype):
+    x, tok = _case(T, V, dtype, V)
+    for top in (0, 6):
+        _check(x, tok, top, ops.token_logprobs(x.to(dev), tok.to(dev), top))
+
+
+@pytest.mark.parametrize("V", [4096, 16384, 65536])
+@pytest.mark.parametrize("T", [2, 400])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_alternatives_side_by_side(dev, V, T, dtype):
+    """The alternatives lie close together: in fours 1024 apart (one lane's logits), in one run of 64, all at the end."""
+    x, tok = _case(T, V, dtype, V)
+    at = torch.arange(V)
+    x[0][(at % 1024 // 4 == 37)] += 40
+    x[1, V // 2 - 9:V // 2 + 55] += 40
+    x[T - 1, V - 64:] += 40
+    _check(x, tok, 64, ops.token_logprobs(x.to(dev), tok.to(dev), 64))
+
+
 @pytest.mark.parametrize("V", [7, 500, 40000])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_masked_rows(dev, V, dtype):
