@@ -20,14 +20,27 @@ __device__ __forceinline__ float quad_max(float x) {
     return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
-// (w - mn) / sc rounded to the nearest, ties to even, in 0..15, as doubles decide it. In fp32 the quotient is off by at
-// most 15.5 * 3 * 2^-24 < 2^-18, so only within 2^-16 of a half can doubles say otherwise: 1 value in 30000, and the
-// division in doubles is left to those (8 M values: 28 us with it for all, bf16, 9 so).
-__device__ __forceinline__ uint32_t q4_code(float w, _Float16 mn, _Float16 sc, float inv) {
-    const float q = (w - (float)mn) * inv, f = q - floorf(q);
-    float c = __builtin_rintf(q);
-    if (fabsf(f - 0.5f) < 0x1p-16f) c = (float)rint(((double)w - (double)mn) / (double)sc);
-    return (uint32_t)fminf(fmaxf(c, 0.f), 15.f);
+// The codes of 8 values: (w - mn) / sc rounded to the nearest, ties to even, in 0..15, as doubles decide it. In fp32, with
+// inv = 1 / sc (0 for no scale) to a unit, the quotient is off by at most 15.5 * 4 * 2^-24 < 2^-18, so only within 2^-16
+// of a half can doubles say otherwise: 1 value in 30000, and the division in doubles is left to the eights that hold
+// one (2048 x 4096 bf16: 28 us with it for all).
+template <typename TW>
+__device__ __forceinline__ uint32_t q4_code8(const X8<TW>& w, _Float16 mn, _Float16 sc, float inv) {
+    float c[8], off = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        const float q = (w.get(e) - (float)mn) * inv;
+        c[e] = __builtin_rintf(q);
+        off = fmaxf(off, fabsf(q - c[e]));
+    }
+    if (off > 0.5f - 0x1p-16f) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) c[e] = (float)rint(((double)w.get(e) - (double)mn) / (double)sc);
+    }
+    uint32_t p = 0;
+#pragma unroll
+    for (int e = 0; e < 8; e++) p |= q4_put((uint32_t)fminf(fmaxf(c[e], 0.f), 15.f), e);
+    return p;
 }
 
 // One wave per 16 rows x 128 k. Lane 16 q + r holds the runs k = 32 j + 8 q .. + 7 of row r, so a group's extremes
@@ -69,28 +82,30 @@ __global__ void __launch_bounds__(256) q4_quantize_kernel(const TW* __restrict__
 #pragma unroll
             for (int j = 0; j < 4; j++) lo[j] = l2[j], hi[j] = h2[j];
         }
+    // lane 16 q + r: the minimum and scale of run q
+    const float h = q == 0 ? hi[0] : q == 1 ? hi[1] : q == 2 ? hi[2] : hi[3];
+    const float l = q == 0 ? lo[0] : q == 1 ? lo[1] : q == 2 ? lo[2] : lo[3];
+    const _Float16 mn = h == INFINITY ? (_Float16)__builtin_nanf("") : (_Float16)l;
+    const double range = ((double)h - (double)mn) / 15.0;
+    const _Float16 sc = range > 0.0 ? (_Float16)range : (_Float16)0.f;
+    const uint32_t both = (uint32_t)__builtin_bit_cast(uint16_t, mn) | (uint32_t)__builtin_bit_cast(uint16_t, sc) << 16;
     u4v codes;
-    _Float16* scale = (_Float16*)(out + d.code_bytes());
-    _Float16* mins = (_Float16*)(out + d.code_bytes() + d.scale_bytes());
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-        const _Float16 mn = hi[j] == INFINITY ? (_Float16)__builtin_nanf("") : (_Float16)lo[j];
-        const double range = ((double)hi[j] - (double)mn) / 15.0;
-        const _Float16 sc = range > 0.0 ? (_Float16)range : (_Float16)0.f;
-        const int k = c * 128 + 32 * j;
+        const uint32_t u = __shfl(both, 16 * j + r, WAVE);
+        const _Float16 sj = __builtin_bit_cast(_Float16, (uint16_t)(u >> 16));
+        const float inv = sj > (_Float16)0.f ? __builtin_amdgcn_rcpf((float)sj) : 0.f;
+        codes[j] = q4_code8(w[j], __builtin_bit_cast(_Float16, (uint16_t)u), sj, inv);
+        if (!row || c * 128 + 32 * j >= d.K || inv == 0.f) codes[j] = 0;
+    }
+    _Float16* scale = (_Float16*)(out + d.code_bytes());
+    _Float16* mins = (_Float16*)(out + d.code_bytes() + d.scale_bytes());
+    const int k = c * 128 + 32 * q;
+    // (the rows past N and the groups past K too: zeros)
+    if (k % d.G == 0 && k / d.G < d.blocks8() * 8) {
         const bool in = row && k < d.K;
-        uint32_t p = 0;
-        if (sc > (_Float16)0.f) {
-            const float inv = 1.f / (float)sc;
-#pragma unroll
-            for (int e = 0; e < 8; e++) p |= q4_put(q4_code(w[j].get(e), mn, sc, inv), e);
-        }
-        codes[j] = in ? p : 0;
-        // (the rows past N and the groups past K too: zeros)
-        if (q == 0 && k % d.G == 0 && k / d.G < d.blocks8() * 8) {
-            scale[q4_group(d, n, k / d.G)] = in ? sc : (_Float16)0.f;
-            mins[q4_group(d, n, k / d.G)] = in ? mn : (_Float16)0.f;
-        }
+        scale[q4_group(d, n, k / d.G)] = in ? sc : (_Float16)0.f;
+        mins[q4_group(d, n, k / d.G)] = in ? mn : (_Float16)0.f;
     }
     if (c == d.chunks() - 1 && q == 0)
         for (int g = d.chunks() * (128 / d.G); g < d.blocks8() * 8; g++) scale[q4_group(d, n, g)] = mins[q4_group(d, n, g)] = 0;
