@@ -12,7 +12,7 @@
 // epilogue writes 16-byte pieces of Y rows. Rows past M or N are loaded from the last row (their
 // results are not stored). XCD-aware order: XCD x runs the logical tiles [x n / 8, (x + 1) n / 8),
 // grouped so that the workgroups resident on one XCD share X and W tiles in its L2.
-#include "common.h"
+#include "logprobs.h"
 
 using namespace aegist;
 
@@ -44,7 +44,95 @@ struct GemmArgs {
     const uint16_t* conv_w;  // conv epilogue: [N][4] bf16 taps, tap 3 on the newest row
     float* edge;             // conv epilogue: [M / 256][6][N] raw rows 0..2 and 253..255 of every tile
     int nseg, ldx, M, N, K, accumulate, tiles_n, ntiles, per_xcd;
+    RowStats stats;          // statistics epilogue
 };
+
+// the lanes l, l ^ 16, l ^ 32 and l ^ 48 together
+template <typename Op>
+__device__ __forceinline__ float quad_join(float x, Op op) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = op(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return op(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+// The log probabilities' share of a wave's 64 rows x 128 columns of logits (as gemm_bf16_kernel holds them): of row m the
+// maximum, the sums relative to it, the token's logit and, if asked for, the key of the largest, from the lanes
+// that hold 32 columns each. `left`: columns from the wave's first to the last there is.
+__device__ __forceinline__ void row_stats(f32x4 (&acc)[8][4], const RowStats& o, int m0, int M, int n0, int left, int split) {
+    constexpr float LOG2E = 1.44269504f, LN2 = 0.693147181f;
+    const int lane = threadIdx.x % WAVE, r16 = lane % 16, g = lane / 16;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const int m = m0 + 16 * j + r16;
+        if (left < 128) {
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) acc[i][j][e] = 16 * i + 4 * g + e < left ? acc[i][j][e] : -INFINITY;
+        }
+        Part p{-INFINITY, 0.f, 0.f, -INFINITY, 0, {}};
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) p.m = fmaxf(p.m, acc[i][j][e]);
+        p.m = quad_join(p.m, [](float a, float b) { return fmaxf(a, b); });
+        const float mz = p.m > -INFINITY ? p.m : 0.f;
+        float z[2] = {0.f, 0.f}, y2[2] = {0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float y = (acc[i][j][e] - mz) * LOG2E, ex = __builtin_amdgcn_exp2f(y);
+                z[e % 2] += ex;
+                y2[e % 2] = __builtin_fmaf(ex, fmaxf(y, -200.f), y2[e % 2]);
+            }
+        const auto add = [](float a, float b) { return a + b; };
+        p.z = quad_join(z[0] + z[1], add);
+        p.s = quad_join(y2[0] + y2[1], add) * LN2;
+        p.bad = !(p.z < INFINITY);  // (NaN, or +inf less itself)
+        const int at = m < M ? o.tokens[m] - n0 : -1;  // the token's column of the wave's
+        if (__any(at >= 0 && at < min(left, 128))) {
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) p.tok = at == 16 * i + 4 * g + e ? acc[i][j][e] : p.tok;
+            if (at >= left) p.tok = -INFINITY;
+            p.tok = quad_join(p.tok, [](float a, float b) { return fmaxf(a, b); });
+        }
+        u64 key = 0;
+        if (o.keys && left > 0) {
+            int first = 128;
+#pragma unroll
+            for (int i = 7; i >= 0; i--)
+#pragma unroll
+                for (int e = 3; e >= 0; e--) first = acc[i][j][e] == p.m ? 16 * i + 4 * g + e : first;
+            first = -(int)quad_join((float)-first, [](float a, float b) { return fmaxf(a, b); });
+            key = lp_key(p.m, n0 + first);
+            if (__any(p.bad)) {  // NaN comes first
+                u64 k = 0;
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int c = 16 * i + 4 * g + e;
+                        const u64 ke = c < left ? lp_key(acc[i][j][e], n0 + c) : 0;
+                        k = ke > k ? ke : k;
+                    }
+#pragma unroll
+                for (int w = 16; w < WAVE; w *= 2) {
+                    const u64 ko = __shfl_xor(k, w, WAVE);
+                    k = ko > k ? ko : k;
+                }
+                key = p.bad ? k : key;
+            }
+        }
+        if (g == 0 && m < M) {
+            o.parts[(size_t)m * o.splits + split] = p;
+            if (o.keys) o.keys[(size_t)m * o.splits + split] = key;
+        }
+    }
+}
 
 // kConv: the output is silu(causal depthwise conv4 over rows) of the product instead of the
 // product itself (the DeltaNet input projection followed by its short convolution): every M tile
@@ -52,7 +140,9 @@ struct GemmArgs {
 // lanes (DPP row rotations), the previous 16-row tile or, across waves, LDS; the first three rows
 // of a tile have their predecessors in another tile, so their outputs are left to
 // conv_edge_kernel, which gets the raw first and last three rows of every tile through `edge`.
-template <bool kConv>
+//
+// kStats: the outputs are the logits of an output head, of which only the rows' statistics are left (row_stats).
+template <bool kConv, bool kStats = false>
 __global__ void __launch_bounds__(512, 1) gemm_bf16_kernel(const GemmArgs ga) {
     __shared__ __attribute__((aligned(1024))) unsigned char A0[kTileBytes];  // W tile, buffer 0
     __shared__ __attribute__((aligned(1024))) unsigned char B0[kTileBytes];  // X tile, buffer 0
@@ -158,7 +248,10 @@ __global__ void __launch_bounds__(512, 1) gemm_bf16_kernel(const GemmArgs ga) {
 
     // lane (c = r16, g) of tile (i, j) holds Y[m][n .. n + 3], m = m0 + 64 wm + 16 j + c,
     // n = n0 + 128 wn + 16 i + 4 g
-    if constexpr (!kConv) {
+    if constexpr (kStats) {
+        const int c0 = n0 + 128 * wn;
+        row_stats(acc, ga.stats, m0 + 64 * wm, M, c0, N - c0, n0 / GBN * 2 + wn);
+    } else if constexpr (!kConv) {
         // each lane's segment is picked by selects over the (uniform) segment fields: indexing
         // the argument array by a lane value would read it from memory, one wait per access
         const GemmSeg s0 = ga.seg[0], s1 = ga.seg[1], s2 = ga.seg[2];
@@ -516,6 +609,28 @@ int launch_gemm_i8f32(const float* X, long long ldx, const int8_t* W, long long 
     gemm_i8f32_kernel<<<8 * per_xcd, 512, 0, st>>>(X, (int)ldx, W, (int)ldw, scale, Y, (int)ldy, M, N, K, accumulate,
                                                    tiles_n, ntiles, per_xcd);
     return after_launch("gemm_i8");
+}
+
+// The statistics of the rows of logits X[M, K] W[N, K]^T (operands as launch_gemm_bf16 takes them), which are not stored.
+int launch_gemm_bf16_stats(const uint16_t* X, long long ldx, const uint16_t* W, int M, int N, int K, const RowStats& stats,
+                           hipStream_t st) {
+    if (M <= 0 || N <= 0) return 0;
+    if (!gemm_bf16_fits(X, ldx, W, K, M, N, K) || stats.splits != row_stats_splits(N))
+        return fail(AEGIST_ERR_SHAPE, "gemm_bf16_stats: need K % 64 == 0, aligned rows, operands < 2 GiB");
+    GemmArgs ga{};
+    ga.X = X;
+    ga.seg[0] = GemmSeg{W, nullptr, 0, 0, N, K};
+    ga.nseg = 1;
+    ga.ldx = (int)ldx;
+    ga.M = M;
+    ga.N = N;
+    ga.K = K;
+    ga.tiles_n = (N + GBN - 1) / GBN;
+    ga.ntiles = (M + GBM - 1) / GBM * ga.tiles_n;
+    ga.per_xcd = (ga.ntiles + 7) / 8;
+    ga.stats = stats;
+    gemm_bf16_kernel<false, true><<<8 * ga.per_xcd, 512, 0, st>>>(ga);
+    return after_launch("gemm_bf16_stats");
 }
 
 // Y_s[M, N_s] (+)= X[M, K] W_s[N_s, K]^T for nseg (<= 3) weights sharing X, in one launch: the

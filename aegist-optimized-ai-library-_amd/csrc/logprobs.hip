@@ -14,6 +14,7 @@
 // Bound by HBM for many rows (2000 x 131072 fp32, 8 alternatives: 162 us, 6.5 TB/s with part of it in the last-level
 // cache; without alternatives 156), by the latency of a launch or two for few: 61 rows of 100003 in bf16 with 5 take
 // 16.5 us, the first 9 of them without any alternatives.
+#include "logprobs.h"
 #include "q4.h"
 
 #include <algorithm>
@@ -23,6 +24,10 @@ using namespace aegist;
 namespace aegist {
 int launch_proj(const void* X, int x_dtype, long long ldx, const void* W, int w_dtype, const uint16_t* scale, float* Y,
                 long long ldy, int M, int N, int K, int accumulate, hipStream_t st);
+bool proj_is_gemm_bf16(const void* X, int x_dtype, long long ldx, const void* W, int w_dtype, const uint16_t* scale, int M,
+                       int N, int K);
+int launch_gemm_bf16_stats(const uint16_t* X, long long ldx, const uint16_t* W, int M, int N, int K, const RowStats& stats,
+                           hipStream_t st);
 }
 
 namespace {
@@ -32,14 +37,6 @@ constexpr int MAX_V = 1 << 30;           // (a logit's index plus a segment stay
 constexpr int NT = 256, NW = NT / WAVE;  // threads, waves
 constexpr int CAP = 512;                 // candidates that are ranked at once
 
-typedef unsigned long long u64;
-
-// Order of the alternatives as one number: the larger value first (NaN before all, -0 as +0), then the lower
-// token. Larger keys come first; 0 is below every element's.
-__device__ __forceinline__ u64 lp_key(float v, uint32_t id) {
-    const uint32_t b = v != v ? 0x7fc00000u : __float_as_uint(v + 0.f);
-    return (u64)(b & 0x80000000u ? ~b : b | 0x80000000u) << 32 | (uint32_t)~id;
-}
 __device__ __forceinline__ float lp_key_value(u64 k) {
     const uint32_t b = (uint32_t)(k >> 32);
     return __uint_as_float(b & 0x80000000u ? b & 0x7fffffffu : ~b);
@@ -59,12 +56,6 @@ struct LogprobOut {
     int top;
 };
 
-// What a split of a row leaves: maximum, sums relative to it, the token's logit if it lies in the split; NaN or
-// +inf seen. Its alternatives follow apart.
-struct Part {
-    float m, z, s, tok;
-    int bad, pad[3];
-};
 __host__ __device__ inline size_t parts_bytes(int T, int splits, int top) {
     return ((size_t)T * splits * (sizeof(Part) + (size_t)top * sizeof(u64)) + 255) / 256 * 256;
 }
@@ -510,6 +501,11 @@ size_t splits_bytes(int T, int V, int top) {
     return f.splits > 1 ? parts_bytes(T, f.splits, top) : 0;
 }
 
+int run_join(const Part* parts, const u64* tops, int T, int V, int splits, const LogprobOut& o, hipStream_t st) {
+    logprobs_join_kernel<<<std::min(T, 1 << 20), NT, 0, st>>>(parts, tops, T, V, splits, o);
+    return after_launch("token_logprobs");
+}
+
 int run_logprobs(const void* L, int dtype, long long ld, int T, int V, void* ws, const LogprobOut& o, hipStream_t st) {
     const Form f = form_of(T, V);
     Part* parts = (Part*)ws;
@@ -525,9 +521,7 @@ int run_logprobs(const void* L, int dtype, long long ld, int T, int V, void* ws,
     }
 #undef AEG_LP
     int rc = after_launch("token_logprobs");
-    if (rc || f.splits == 1) return rc;
-    logprobs_join_kernel<<<std::min(T, 1 << 20), NT, 0, st>>>(parts, tops, T, V, f.splits, o);
-    return after_launch("token_logprobs");
+    return rc || f.splits == 1 ? rc : run_join(parts, tops, T, V, f.splits, o, st);
 }
 
 // rows of logits that are whole at a time: 256 MiB
@@ -588,14 +582,26 @@ extern "C" int aegist_head_logprobs(const void* X, int x_dtype, long long ldx, c
     const size_t lb = head_logits_bytes(T, V), pb = aegist_token_logprobs_workspace_bytes(block, V, top);
     float* logits = (float*)ws;
     char *pws = (char*)ws + lb, *lws = pws + pb;
+    const int splits = row_stats_splits(V);
+    Part* parts = (Part*)ws;
+    u64* keys = (u64*)(parts + (size_t)block * splits);
     for (int t = 0; t < T; t += block) {
         const int m = std::min(block, T - t);
         const void* x = (const char*)X + (size_t)t * ldx * xs;
+        const LogprobOut part{tokens + t, logprob + t, entropy + t, top_ids ? top_ids + (size_t)t * top : nullptr,
+                              top_logprobs ? top_logprobs + (size_t)t * top : nullptr, top};
+        // At most one alternative, on the tiles of gemm_bf16: the product leaves the rows' statistics in the place of the
+        // logits (40 bytes per 128 columns), which a lane has nearly to itself: it holds 32 columns of a row (1000 rows of
+        // 32768 x 2048: 119 us, 112 without alternatives, by way of the logits 159; their product alone takes 130).
+        if (top <= 1 && V >= 256 && proj_is_gemm_bf16(x, x_dtype, ldx, W, w_dtype, scale, m, V, K)) {
+            rc = launch_gemm_bf16_stats((const uint16_t*)x, ldx, (const uint16_t*)W, m, V, K,
+                                        RowStats{part.tokens, parts, top ? keys : nullptr, splits}, st);
+            if (rc || (rc = run_join(parts, keys, m, V, splits, part, st))) return rc;
+            continue;
+        }
         rc = w_dtype == AEGIST_Q4 ? launch_linear_q4(x, x_dtype, ldx, W, logits, V, m, V, K, group, 0, lws, ws_bytes - lb - pb, st)
                                   : launch_proj(x, x_dtype, ldx, W, w_dtype, scale, logits, V, m, V, K, 0, st);
         if (rc) return rc;
-        const LogprobOut part{tokens + t, logprob + t, entropy + t, top_ids ? top_ids + (size_t)t * top : nullptr,
-                              top_logprobs ? top_logprobs + (size_t)t * top : nullptr, top};
         if ((rc = run_logprobs(logits, AEGIST_F32, V, m, V, pws, part, st))) return rc;
     }
     return 0;

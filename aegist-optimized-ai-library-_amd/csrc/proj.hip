@@ -345,6 +345,13 @@ int launch_proj_splitk(const uint16_t* X, long long ldx, const uint16_t* W, floa
     return after_launch("proj_stream_splitk");
 }
 
+// Whether launch_proj makes the product on the 256 x 256 tiles of gemm_bf16 in one launch.
+bool proj_is_gemm_bf16(const void* X, int x_dtype, long long ldx, const void* W, int w_dtype, const uint16_t* scale, int M,
+                       int N, int K) {
+    return x_dtype == AEGIST_BF16 && w_dtype == AEGIST_BF16 && !scale && M > 64 && gemm_bf16_fits(X, ldx, W, K, M, N, K) &&
+           gemm_mid_form(x_dtype, 1, &N, M, K, true, true) < 0;
+}
+
 int launch_proj(const void* X, int x_dtype, long long ldx, const void* W, int w_dtype, const uint16_t* scale, float* Y,
                 long long ldy, int M, int N, int K, int accumulate, hipStream_t st) {
     return launch_proj_multi(X, x_dtype, ldx, w_dtype, 1, &W, &scale, &Y, &ldy, &N, M, K, accumulate, st);

@@ -458,7 +458,7 @@ int aegist_token_logprobs(const void* logits, int dtype, long long ld, const int
                           size_t ws_bytes, void* stream);
 /* The same for the logits X W^T of an output head W [V, K]: AEGIST_I8 with scale, AEGIST_BF16 (scale NULL
  * or per row; group is ignored) as in aegist_linear, or AEGIST_Q4 (scale is ignored). The logits are made
- * in parts in the workspace and are never whole. */
+ * in blocks of rows in the workspace, or (bf16 operands, many rows, at most one alternative) not at all. */
 size_t aegist_head_logprobs_workspace_bytes(int x_dtype, int w_dtype, int T, int V, int K, int group, int top);
 int aegist_head_logprobs(const void* X, int x_dtype, long long ldx, const void* W, int w_dtype, const uint16_t* scale,
                          const int* tokens, float* logprob, float* entropy, int* top_ids, float* top_logprobs, int T,

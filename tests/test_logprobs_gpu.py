@@ -346,3 +346,35 @@ def test_head_scales_bf16_rows(dev):
     lp, ent, _, _, _ = _ref(x.double() @ wd.t(), tok, 0)
     assert ((r.logprob.cpu().double() - lp).abs() <= 2 * off + 2.0 ** -15).all()
     assert ((r.entropy.cpu().double() - ent).abs() <= 40 * off + 30 * 2.0 ** -16).all()
+
+
+@pytest.mark.parametrize("T,V,K", [(70, 20000, 64), (300, 2053, 128), (257, 9001, 192), (1000, 32768, 64), (515, 4225, 2048)])
+@pytest.mark.parametrize("top", [0, 1])
+def test_head_of_many_rows_without_logits(dev, T, V, K, top):
+    """Rows whose statistics the product itself leaves: the answers of the logits that linear makes of the same rows (the
+    same sums in the same order, so the same ids), also where a row is NaN, infinite or all alike."""
+    g = torch.Generator().manual_seed(V)
+    w = (torch.randn(V, K, generator=g) * 0.05).bfloat16().to(dev)
+    x = torch.randn(T, K, generator=g).bfloat16()
+    x[1], x[2, 3], x[3, K - 1], x[T - 1] = 0, float("nan"), INF, 0
+    w[V - 1], w[V // 2] = w[5], w[5]  # equal logits: the lowest token
+    tok = torch.randint(0, V, (T,), generator=g, dtype=torch.int32)
+    tok[4], tok[5], tok[6], tok[7] = -1, V, V - 1, 0
+    x, tok = x.to(dev), tok.to(dev)
+    a, b = ops.head_logprobs(x, w, tok, top), ops.token_logprobs(ops.linear(x, w), tok, top)
+    # both are within the bounds of _check of the same logits
+    for p, q, off in zip(a, b, (2.0 ** -15, 60 * 2.0 ** -16, 0, 2.0 ** -15)):
+        if p is None:
+            assert q is None
+        elif p.dtype == torch.int32:
+            assert torch.equal(p, q)
+        else:
+            assert torch.equal(torch.isnan(p), torch.isnan(q)) and torch.isnan(p[2]).all() and torch.isnan(p[3]).all()
+            ok = ~torch.isnan(p)
+            assert ((p - q).abs()[ok] <= off + q.abs()[ok] * 2.0 ** -21).all()
+    assert abs(float(a.logprob[1]) + math.log(V)) < 1e-4 and abs(float(a.entropy[T - 1]) - math.log(V)) < 1e-3
+    assert a.logprob[4] == 0 and torch.isnan(a.logprob[5])
+    if top:
+        assert a.top_ids[1, 0] == 0 and a.top_ids[2, 0] == 0 and (a.top_ids[8:] != V - 1).all()
+    again = ops.head_logprobs(x, w, tok, top)
+    assert all(p is None or torch.equal(p.nan_to_num(nan=7.0), q.nan_to_num(nan=7.0)) for p, q in zip(a, again))
