@@ -582,13 +582,13 @@ def _logprob_outputs(lead, tokens, top: int, device):
     if tokens.shape != lead:
         raise AegistError("shape", -1, f"tokens {tuple(tokens.shape)} for rows {tuple(lead)}")
     _need_contig(tokens)
+    # (empty_like: torch.empty of a torch.Size takes 0.8 us longer)
+    f32 = torch.float32
+    logprob, entropy = torch.empty_like(tokens, dtype=f32), torch.empty_like(tokens, dtype=f32)
     if top <= 0:
-        return TokenLogprobs(torch.empty(lead, dtype=torch.float32, device=device),
-                             torch.empty(lead, dtype=torch.float32, device=device), None, None)
-    return TokenLogprobs(torch.empty(lead, dtype=torch.float32, device=device),
-                         torch.empty(lead, dtype=torch.float32, device=device),
-                         torch.empty(*lead, top, dtype=torch.int32, device=device),
-                         torch.empty(*lead, top, dtype=torch.float32, device=device))
+        return TokenLogprobs(logprob, entropy, None, None)
+    ids = torch.empty(*lead, top, dtype=torch.int32, device=device)
+    return TokenLogprobs(logprob, entropy, ids, torch.empty_like(ids, dtype=f32))
 
 
 def token_logprobs(logits, tokens, top: int = 0) -> TokenLogprobs:
