@@ -247,6 +247,15 @@ __device__ __forceinline__ int select_keys(Lds& s, int have, int top, Key key) {
     u64 k = 0;
 #pragma unroll UNROLL
     for (int i = 0; i < N; i++) k = max64(k, key(i));
+    if (top == 1) {  // (the largest, without a bound)
+        k = wave_max64(k);
+        if (lane == 0) s.key[wave] = k;
+        __syncthreads();
+        k = max64(max64(s.key[0], s.key[1]), max64(s.key[2], s.key[3]));
+        if (threadIdx.x == 0) s.list[0] = have ? max64(k, s.list[0]) : k;
+        __syncthreads();
+        return have || k;
+    }
     __syncthreads();
     bound_part(s, (uint32_t)(k >> 32), top, lane, wave);
     if ((int)threadIdx.x < have) s.cand[threadIdx.x] = s.list[threadIdx.x];
