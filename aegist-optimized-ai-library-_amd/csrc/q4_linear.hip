@@ -706,6 +706,11 @@ int launch_linear_q4(const void* X, int x_dtype, long long ldx, const void* W, f
     if (ldy < N) return fail(AEGIST_ERR_SHAPE, "linear_q4: ldy < N");
     if ((uintptr_t)W % 16) return fail(AEGIST_ERR_SHAPE, "linear_q4: W must be 16-byte aligned");
     const Q4Dims d{N, K, G};
+    // (workgroups read X and W while others write their part of Y)
+    const uintptr_t y0 = (uintptr_t)Y, y1 = y0 + ((M - 1) * (size_t)ldy + N) * 4;
+    auto meets = [&](const void* p, size_t n) { return (uintptr_t)p < y1 && y0 < (uintptr_t)p + n; };
+    if (meets(X, ((M - 1) * (size_t)ldx + K) * xs) || meets(W, d.bytes()))
+        return fail(AEGIST_ERR_SHAPE, "linear_q4: Y overlaps X or W");
     for (int m = 0; m < M && !rc; m += std::min(kMaxRows, M - m)) {
         const Q4Args a{(const char*)X + (size_t)m * ldx * xs, ldx, (const unsigned char*)W, Y + (size_t)m * ldy, ldy,
                        std::min(kMaxRows, M - m), accumulate, d, 0};

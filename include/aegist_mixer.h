@@ -430,7 +430,7 @@ int aegist_q4_pack(const void* codes, const uint16_t* scale, const uint16_t* min
 /* out [N, K] fp32 (16-byte aligned) = code * scale + min. */
 int aegist_q4_dequantize(const void* q4, float* out, int N, int K, int group, void* stream);
 /* Y[m, n] (+)= sum_k X[m, k] w[n, k], Y fp32 with row stride ldy; X AEGIST_F32 | AEGIST_BF16 with row
- * stride ldx elements, rows 16-byte aligned. Deterministic. A value of X counts with 22 bits (bf16: all),
+ * stride ldx elements, rows 16-byte aligned; the ranges of Y and of X or W do not overlap. Deterministic. A value of X counts with 22 bits (bf16: all),
  * as far as they reach 2^-39 of the largest of its row; a row with an infinity or NaN has no finite
  * output. Needs aegist_linear_q4_workspace_bytes(x_dtype, M, N, K, group) bytes (256-byte aligned; 0 at
  * few rows), which serve every smaller M too. */

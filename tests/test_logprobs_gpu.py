@@ -378,3 +378,30 @@ def test_head_of_many_rows_without_logits(dev, T, V, K, top):
         assert a.top_ids[1, 0] == 0 and a.top_ids[2, 0] == 0 and (a.top_ids[8:] != V - 1).all()
     again = ops.head_logprobs(x, w, tok, top)
     assert all(p is None or torch.equal(p.nan_to_num(nan=7.0), q.nan_to_num(nan=7.0)) for p, q in zip(a, again))
+
+
+def test_many_rows_of_a_wider_matrix_in_a_graph(dev):
+    """Rows with a stride, and the statistics of the product captured and replayed between eager calls."""
+    T, V, K = 300, 9001, 128
+    w = (torch.randn(V, K, device=dev) * 0.05).bfloat16()
+    wide = torch.randn(T, K + 64, device=dev).bfloat16()
+    x = wide[:, 64:]
+    tok = torch.randint(0, V, (T,), device=dev, dtype=torch.int32)
+    ops.head_logprobs(x, w, tok, 1)
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        out = ops.head_logprobs(x, w, tok, 1)
+    for _ in range(3):
+        wide.copy_(torch.randn(T, K + 64, device=dev))
+        gr.replay()
+        ops.head_logprobs(torch.randn(T + 70, K, device=dev).bfloat16(), w, torch.zeros(T + 70, device=dev, dtype=torch.int32), 1)
+        torch.cuda.synchronize()
+        for a, b in zip(out, ops.head_logprobs(x.contiguous(), w, tok, 1)):
+            assert torch.equal(a, b)
+
+
+def test_one_row_without_leading_dimensions(dev):
+    x, tok = _case(1, 700, torch.float32, 5)
+    a, b = ops.token_logprobs(x[0].to(dev), tok[0].to(dev), 3), ops.token_logprobs(x.to(dev), tok.to(dev), 3)
+    assert a.logprob.shape == () and a.top_ids.shape == (3,)
+    assert all(torch.equal(p, q[0]) for p, q in zip(a, b))

@@ -222,3 +222,13 @@ def test_q4_sizes_past_the_index_are_refused():
         assert L.aegist_linear_q4(64, 0, K, 64, 64, N, 1, N, K, 64, 0, None, 0, None) == -1
     # rows go in blocks: the workspace of a projection is no larger for 2^31 of them than for 2^19
     assert L.aegist_linear_q4_workspace_bytes(1, 2 ** 31 - 1, 64, 64, 64) == L.aegist_linear_q4_workspace_bytes(1, 2 ** 19, 64, 64, 64)
+
+
+def test_linear_q4_refuses_an_output_that_overlaps():
+    L = _lib.lib()
+    def call(x, w, y, M=2, N=64, K=64):
+        return L.aegist_linear_q4(x, 0, K, w, y, N, M, N, K, 64, 0, None, 0, None)
+    base, w = 1 << 20, L.aegist_q4_bytes(64, 64, 64)
+    for x, q, y in ((base, base << 1, base), (base, base << 1, base + 256 + 252), (base + 252 + 4, base << 1, base),
+                    (base, base << 1, (base << 1) + w - 4), (base, base << 1, (base << 1) - 508)):
+        assert call(x, q, y) == -1 and "overlaps" in _lib.last_error()
