@@ -11,8 +11,8 @@
 // selection of the alternatives read it from there. Segments of a row are joined by their maxima in fixed order; few
 // long rows are cut into splits, which a second launch joins.
 //
-// Bound by HBM for many rows (2000 x 131072 fp32, 8 alternatives: 162 us, 6.5 TB/s with part of it in the last-level
-// cache; without alternatives 156), by the latency of a launch or two for few: 61 rows of 100003 in bf16 with 5 take
+// Bound by HBM for many rows (2000 x 131072 fp32, 8 alternatives: 160 us, 6.5 TB/s with part of it in the last-level
+// cache; without alternatives 154), by the latency of a launch or two for few: 61 rows of 100003 in bf16 with 5 take
 // 16.5 us, the first 9 of them without any alternatives.
 #include "logprobs.h"
 #include "q4.h"
@@ -186,10 +186,11 @@ __device__ __forceinline__ int lanes_below(u64 b) {
 
 // The candidates among a segment's logits: those at or above thr. Few lanes hold any. Up to HITS of those
 // at a time lay all their logits down in LDS, and the wave looks at 64 of them at once: a test and a branch per
-// register would be paid by every wave that holds a single one.
+// register would be paid by every wave that holds a single one. (1703 rows of 38708 bf16, 20 alternatives: 57 us with
+// 4 lanes of 64 logits at a time, 64 with 2, 63 with 8.)
 template <int VPT>
 struct alignas(16) Hits {
-    static constexpr int LANES = 32 / VPT, EACH = 4 * VPT, ROW = EACH + 4;  // (rows 16 bytes apart in the banks)
+    static constexpr int LANES = VPT == 4 ? 8 : 4, EACH = 4 * VPT, ROW = EACH + 4, J = LANES * EACH / WAVE;  // (rows 16 bytes apart in the banks)
     float x[LANES][ROW];
     int c[LANES];
 };
@@ -209,20 +210,24 @@ __device__ __forceinline__ void add_candidates(Lds& s, Hits<VPT>& hits, const V 
         }
         todo &= ~__ballot(mine);
         wave_sync();
-        u64 key[2], is[2];
+        u64 key[H::J], is[H::J];
+        int n = 0;
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
+        for (int j = 0; j < H::J; j++) {
             const int id = lane + WAVE * j, h = id / H::EACH, k = id % H::EACH;
             const float f = hits.x[h][k];
             const int ce = hits.c[h] + 4 * NT * (k / 4) + k % 4;
             key[j] = lp_key(f, ce);
             is[j] = __ballot(h < cnt && ce < c1 && f >= thr);
+            n += (int)__popcll(is[j]);
         }
-        int to = candidate_places(s, (int)__popcll(is[0]) + (int)__popcll(is[1]), lane);
+        int to = candidate_places(s, n, lane);
         if (to < 0) return;
-        if (is[0] >> lane & 1) s.cand[to + lanes_below(is[0])] = key[0];
-        to += (int)__popcll(is[0]);
-        if (is[1] >> lane & 1) s.cand[to + lanes_below(is[1])] = key[1];
+#pragma unroll
+        for (int j = 0; j < H::J; j++) {
+            if (is[j] >> lane & 1) s.cand[to + lanes_below(is[j])] = key[j];
+            to += (int)__popcll(is[j]);
+        }
         wave_sync();  // (the next ones' logits go where these were read)
     }
 }
@@ -376,17 +381,18 @@ __global__ void __launch_bounds__(NT) logprobs_kernel(const T* __restrict__ L, l
             q.s = wave_sum_dpp(q.s);
             if (lane == 0) s.red[1][wave] = q.z, s.red[2][wave] = q.s;
             if (threadIdx.x == 0) s.count = have;
-            // the alternatives' lower bound: from the first segment's lanes, then from the list
-            if (top && have < top) bound_part(s, (uint32_t)(lp_key(mt, 0) >> 32), top, lane, wave);
+            // the alternatives' lower bound: from the first segment's lanes (of one: the maximum), then from the list
+            if (top > 1 && have < top) bound_part(s, (uint32_t)(lp_key(mt, 0) >> 32), top, lane, wave);
             __syncthreads();
             q.z = (s.red[1][0] + s.red[1][1]) + (s.red[1][2] + s.red[1][3]);
             q.s = (s.red[2][0] + s.red[2][1]) + (s.red[2][2] + s.red[2][3]);
             if (!(q.z < INFINITY)) q.bad = 1;
-            if (top) {
+            const uint32_t most = (uint32_t)(lp_key(m, 0) >> 32);
+            if (top && (have < top || q.bad || most > (uint32_t)(s.list[top - 1] >> 32))) {
                 // later tokens lose ties with the list's, so after it come values above its last. Where fewer logits than
                 // asked for are not masked, those are all of them and masked ones of the lowest tokens: of the first 2
                 // top, at least top are
-                uint32_t low = have == top ? (uint32_t)(s.list[top - 1] >> 32) : bound(s);
+                uint32_t low = have == top ? (uint32_t)(s.list[top - 1] >> 32) : top == 1 ? most : bound(s);
                 const bool masked = have < top && low == (uint32_t)(lp_key(-INFINITY, 0) >> 32);
                 if (have == top || masked) low++;
                 const float thr = lp_key_value((u64)low << 32);  // (past +inf: NaN, which nothing is above)
@@ -481,9 +487,9 @@ int check_out(const char* who, int T, int V, const LogprobOut& o) {
 }
 
 // How T rows are taken: segments of 1024 vpt logits, `splits` of `span` logits.
-//   - up to 8192 logits: one workgroup per row, small segments (1 row of 8000, 20 alternatives: 8.4 us, large segments
-//     10.2, two splits 10.0; 1000 rows with 5: 14, 16, 21);
-//   - up to 16384, and 32768 from 128 rows on: one workgroup per row, large segments (1 row of 16000 with 20: 10.7 us and one
+//   - up to 8192 logits: one workgroup per row, small segments (1 row of 8000, 20 alternatives: 9.1 us, large segments
+//     9.4, two splits 10.0; 1000 rows with 5: 14, 16, 21);
+//   - up to 16384, and 32768 from 128 rows on: one workgroup per row, large segments (1 row of 16000 with 20: 8.9 us and one
 //     launch, four splits 10.9 and two launches; 200 rows of 32768 with 5: 14.2, in 7 splits 17.8. But 1 row of 32000
 //     with 20: 16, in 8 splits 10.7);
 //   - longer rows, fewer than 384: so many splits that about 1536 workgroups share them (6 per CU); of the small
