@@ -12,6 +12,21 @@ __device__ __forceinline__ size_t q4_group(const Q4Dims& d, int n, int g) {
     return ((size_t)(n / 16) * d.blocks8() + g / 8) * 128 + (n % 16) * 8 + g % 8;
 }
 
+// (fminf and fmaxf would first make a quiet NaN of every value, an instruction each)
+__device__ __forceinline__ float min3(float a, float b, float c) {
+    asm("v_min3_f32 %0, %0, %1, %2" : "+v"(a) : "v"(b), "v"(c));
+    return a;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    asm("v_max3_f32 %0, %0, %1, %2" : "+v"(a) : "v"(b), "v"(c));
+    return a;
+}
+
+__device__ __forceinline__ float abs_max3(float a, float b, float c) {
+    asm("v_max3_f32 %0, %0, |%1|, |%2|" : "+v"(a) : "v"(b), "v"(c));
+    return a;
+}
+
 // largest of the lanes l, l ^ 16, l ^ 32 and l ^ 48
 __device__ __forceinline__ float quad_max(float x) {
     const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -28,10 +43,11 @@ template <typename TW>
 __device__ __forceinline__ uint32_t q4_code8(const X8<TW>& w, _Float16 mn, _Float16 sc, float inv) {
     float c[8], off = 0.f;
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-        const float q = (w.get(e) - (float)mn) * inv;
-        c[e] = __builtin_rintf(q);
-        off = fmaxf(off, fabsf(q - c[e]));
+    for (int e = 0; e < 8; e += 2) {
+        const float q0 = (w.get(e) - (float)mn) * inv, q1 = (w.get(e + 1) - (float)mn) * inv;
+        c[e] = __builtin_rintf(q0);
+        c[e + 1] = __builtin_rintf(q1);
+        off = abs_max3(off, q0 - c[e], q1 - c[e + 1]);
     }
     if (off > 0.5f - 0x1p-16f) {
 #pragma unroll
@@ -39,7 +55,7 @@ __device__ __forceinline__ uint32_t q4_code8(const X8<TW>& w, _Float16 mn, _Floa
     }
     uint32_t p = 0;
 #pragma unroll
-    for (int e = 0; e < 8; e++) p |= q4_put((uint32_t)fminf(fmaxf(c[e], 0.f), 15.f), e);
+    for (int e = 0; e < 8; e++) p |= q4_put((uint32_t)__builtin_amdgcn_fmed3f(c[e], 0.f, 15.f), e);
     return p;
 }
 
@@ -60,12 +76,14 @@ __global__ void __launch_bounds__(256) q4_quantize_kernel(const TW* __restrict__
 #pragma unroll
     for (int j = 0; j < 4; j++) {
         lo[j] = hi[j] = w[j].get(0);
+        float bad = 0.f;  // NaN with a NaN or infinity among the values, which the extremes may pass over
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const float f = w[j].get(e);
-            lo[j] = fminf(lo[j], f);
-            hi[j] = fmaxf(hi[j], fabsf(f) <= 65504.f ? f : INFINITY);
+        for (int e = 0; e < 8; e += 2) {
+            lo[j] = min3(lo[j], w[j].get(e), w[j].get(e + 1));
+            hi[j] = max3(hi[j], w[j].get(e), w[j].get(e + 1));
+            bad = __builtin_fmaf(w[j].get(e), 0.f, __builtin_fmaf(w[j].get(e + 1), 0.f, bad));
         }
+        if (!(bad == 0.f && hi[j] <= 65504.f && lo[j] >= -65504.f)) hi[j] = INFINITY;
         lo[j] = -quad_max(-lo[j]);
         hi[j] = quad_max(hi[j]);
     }
