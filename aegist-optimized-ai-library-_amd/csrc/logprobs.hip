@@ -123,6 +123,12 @@ struct Lds {
     u64 list[MAX_TOP];         // the alternatives so far, descending
 };
 
+// (fmaxf would first make a quiet NaN of every value, an instruction each)
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    asm("v_max3_f32 %0, %0, %1, %2" : "+v"(a) : "v"(b), "v"(c));
+    return a;
+}
+
 // Largest value of the wave by DPP steps (as wave_sum_dpp), in every lane
 __device__ __forceinline__ float wave_max_dpp(float v) {
 #define AEG_DPP_MAX(CTRL, ROWS) \
@@ -348,10 +354,10 @@ __global__ void __launch_bounds__(NT) logprobs_kernel(const T* __restrict__ L, l
                 }
             }
             if (b == c0 && tok >= c0 && tok < c1) p.tok = Act<T>::ld(x, tok);  // (with the segment's, not after it)
-            float mt = -INFINITY;  // the thread's largest (NaN apart)
+            float mt = -INFINITY;  // the thread's largest (quiet NaN apart)
 #pragma unroll
             for (int i = 0; i < VPT; i++)
-                mt = fmaxf(fmaxf(fmaxf(mt, v[i].get(0)), fmaxf(v[i].get(1), v[i].get(2))), v[i].get(3));
+                mt = max3(max3(mt, v[i].get(0), v[i].get(1)), v[i].get(2), v[i].get(3));
 #pragma unroll
             for (int i = 0; i < VPT; i++) v[i].again();
             const float mw = wave_max_dpp(mt);
@@ -361,7 +367,7 @@ __global__ void __launch_bounds__(NT) logprobs_kernel(const T* __restrict__ L, l
             // e^(x - m) = 2^y. The entropy's y is held at -200, so that a masked logit's term is 0, not 0 times -inf;
             // NaN reaches z.
             const float mz = m > -INFINITY ? m : 0.f;
-            Part q{m, 0.f, 0.f, -INFINITY, m == INFINITY, {}};
+            Part q{m, 0.f, 0.f, -INFINITY, !(m < INFINITY), {}};
             if (m < INFINITY) {
                 float z[2] = {0.f, 0.f}, y2[2] = {0.f, 0.f};
 #pragma unroll

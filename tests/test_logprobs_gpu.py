@@ -142,6 +142,24 @@ def test_nan_infinity_and_other_tokens(dev, T, V):
     _check(x[3:], keep[3:], 4, ops.token_logprobs(x[3:].to(dev), keep[3:].to(dev), 4))
 
 
+@pytest.mark.parametrize("dtype,bits", [(torch.float32, 0x7f800001), (torch.float32, -0x400001), (torch.bfloat16, 0x7f81), (torch.bfloat16, -0x7f)])
+@pytest.mark.parametrize("V", [300, 9001, 70001])
+@pytest.mark.parametrize("top", [0, 1, 7])
+def test_nan_of_either_kind(dev, dtype, bits, V, top):
+    """Signaling NaNs of either sign, which maxima treat as they do not treat quiet ones."""
+    x, tok = _case(6, V, dtype, 9)
+    raw = x.view(torch.int32 if dtype == torch.float32 else torch.int16)
+    raw[1, V // 3] = raw[4, V - 1] = bits
+    assert torch.isnan(x[1, V // 3])
+    r = ops.token_logprobs(x.to(dev), tok.to(dev), top)
+    for t, at in ((1, V // 3), (4, V - 1)):
+        assert torch.isnan(r.logprob[t]) and torch.isnan(r.entropy[t])
+        if top:
+            assert r.top_ids[t, 0] == at and torch.isnan(r.top_logprobs[t]).all()
+    keep = torch.tensor([0, 2, 3, 5])
+    _check(x[keep], tok[keep], top, type(r)(*(f if f is None else f[keep.to(dev)] for f in r)))
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("T", [4, 300])
 def test_strides_and_odd_places(dev, T, dtype):
