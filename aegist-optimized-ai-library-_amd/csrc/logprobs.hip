@@ -554,10 +554,10 @@ size_t head_logits_bytes(int T, int V) { return ((size_t)head_rows(T, V) * V * 4
 
 extern "C" size_t aegist_token_logprobs_workspace_bytes(int T, int V, int top) {
     if (T < 1 || V < 1 || V > MAX_V || top < 0 || top > MAX_TOP) return 0;
-    // what any T up to this needs: few rows are cut into the most splits, from 384 on none
-    size_t need = 0;
-    for (int t = 1; t < std::min(T + 1LL, 384LL); t++) need = std::max(need, splits_bytes(t, V, top));
-    return need;
+    // no T up to this needs more: rows of up to 16384 logits are not cut, others into splits of at least 4096 and of no more
+    // than 1536 in all
+    if (V <= 16384) return 0;
+    return parts_bytes((int)std::min(1536LL, T * ((V + 4095LL) / 4096)), 1, top);
 }
 
 extern "C" int aegist_token_logprobs(const void* logits, int dtype, long long ld, const int* tokens, float* logprob,
@@ -595,12 +595,11 @@ extern "C" int aegist_head_logprobs(const void* X, int x_dtype, long long ldx, c
     if (w_dtype == AEGIST_Q4 && (rc = check_q4("head_logprobs", V, K, group))) return rc;
     if (T == 0) return 0;
     if (!X || !W || K < 1) return fail(AEGIST_ERR_SHAPE, "head_logprobs: null operand or K < 1");
-    rc = check_workspace(ws, ws_bytes, aegist_head_logprobs_workspace_bytes(x_dtype, w_dtype, T, V, K, group, top),
-                         "head_logprobs");
-    if (rc) return rc;
     const hipStream_t st = AEG_STREAM(stream);
     const int block = head_rows(T, V), xs = x_dtype == AEGIST_F32 ? 4 : 2;
     const size_t lb = head_logits_bytes(T, V), pb = aegist_token_logprobs_workspace_bytes(block, V, top);
+    rc = check_workspace(ws, ws_bytes, lb + pb, "head_logprobs");  // (what is behind them linear_q4 checks)
+    if (rc) return rc;
     float* logits = (float*)ws;
     char *pws = (char*)ws + lb, *lws = pws + pb;
     const int splits = row_stats_splits(V);

@@ -232,3 +232,14 @@ def test_linear_q4_refuses_an_output_that_overlaps():
     for x, q, y in ((base, base << 1, base), (base, base << 1, base + 256 + 252), (base + 252 + 4, base << 1, base),
                     (base, base << 1, (base << 1) + w - 4), (base, base << 1, (base << 1) - 508)):
         assert call(x, q, y) == -1 and "overlaps" in _lib.last_error()
+
+
+def test_head_refuses_a_workspace_without_the_operands_of_a_4_bit_product():
+    L = _lib.lib()
+    T, V, K = 4000, 8192, 2048  # (tiles, with rows as operands in the workspace)
+    need = L.aegist_head_logprobs_workspace_bytes(1, 3, T, V, K, 64, 0)
+    assert need > L.aegist_head_logprobs_workspace_bytes(1, 1, T, V, K, 64, 0)   # (bf16: logits alone)
+    def call(n):
+        return L.aegist_head_logprobs(1 << 40, 1, K, 1 << 41, 3, None, 64, 64, 64, None, None, T, V, K, 64, 0, 1 << 42, n, None)
+    assert call(need - 1) == -2 and "linear_q4" in _lib.last_error()
+    assert call(100) == -2 and "head_logprobs" in _lib.last_error()
