@@ -314,8 +314,8 @@ __device__ __forceinline__ int select_keys(Lds& s, int have, int top, Key key) {
 // outputs are written here.
 template <typename T, int VPT>
 __global__ void __launch_bounds__(NT) logprobs_kernel(const T* __restrict__ L, long long ld, int rows, int V, int span,
-                                                         int splits, Part* __restrict__ parts, u64* __restrict__ tops,
-                                                         const LogprobOut o) {
+                                                      int splits, Part* __restrict__ parts, u64* __restrict__ tops,
+                                                      const LogprobOut o) {
     __shared__ Lds s;
     __shared__ Hits<VPT> hits[NW];
     const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE, top = o.top;

@@ -454,7 +454,7 @@ __device__ __forceinline__ void q4_g2lds(const void* src, void* lds) {
 // GR: 16-row tiles, of the workgroup and of each wave.
 template <int P, int SPG, int GR>
 __global__ void __launch_bounds__(512) q4_gemm_kernel(const Q4Args a, int tiles_m, int tiles_n, int ntiles, int per_xcd) {
-    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];  // [2 stages][GR][P][4 steps][1 KB]
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];  // [2 stages][GR][P][4 steps][1 KB], exponents [GM]
     constexpr int GM = 16 * GR, BUF = GR * P * 4 * 1024, GP = 4 / SPG;
     // steps whose products are summed before they are scaled: two of one group, where X's operands leave the registers
     constexpr int U = P == 2 || SPG == 1 ? 1 : 2;
@@ -499,6 +499,10 @@ __global__ void __launch_bounds__(512) q4_gemm_kernel(const Q4Args a, int tiles_
     };
     stage(0, 0);
     load(0, 0);
+    // (the rows' exponents for the end, where their latency would stand alone)
+    int* exps = (int*)(lds + 2 * BUF);
+    if (threadIdx.x < GM)
+        exps[threadIdx.x] = ((const int*)((const unsigned char*)a.X + o.exps_at()))[min(bm * GM + (int)threadIdx.x, xt * 16 - 1)];
 
     // the minima's term first, in the units of the codes' sums
     f32x4 acc[GR][GC];
@@ -596,11 +600,10 @@ __global__ void __launch_bounds__(512) q4_gemm_kernel(const Q4Args a, int tiles_
         if (c + 1 < KC) step(1, c + 1);
     }
 
-    const int* exps = (const int*)((const unsigned char*)a.X + o.exps_at());
 #pragma unroll
     for (int m = 0; m < GR; m++) {
         const int row = bm * GM + m * 16 + 4 * q;
-        const int4 e = *(const int4*)(exps + min(row, xt * 16 - 4));
+        const int4 e = *(const int4*)(exps + m * 16 + 4 * q);
         const int es[4] = {18 - e.x, 18 - e.y, 18 - e.z, 18 - e.w};
 #pragma unroll
         for (int n = 0; n < GC; n++) {
@@ -619,7 +622,7 @@ __global__ void __launch_bounds__(512) q4_gemm_kernel(const Q4Args a, int tiles_
 template <int P, int SPG, int GR>
 int launch_gemm(const Q4Args& a, hipStream_t st) {
     const int tm = (a.M + 16 * GR - 1) / (16 * GR), tn = (a.d.N + GN - 1) / GN, n = tm * tn, per = (n + 7) / 8;
-    constexpr int lds = 2 * (GR * P * 4 * 1024);
+    constexpr int lds = 2 * (GR * P * 4 * 1024) + GR * 64;
     if (lds > 65536)
         AEG_HIP(hipFuncSetAttribute((const void*)q4_gemm_kernel<P, SPG, GR>, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
     q4_gemm_kernel<P, SPG, GR><<<8 * per, 512, lds, st>>>(a, tm, tn, n, per);
