@@ -12,8 +12,8 @@
 // long rows are cut into splits, which a second launch joins.
 //
 // Bound by HBM for many rows (2000 x 131072 fp32, 8 alternatives: 160 us, 6.5 TB/s with part of it in the last-level
-// cache; without alternatives 154), by the latency of a launch or two for few: 61 rows of 100003 in bf16 with 5 take
-// 16.5 us, the first 9 of them without any alternatives.
+// cache; without alternatives 154), by the latency of a launch or two for few: 61 rows of 100003 in bf16 take 9.8 us, with
+// 5 alternatives 14.2.
 #include "logprobs.h"
 #include "q4.h"
 
@@ -158,12 +158,30 @@ __device__ __forceinline__ uint32_t wave_umax_dpp(uint32_t v) {
 // Bounds from below of the `top`-th largest of a workgroup's values, where v is the largest of a lane's, as the upper
 // halves of keys (0: below all). A wave's top-th largest lane is one: so many values of the wave are at or above it. The
 // smallest, over the waves, of their (top / NW)-th largest is another, closer one where values are spread evenly
-// (one row of 4000, 20 alternatives: 30 candidates are left instead of 80). Each wave leaves both in LDS.
+// (one row of 4000, 20 alternatives: 30 candidates are left instead of 80). Each wave leaves both in LDS. A few are taken
+// by maxima one after the other, more by the ranks of all lanes (61 rows of 100003 bf16, 5 alternatives: 14.2 us, by ranks
+// 16.7; 1 row of 131072 with 12 10.9 by ranks, 11.2).
+constexpr int kFewTop = 8;
 __device__ __forceinline__ void bound_part(Lds& s, uint32_t v, int top, int lane, int wave) {
-    int r = 0;
+    const int share = (top + NW - 1) / NW;
+    uint32_t nth, part = 0;
+    if (top <= kFewTop) {
+        uint32_t rest = v;
+        int n = 0;  // lanes so far
+        do {
+            nth = wave_umax_dpp(rest);
+            const bool is = rest == nth;
+            if (n < share) part = nth;
+            n += (int)__popcll(__ballot(is));
+            rest = is ? 0 : rest;
+        } while (n < top);
+    } else {
+        int r = 0;
 #pragma unroll 16
-    for (int j = 0; j < WAVE; j++) r += (uint32_t)__builtin_amdgcn_readlane((int)v, j) > v;
-    const uint32_t nth = ~wave_umax_dpp(r < top ? ~v : 0), part = ~wave_umax_dpp(r < (top + NW - 1) / NW ? ~v : 0);
+        for (int j = 0; j < WAVE; j++) r += (uint32_t)__builtin_amdgcn_readlane((int)v, j) > v;
+        nth = ~wave_umax_dpp(r < top ? ~v : 0);
+        part = ~wave_umax_dpp(r < share ? ~v : 0);
+    }
     if (lane == 0) s.thr[0][wave] = nth, s.thr[1][wave] = part;
 }
 __device__ __forceinline__ uint32_t bound(const Lds& s) {
@@ -493,14 +511,14 @@ int check_out(const char* who, int T, int V, const LogprobOut& o) {
 }
 
 // How T rows are taken: segments of 1024 vpt logits, `splits` of `span` logits.
-//   - up to 8192 logits: one workgroup per row, small segments (1 row of 8000, 20 alternatives: 9.1 us, large segments
-//     9.4, two splits 10.0; 1000 rows with 5: 14, 16, 21);
-//   - up to 16384, and 32768 from 128 rows on: one workgroup per row, large segments (1 row of 16000 with 20: 8.9 us and one
-//     launch, four splits 10.9 and two launches; 200 rows of 32768 with 5: 14.2, in 7 splits 17.8. But 1 row of 32000
-//     with 20: 16, in 8 splits 10.7);
+//   - up to 8192 logits: one workgroup per row, small segments (1 row of 8000, 20 alternatives: 8.8 us, large segments
+//     9.5, two splits 10.3; 1000 rows with 5: 12, 14, 18);
+//   - up to 16384, and 32768 from 128 rows on: one workgroup per row, large segments (1 row of 16000 with 20: 9.1 us and one
+//     launch, four splits 11.2 and two launches; 200 rows of 32768 with 5: 13.0, in 8 splits 15.4. But 1 row of 32000
+//     with 20: 14.4, in 8 splits 11.0);
 //   - longer rows, fewer than 384: so many splits that about 1536 workgroups share them (6 per CU); of the small
-//     segments if those are up to 8192 logits (1 row of 131072 with 20: 11.6 us, in 8 large splits 16.7);
-//   - more rows: one workgroup each (500 rows of 100000 with 5: 43 us, in 3 splits 49).
+//     segments if those are up to 8192 logits (1 row of 131072 with 20: 11.9 us, in 8 large splits 15.3);
+//   - more rows: one workgroup each (500 rows of 100000 with 5: 42 us, in 3 splits 46).
 struct Form {
     int vpt, span, splits;
 };
