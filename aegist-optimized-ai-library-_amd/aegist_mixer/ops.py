@@ -462,15 +462,16 @@ def _scratch(nbytes: int, device):
 
 def _rows(x, what: str):
     """x [..., K] as [M, K] with contiguous rows, and its row stride."""
-    if x.dim() < 1 or x.shape[-1] == 0:
+    shape = x.shape
+    if len(shape) == 0 or shape[-1] == 0:
         raise AegistError("shape", -1, f"{what} needs a last dimension")
-    if x.dim() != 2:
-        x = x.reshape(-1, x.shape[-1])
-    M, K = x.shape
+    if len(shape) != 2:
+        x = x.reshape(-1, shape[-1])
+        shape = x.shape
     ld, one = x.stride()
-    if one != 1 and K > 1:
+    if one != 1 and shape[1] > 1:
         raise AegistError("layout", -1, f"{what} rows must be contiguous")
-    return x, ld if M > 1 else -(-K // 8) * 8
+    return x, ld if shape[0] > 1 else -(-shape[1] // 8) * 8
 
 
 class Q4Weight:

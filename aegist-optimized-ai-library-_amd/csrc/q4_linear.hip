@@ -639,10 +639,10 @@ int gemm_spg(const Q4Args& a, hipStream_t st) {
 
 // The kernel of M rows: 0 for the stream, else the GR of the tiles (32, 64 or 128 rows of X x 256 of W), whichever the
 // estimate is shortest for (us; fitted to M 64 to 4000, N 512 to 32768, K 512 to 4096; over 176 other sizes of these
-// ranges the choice is at most 9% above the fastest). The stream: 1.2 per round of tiles (fp32 X 0.95, 1.4 in slices of 512), all rows of X at once. The
-// tiles: rounds of 256 workgroups, each a walk along K; of the small ones, two of a CU overlap. Measured (bf16, K =
-// 2048; stream, 32, 64, 128 rows): 1000 rows x 512 12.9, 22.6, 28.8, 43.6; 1000 x 4096 46.9, 33.9, 32.9, 45.3; 200 x
-// 8192 31.6, 24.2, 28.6, 41.2; 4000 x 8192 300, 195, 188, 172.
+// ranges the choice is at most 9% above the fastest). The stream: 1.2 per round of tiles (fp32 X 0.95, 1.4 in slices of
+// 512), all rows of X at once. The tiles: rounds of 256 workgroups, each a walk along K; of the small ones, two of a CU
+// overlap. Measured (bf16, K = 2048; stream, 32, 64, 128 rows): 1000 rows x 512 12.9, 22.6, 28.8, 43.6; 1000 x 4096
+// 46.9, 33.9, 32.9, 45.3; 200 x 8192 31.6, 24.2, 28.6, 41.2; 4000 x 8192 300, 190, 184, 168.
 int q4_form(int x_dtype, int M, const Q4Dims& d) {
     if (M <= 16) return 0;
     const bool f32 = x_dtype == AEGIST_F32;
