@@ -20,17 +20,12 @@ VOCAB = 32768  # a generic output head
 _DT = {"f32": torch.float32, "bf16": torch.bfloat16}
 
 
-_found = []
-
-
 def _ops():
-    if not _found:  # looked for once, as a program's import is
-        for p in (str(Path.cwd()), str(Path.cwd() / "aegist-optimized-ai-library-_amd")):
-            if p not in sys.path:
-                sys.path.insert(0, p)
-        from aegist_mixer import ops
-        _found.append(ops)
-    return _found[0]
+    for p in (str(Path.cwd()), str(Path.cwd() / "aegist-optimized-ai-library-_amd")):
+        if p not in sys.path:
+            sys.path.insert(0, p)
+    from aegist_mixer import ops
+    return ops
 
 
 def listed():
