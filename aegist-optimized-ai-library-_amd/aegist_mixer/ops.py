@@ -460,6 +460,12 @@ def _scratch(nbytes: int, device):
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
+def _int_sizes(*sizes):
+    """The library's sizes are 32-bit, and ctypes cuts longer ones off without a word."""
+    if max(sizes) > 0x7fffffff:
+        raise AegistError("shape", -1, f"sizes {sizes}: at most 2^31 - 1 each")
+
+
 def _rows(x, what: str):
     """x [..., K] as [M, K] with contiguous rows, and its row stride."""
     shape = x.shape
@@ -471,6 +477,7 @@ def _rows(x, what: str):
     ld, one = x.stride()
     if one != 1 and shape[1] > 1:
         raise AegistError("layout", -1, f"{what} rows must be contiguous")
+    _int_sizes(*shape)
     return x, ld if shape[0] > 1 else -(-shape[1] // 8) * 8
 
 
@@ -489,6 +496,7 @@ class Q4Weight:
 
 
 def _q4_empty(N: int, K: int, group: int, device):
+    _int_sizes(N, K, group)
     nbytes = lib().aegist_q4_bytes(N, K, group)
     if nbytes == 0 and N > 0:
         raise AegistError("q4", -1, f"no 4-bit form of [{N}, {K}] in groups of {group}: groups of 32, 64 or 128, "
@@ -583,10 +591,12 @@ def _logprob_outputs(lead, tokens, top: int, device):
     if tokens.shape != lead:
         raise AegistError("shape", -1, f"tokens {tuple(tokens.shape)} for rows {tuple(lead)}")
     _need_contig(tokens)
+    if not 0 <= top <= 64:  # (before the lists are allocated)
+        raise AegistError("shape", -1, f"{top} alternatives: 0 to 64 expected")
     # (empty_like: torch.empty of a torch.Size takes 0.8 us longer)
     f32 = torch.float32
     logprob, entropy = torch.empty_like(tokens, dtype=f32), torch.empty_like(tokens, dtype=f32)
-    if top <= 0:
+    if top == 0:
         return TokenLogprobs(logprob, entropy, None, None)
     ids = torch.empty(*lead, top, dtype=torch.int32, device=device)
     return TokenLogprobs(logprob, entropy, ids, torch.empty_like(ids, dtype=f32))
@@ -618,6 +628,7 @@ def head_logprobs(x, weight, tokens, top: int = 0, scale=None) -> TokenLogprobs:
     x [..., K] fp32 or bf16 (rows contiguous, 16-byte aligned); weight [V, K]: a Q4Weight, int8 with scale bf16
     [V], or bf16 (scale None or bf16 [V]); tokens int32 [...]."""
     V, K = weight.shape
+    _int_sizes(V)
     q4 = isinstance(weight, Q4Weight)
     x2, ldx = _rows(x, "x")
     if x2.shape[1] != K:

@@ -243,3 +243,23 @@ def test_head_refuses_a_workspace_without_the_operands_of_a_4_bit_product():
         return L.aegist_head_logprobs(1 << 40, 1, K, 1 << 41, 3, None, 64, 64, 64, None, None, T, V, K, 64, 0, 1 << 42, n, None)
     assert call(need - 1) == -2 and "linear_q4" in _lib.last_error()
     assert call(100) == -2 and "head_logprobs" in _lib.last_error()
+
+
+def test_sizes_past_32_bits_are_refused(launches):
+    """ctypes would pass them on modulo 2^32: a vocabulary of 2^32 + 5 as one of 5."""
+    def m(*shape, dtype=torch.float32):
+        return torch.empty(*shape, dtype=dtype, device="meta").as_subclass(_OnGpu)
+    big, u8, i32, f16, bf = 2 ** 32, torch.uint8, torch.int32, torch.float16, torch.bfloat16
+    w4 = ops.Q4Weight(m(1, dtype=u8), (16, 64), 64)
+    for call in (lambda: ops.q4_pack(m(big + 16, 32, dtype=u8), m(big + 16, 1, dtype=f16)),
+                 lambda: ops.q4_quantize(m(big + 16, 64)), lambda: ops.q4_quantize(m(16, big + 64)),
+                 lambda: ops.q4_quantize(m(16, 64), big + 64), lambda: ops.linear_q4(m(big + 2, 64), w4),
+                 lambda: ops.linear_q4(m(2, big // 4, 1, 64), w4),
+                 lambda: ops.token_logprobs(m(1, big + 5), m(1, dtype=i32)),
+                 lambda: ops.token_logprobs(m(big + 3, 5), m(big + 3, dtype=i32)),
+                 lambda: ops.token_logprobs(m(3, 5), m(3, dtype=i32), big + 2), lambda: ops.token_logprobs(m(3, 5), m(3, dtype=i32), -1),
+                 lambda: ops.head_logprobs(m(3, 64), m(big + 7, 64, dtype=bf), m(3, dtype=i32)),
+                 lambda: ops.head_logprobs(m(big + 3, 64), w4, m(big + 3, dtype=i32))):
+        with pytest.raises(ops.AegistError):
+            call()
+    assert not launches
