@@ -625,8 +625,9 @@ def token_logprobs(logits, tokens, top: int = 0) -> TokenLogprobs:
 def head_logprobs(x, weight, tokens, top: int = 0, scale=None) -> TokenLogprobs:
     """token_logprobs of the logits x weight^T of an output head, which are never whole in memory.
 
-    x [..., K] fp32 or bf16 (rows contiguous, 16-byte aligned); weight [V, K]: a Q4Weight, int8 with scale bf16
-    [V], or bf16 (scale None or bf16 [V]); tokens int32 [...]."""
+    x [..., K] fp32 or bf16 (rows contiguous, 16-byte aligned), K a multiple of 16; weight [V, K]: a Q4Weight, int8
+    with scale bf16 [V], or bf16 (scale None or bf16 [V]); tokens int32 [...]. Rows count with all their bits
+    (a Q4Weight: as in linear_q4), so that their answers do not depend on the batch but for the order of sums."""
     V, K = weight.shape
     _int_sizes(V)
     q4 = isinstance(weight, Q4Weight)

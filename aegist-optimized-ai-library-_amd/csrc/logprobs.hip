@@ -498,6 +498,26 @@ __global__ void __launch_bounds__(NT) logprobs_join_kernel(const Part* __restric
     }
 }
 
+// fp32 rows [rows, K] (K a multiple of 16) as A + R, A the first 16 bits of each value and R the other 8, which bf16 holds:
+// the projections of several rows count an fp32 value with 16 bits, so A's product is one of all its bits and R's adds the
+// rest. (An infinity leaves a NaN in R.)
+__global__ void __launch_bounds__(256) split_rows_kernel(const float* __restrict__ X, long long ldx, int rows, int K,
+                                                         float* __restrict__ A, uint16_t* __restrict__ R) {
+    const int k4 = K / 4;
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < (size_t)rows * k4; i += (size_t)gridDim.x * 256) {
+        const f32x4 x = *(const f32x4*)(X + (i / k4) * ldx + i % k4 * 4);
+        f32x4 a;
+        uint32_t r[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            a[e] = __uint_as_float(__float_as_uint(x[e]) & 0xffffff00u);
+            r[e] = __float_as_uint(x[e] - a[e]) >> 16;  // (exact)
+        }
+        *(f32x4*)(A + i * 4) = a;
+        *(uint2*)(R + i * 4) = uint2{r[0] | r[1] << 16, r[2] | r[3] << 16};
+    }
+}
+
 int check_out(const char* who, int T, int V, const LogprobOut& o) {
     const std::string w(who);
     if (T < 0 || V < 1 || V > MAX_V)
@@ -568,6 +588,16 @@ int head_rows(int T, int V) { return (int)std::max(1LL, std::min<long long>(T, (
 
 size_t head_logits_bytes(int T, int V) { return ((size_t)head_rows(T, V) * V * 4 + 255) / 256 * 256; }
 
+// Whether `rows` rows go to the product as A + R: fp32 ones on int8 or bf16 weights, where the projection does not take all
+// their bits as it is (it does for one row, and for two on bf16 weights).
+bool head_splits(int x_dtype, int w_dtype, int rows) {
+    return x_dtype == AEGIST_F32 && w_dtype != AEGIST_Q4 && rows > (w_dtype == AEGIST_BF16 ? 2 : 1);
+}
+size_t head_a_bytes(int rows, int K) { return ((size_t)rows * K * 4 + 255) / 256 * 256; }
+size_t head_split_bytes(int x_dtype, int w_dtype, int rows, int K) {
+    return head_splits(x_dtype, w_dtype, rows) ? head_a_bytes(rows, K) + ((size_t)rows * K * 2 + 255) / 256 * 256 : 0;
+}
+
 }  // namespace
 
 extern "C" size_t aegist_token_logprobs_workspace_bytes(int T, int V, int top) {
@@ -596,6 +626,7 @@ extern "C" size_t aegist_head_logprobs_workspace_bytes(int x_dtype, int w_dtype,
     if (T < 1 || V < 1 || V > MAX_V || K < 1) return 0;
     const int rows = head_rows(T, V);
     return head_logits_bytes(T, V) + aegist_token_logprobs_workspace_bytes(rows, V, top) +
+           head_split_bytes(x_dtype, w_dtype, rows, K) +
            (w_dtype == AEGIST_Q4 ? aegist_linear_q4_workspace_bytes(x_dtype, rows, V, K, group) : 0);
 }
 
@@ -613,13 +644,17 @@ extern "C" int aegist_head_logprobs(const void* X, int x_dtype, long long ldx, c
     if (w_dtype == AEGIST_Q4 && (rc = check_q4("head_logprobs", V, K, group))) return rc;
     if (T == 0) return 0;
     if (!X || !W || K < 1) return fail(AEGIST_ERR_SHAPE, "head_logprobs: null operand or K < 1");
+    if (w_dtype != AEGIST_Q4 && (K % 16 || ldx < K || ldx * (x_dtype == AEGIST_F32 ? 4 : 2) % 16 || (uintptr_t)X % 16))
+        return fail(AEGIST_ERR_SHAPE, "head_logprobs: X needs 16-byte aligned rows (ldx >= K), K a multiple of 16");
     const hipStream_t st = AEG_STREAM(stream);
     const int block = head_rows(T, V), xs = x_dtype == AEGIST_F32 ? 4 : 2;
     const size_t lb = head_logits_bytes(T, V), pb = aegist_token_logprobs_workspace_bytes(block, V, top);
-    rc = check_workspace(ws, ws_bytes, lb + pb, "head_logprobs");  // (what is behind them linear_q4 checks)
-    if (rc) return rc;
+    rc = check_workspace(ws, ws_bytes, lb + pb + head_split_bytes(x_dtype, w_dtype, block, K), "head_logprobs");
+    if (rc) return rc;  // (what a 4-bit product needs behind them linear_q4 checks)
     float* logits = (float*)ws;
     char *pws = (char*)ws + lb, *lws = pws + pb;
+    float* xa = (float*)lws;
+    uint16_t* xr = (uint16_t*)(lws + head_a_bytes(block, K));
     const int splits = row_stats_splits(V);
     Part* parts = (Part*)ws;
     u64* keys = (u64*)(parts + (size_t)block * splits);
@@ -637,8 +672,15 @@ extern "C" int aegist_head_logprobs(const void* X, int x_dtype, long long ldx, c
             if (rc || (rc = run_join(parts, keys, m, V, splits, part, st))) return rc;
             continue;
         }
-        rc = w_dtype == AEGIST_Q4 ? launch_linear_q4(x, x_dtype, ldx, W, logits, V, m, V, K, group, 0, lws, ws_bytes - lb - pb, st)
-                                  : launch_proj(x, x_dtype, ldx, W, w_dtype, scale, logits, V, m, V, K, 0, st);
+        if (head_splits(x_dtype, w_dtype, m)) {
+            const size_t n = ((size_t)m * K / 4 + 255) / 256;
+            split_rows_kernel<<<(unsigned)std::min<size_t>(n, 1 << 16), 256, 0, st>>>((const float*)x, ldx, m, K, xa, xr);
+            if ((rc = after_launch("head_logprobs"))) return rc;
+            rc = launch_proj(xr, AEGIST_BF16, K, W, w_dtype, scale, logits, V, m, V, K, 0, st);
+            if (!rc) rc = launch_proj(xa, AEGIST_F32, K, W, w_dtype, scale, logits, V, m, V, K, 1, st);
+        } else
+            rc = w_dtype == AEGIST_Q4 ? launch_linear_q4(x, x_dtype, ldx, W, logits, V, m, V, K, group, 0, lws, ws_bytes - lb - pb, st)
+                                      : launch_proj(x, x_dtype, ldx, W, w_dtype, scale, logits, V, m, V, K, 0, st);
         if (rc) return rc;
         if ((rc = run_logprobs(logits, AEGIST_F32, V, m, V, pws, part, st))) return rc;
     }

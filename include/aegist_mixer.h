@@ -345,7 +345,8 @@ int aegist_gated_norm2(const float* o, const float* z, const uint16_t* w, float*
 /* -------------------------------------------------------------------------------------
  * Projections (QLinear, aegist/model.py:78-93: int8 weight W [N, K] with a per-output-row bf16
  * absmax scale; and plain bf16 weights):  Y[m, n] (+)= scale[n] * sum_k X[m, k] W[n, k],
- * fp32 accumulation; accumulate != 0 adds into Y (the fused residual add). K % 16 == 0 and
+ * fp32 accumulation; accumulate != 0 adds into Y (the fused residual add). From three rows on (two on wide int8
+ * weights) an fp32 value of X counts with 16 bits. K % 16 == 0 and
  * 16-byte aligned X / W rows. Weight-streaming MFMA kernel: one pass over W for M <= 64.
  * ------------------------------------------------------------------------------------- */
 /* gemv_i8, aegist_rs/kernels/aegist.cu:85-91 (launched by HybridEngine::mm, hybrid.rs:717-724) */
@@ -458,7 +459,9 @@ int aegist_token_logprobs(const void* logits, int dtype, long long ld, const int
                           size_t ws_bytes, void* stream);
 /* The same for the logits X W^T of an output head W [V, K]: AEGIST_I8 with scale, AEGIST_BF16 (scale NULL
  * or per row; group is ignored) as in aegist_linear, or AEGIST_Q4 (scale is ignored). The logits are made
- * in blocks of rows in the workspace, or (bf16 operands, many rows, at most one alternative) not at all. */
+ * in blocks of rows in the workspace, or (bf16 operands, many rows, at most one alternative) not at all.
+ * Rows of X count with all their bits (on a 4-bit head with those of aegist_linear_q4), however many there are: fp32 rows
+ * on the other heads are two products, of 16 bits and of the rest. X needs 16-byte aligned rows, K % 16 == 0. */
 size_t aegist_head_logprobs_workspace_bytes(int x_dtype, int w_dtype, int T, int V, int K, int group, int top);
 int aegist_head_logprobs(const void* X, int x_dtype, long long ldx, const void* W, int w_dtype, const uint16_t* scale,
                          const int* tokens, float* logprob, float* entropy, int* top_ids, float* top_logprobs, int T,

@@ -423,3 +423,73 @@ def test_one_row_without_leading_dimensions(dev):
     a, b = ops.token_logprobs(x[0].to(dev), tok[0].to(dev), 3), ops.token_logprobs(x.to(dev), tok.to(dev), 3)
     assert a.logprob.shape == () and a.top_ids.shape == (3,)
     assert all(torch.equal(p, q[0]) for p, q in zip(a, b))
+
+
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+@pytest.mark.parametrize("T", [1, 2, 3, 16, 70, 300, 1000])
+@pytest.mark.parametrize("V", [1003, 9001])
+def test_head_counts_fp32_rows_with_all_their_bits(dev, kind, T, V):
+    """Values 1 + i 2^-7 + 2^-8 + 2^-17 against weights of 0 and 1: every partial sum is a multiple of 2^-17 below 2^7, so
+    the logits are exact in fp32 in any order, and held to the tolerances of given logits. The first 16 bits of a value
+    alone are 2^-17 off, up to 64 2^-17 in the difference of two logits: 16 of those tolerances. Beside them rows at the
+    ends of fp32's range, of zeros and with a NaN or an infinity."""
+    K, top = 64, 5
+    g = torch.Generator().manual_seed(T + V)
+    x = 1 + torch.randint(0, 64, (T, K), generator=g) * 2.0 ** -7 + 2.0 ** -8 + 2.0 ** -17
+    x *= torch.where(torch.arange(T) % 3 == 2, -1.0, 1.0).unsqueeze(1)
+    w = (torch.arange(K) < torch.randint(0, K + 1, (V, 1), generator=g)).float()
+    tok = torch.randint(0, V, (T,), generator=g, dtype=torch.int32)
+    if T > 10:
+        x[3], x[4], x[5] = 0, 0, 1e-38
+        x[4, 20] = 3.3e38
+    args = (w.to(dev).to(torch.bfloat16), None) if kind == "bf16" else (w.to(dev).to(torch.int8), torch.ones(V, device=dev).bfloat16())
+    r = ops.head_logprobs(x.to(dev), args[0], tok.to(dev), top, scale=args[1])
+    keep = torch.arange(T) != 5  # (logits next to 0: ties by the order of their sums)
+    _check((x.double() @ w.double().t())[keep], tok[keep], top, type(r)(*(f[keep.to(dev)] for f in r)))
+    if T > 10:
+        assert abs(float(r.logprob[5]) + math.log(V)) < 1e-4
+        xb = x.clone()
+        xb[0, 3], xb[T - 1, K - 1] = float("nan"), INF
+        b = ops.head_logprobs(xb.to(dev), args[0], tok.to(dev), top, scale=args[1])
+        for p, q in zip(b, r):
+            assert torch.equal(p[1:T - 1], q[1:T - 1])
+        assert all(torch.isnan(p[t]).all() for p in (b.logprob, b.entropy, b.top_logprobs) for t in (0, T - 1))
+
+
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+def test_head_of_fp32_rows_takes_strides_and_graphs(dev, kind):
+    """Rows of a wider matrix, replayed between eager calls, and a last block that is smaller than the ones before it."""
+    T, V, K, top = 40, 5003, 128, 3
+    w, s, _ = _head(kind, V, K, 3, dev)
+    wide = torch.randn(T, K + 64, device=dev)
+    x = wide[:, 64:]
+    tok = torch.randint(0, V, (T,), device=dev, dtype=torch.int32)
+    ops.head_logprobs(x, w, tok, top, scale=s)
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        out = ops.head_logprobs(x, w, tok, top, scale=s)
+    for _ in range(3):
+        wide.copy_(torch.randn(T, K + 64, device=dev))
+        gr.replay()
+        ops.head_logprobs(torch.randn(3 * T, K, device=dev), w, torch.zeros(3 * T, device=dev, dtype=torch.int32), top, scale=s)
+        torch.cuda.synchronize()
+        for a, b in zip(out, ops.head_logprobs(x.contiguous(), w, tok, top, scale=s)):
+            assert torch.equal(a, b)
+    V = 2 ** 22 + 5  # 15 rows to a block of 256 MiB: 2 blocks and one row
+    w = (torch.randn(V, 16, device=dev) * 0.05).bfloat16()
+    x, tok = torch.randn(31, 16, device=dev), torch.randint(0, V, (31,), device=dev, dtype=torch.int32)
+    a, b = ops.head_logprobs(x, w, tok, top), ops.head_logprobs(x[28:].contiguous(), w, tok[28:], top)
+    # 16 products in another order
+    off = 2 * 16 * 2.0 ** -24 * 2 * float((x.abs() @ w.float().abs().t()).amax()) + 2.0 ** -15
+    assert (a.logprob[28:] - b.logprob).abs().max() <= off and (a.top_logprobs[28:] - b.top_logprobs).abs().max() <= off
+
+
+def test_head_refuses_rows_that_are_not_aligned(dev):
+    V, K = 100, 64
+    w, tok = torch.zeros(V, K, device=dev).bfloat16(), torch.zeros(4, device=dev, dtype=torch.int32)
+    wide = torch.zeros(4, K + 6, device=dev)
+    for x in (wide[:, :K], torch.zeros(4, K + 4, device=dev)[:, 1:1 + K]):
+        with pytest.raises(ops.AegistError, match="aligned"):
+            ops.head_logprobs(x, w, tok)
+    with pytest.raises(ops.AegistError, match="multiple of 16"):
+        ops.head_logprobs(torch.zeros(4, 24, device=dev), torch.zeros(V, 24, device=dev).bfloat16(), tok)
