@@ -429,8 +429,26 @@ __global__ void __launch_bounds__(NT) logprobs_kernel(const T* __restrict__ L, l
                 }
                 add_candidates(s, hits[wave], v, mt, thr, c, c1, lane);
                 __syncthreads();
-                const int n = s.count;
-                if (n <= CAP + MAX_TOP && !q.bad) {  // (NaN comes first, and no float comparison finds it)
+                int n = s.count, least = 0;
+                if (n > CAP + MAX_TOP && have < top && !q.bad) {
+                    // too many, as where masks are the type's lowest value: values above the bound, and of those equal to
+                    // it the ones among the first 2 top tokens, which are the lowest, if that makes enough. (Read
+                    // again. 1000 rows of 32768 with all but 16 masked, 20 alternatives: 55 us, by maxima one after the other
+                    // 503, masked with -inf 28.)
+                    __syncthreads();
+                    if (threadIdx.x == 0) s.count = have;
+                    __syncthreads();
+#pragma unroll 4
+                    for (int i = 0; i < 4 * VPT; i++) {
+                        const int ce = c + 4 * NT * (i / 4) + i % 4;
+                        const u64 k = ce < c1 ? lp_key(Act<T>::ld(x, ce), ce) : 0;
+                        if ((uint32_t)(k >> 32) > low || ((uint32_t)(k >> 32) == low && ce - b < 2 * top)) add_candidate(s, k);
+                    }
+                    __syncthreads();
+                    n = s.count;
+                    least = min(top, c1 - b);
+                }
+                if (n >= least && n <= CAP + MAX_TOP && !q.bad) {  // (NaN comes first, and no float comparison finds it)
                     if (n > have) rank_keys(s, n, top);
                     have = min(top, n);
                 } else {

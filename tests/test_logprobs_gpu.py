@@ -493,3 +493,51 @@ def test_head_refuses_rows_that_are_not_aligned(dev):
             ops.head_logprobs(x, w, tok)
     with pytest.raises(ops.AegistError, match="multiple of 16"):
         ops.head_logprobs(torch.zeros(4, 24, device=dev), torch.zeros(V, 24, device=dev).bfloat16(), tok)
+
+
+@pytest.mark.parametrize("V", [100, 3000, 9001, 40000, 70001])
+@pytest.mark.parametrize("T", [10, 400])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_many_logits_alike(dev, V, T, dtype):
+    """Most of a row equal, at the type's lowest value or in the middle, with few or many above it and others below it
+    among the first tokens, in the middle or nowhere."""
+    g = torch.Generator().manual_seed(V)
+    low, at = torch.finfo(dtype).min, torch.arange(V)
+    live = torch.randperm(V, generator=g)[:16]
+    rows = [torch.full((V,), low) for _ in range(4)] + [torch.zeros(V) for _ in range(5)]
+    for r in rows[:2]:
+        r[live[:3]] = torch.tensor([1.0, 2.0, 2.0])
+    rows[1][:min(200, V // 2)] = -INF                       # none of the first tokens is at the mask
+    rows[2][at % 2 == 0] = -INF
+    rows[3][V - min(1000, V // 2):] = torch.randn(min(1000, V // 2), generator=g)
+    rows[4][live] = torch.arange(16) * 0.25 + 0.25          # above the others, fewer than asked for
+    rows[5][torch.randperm(V, generator=g)[:min(300, V // 2)]] = 3.0   # two values alike, one more often than asked for
+    rows[6][:min(150, V // 2)] = -1.0                       # the lowest tokens are below
+    rows[7][at % 2 == 0] = -0.0
+    rows[7][live[:5]] = 1e-3
+    rows[8][live] = -1.0
+    rows.append(torch.full((V,), torch.finfo(dtype).max))
+    x = torch.stack([rows[t % 10] for t in range(T)]).to(dtype)
+    tok = torch.where(torch.arange(T) % 2 == 0, live[torch.arange(T) % 16], torch.randint(0, V, (T,), generator=g)).int()
+    for top in (1, 3, 20, 64):
+        _check(x, tok, top, ops.token_logprobs(x.to(dev), tok.to(dev), top))
+
+
+def test_masks_of_the_lowest_value_cost_about_what_minus_infinity_costs(dev):
+    """(By maxima one after the other 20 alternatives took 18 times as long, 64 of them 50 times.)"""
+    T, V, top = 1000, 32768, 20
+    x = torch.randn(T, V, device=dev)
+    keep = torch.rand(T, V, device=dev) < 16 / V
+    tok = torch.zeros(T, dtype=torch.int32, device=dev)
+    def us(mask):
+        y, best = torch.where(keep, x, mask), INF
+        for _ in range(8):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            for _ in range(8):
+                ops.token_logprobs(y, tok, top)
+            b.record()
+            torch.cuda.synchronize()
+            best = min(best, a.elapsed_time(b))
+        return best
+    assert us(torch.finfo(torch.float32).min) < 6 * us(-INF)
