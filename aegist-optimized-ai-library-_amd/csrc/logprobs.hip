@@ -3,7 +3,9 @@
 //
 //   m = max x,  z = sum e^(x - m),  logprob = x[token] - m - ln z,  entropy = ln z - sum e^(x - m) (x - m) / z
 //
-// (the entropy's sum is taken over x - m, not x, so that a common offset of the logits costs no digits). Logits
+// (the entropy's sum is taken over x - m, not x, so that a common offset of the logits costs no digits). Exponentials are
+// the hardware's 2^y of the rounded product y = (x - m) log2 e: an error of |x - m| 2^-24 and an ulp in a term, where a
+// library exponential has an ulp or two; it is felt below an ulp of the log probability. Logits
 // of -inf have no probability; a row of nothing else has logprob -inf for every token and entropy 0. NaN or
 // +inf anywhere in a row makes its logprobs and entropy NaN.
 //
@@ -556,7 +558,12 @@ int check_out(const char* who, int T, int V, const LogprobOut& o) {
 //     with 20: 14.4, in 8 splits 11.0);
 //   - longer rows, fewer than 384: so many splits that about 1536 workgroups share them (6 per CU); of the small
 //     segments if those are up to 8192 logits (1 row of 131072 with 20: 11.9 us, in 8 large splits 15.3);
-//   - more rows: one workgroup each (500 rows of 100000 with 5: 42 us, in 3 splits 46).
+//   - more rows: one workgroup each. Without alternatives and with 5, against 3 or 4 splits, us:
+//       rows x logits   384 x 40000         450 x 100003        512 x 262144        384 x 2^20          600 x 2^20
+//       fp32            16, 22 (17, 23)     34, 43 (39, 44)     86, 89 (88, 96)     237, 273 (240, 245) 447, 440 (388, 394)
+//       bf16            16, 23 (16, 22)     35, 46 (35, 46)     65, 84 (64, 81)     233, 269 (159, 186) 309, 340 (246, 284)
+//     At 700 x 40000 it is 24, 27 (29, 37). What it costs: bf16 rows longer than about 200000 at up to 700 rows (700 x 2^20:
+//     317, 343 against 289, 320), where a workgroup's segments follow one another by their latency.
 struct Form {
     int vpt, span, splits;
 };
