@@ -608,10 +608,7 @@ int run_logprobs(const void* L, int dtype, long long ld, int T, int V, void* ws,
     return rc || f.splits == 1 ? rc : run_join(parts, tops, T, V, f.splits, o, st);
 }
 
-// rows of logits that are whole at a time: 256 MiB
-int head_rows(int T, int V) { return (int)std::max(1LL, std::min<long long>(T, (256LL << 20) / (4LL * V))); }
-
-size_t head_logits_bytes(int T, int V) { return ((size_t)head_rows(T, V) * V * 4 + 255) / 256 * 256; }
+size_t head_logits_bytes(int rows, int V) { return ((size_t)rows * V * 4 + 255) / 256 * 256; }
 
 // Whether `rows` rows go to the product as A + R: fp32 ones on int8 or bf16 weights, where the projection does not take all
 // their bits as it is (it does for one row, and for two on bf16 weights).
@@ -621,6 +618,13 @@ bool head_splits(int x_dtype, int w_dtype, int rows) {
 size_t head_a_bytes(int rows, int K) { return ((size_t)rows * K * 4 + 255) / 256 * 256; }
 size_t head_split_bytes(int x_dtype, int w_dtype, int rows, int K) {
     return head_splits(x_dtype, w_dtype, rows) ? head_a_bytes(rows, K) + ((size_t)rows * K * 2 + 255) / 256 * 256 : 0;
+}
+
+// Rows of a block: 256 MiB of logits, and no more of split rows.
+int head_rows(int x_dtype, int w_dtype, int T, int V, int K) {
+    long long rows = (256LL << 20) / (4LL * V);
+    if (head_splits(x_dtype, w_dtype, T)) rows = std::min(rows, (256LL << 20) / (6LL * K));
+    return (int)std::max(1LL, std::min<long long>(T, rows));
 }
 
 }  // namespace
@@ -649,8 +653,8 @@ extern "C" int aegist_token_logprobs(const void* logits, int dtype, long long ld
 
 extern "C" size_t aegist_head_logprobs_workspace_bytes(int x_dtype, int w_dtype, int T, int V, int K, int group, int top) {
     if (T < 1 || V < 1 || V > MAX_V || K < 1) return 0;
-    const int rows = head_rows(T, V);
-    return head_logits_bytes(T, V) + aegist_token_logprobs_workspace_bytes(rows, V, top) +
+    const int rows = head_rows(x_dtype, w_dtype, T, V, K);
+    return head_logits_bytes(rows, V) + aegist_token_logprobs_workspace_bytes(rows, V, top) +
            head_split_bytes(x_dtype, w_dtype, rows, K) +
            (w_dtype == AEGIST_Q4 ? aegist_linear_q4_workspace_bytes(x_dtype, rows, V, K, group) : 0);
 }
@@ -672,8 +676,8 @@ extern "C" int aegist_head_logprobs(const void* X, int x_dtype, long long ldx, c
     if (w_dtype != AEGIST_Q4 && (K % 16 || ldx < K || ldx * (x_dtype == AEGIST_F32 ? 4 : 2) % 16 || (uintptr_t)X % 16))
         return fail(AEGIST_ERR_SHAPE, "head_logprobs: X needs 16-byte aligned rows (ldx >= K), K a multiple of 16");
     const hipStream_t st = AEG_STREAM(stream);
-    const int block = head_rows(T, V), xs = x_dtype == AEGIST_F32 ? 4 : 2;
-    const size_t lb = head_logits_bytes(T, V), pb = aegist_token_logprobs_workspace_bytes(block, V, top);
+    const int block = head_rows(x_dtype, w_dtype, T, V, K), xs = x_dtype == AEGIST_F32 ? 4 : 2;
+    const size_t lb = head_logits_bytes(block, V), pb = aegist_token_logprobs_workspace_bytes(block, V, top);
     rc = check_workspace(ws, ws_bytes, lb + pb + head_split_bytes(x_dtype, w_dtype, block, K), "head_logprobs");
     if (rc) return rc;  // (what a 4-bit product needs behind them linear_q4 checks)
     float* logits = (float*)ws;

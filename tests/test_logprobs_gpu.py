@@ -541,3 +541,14 @@ def test_masks_of_the_lowest_value_cost_about_what_minus_infinity_costs(dev):
             best = min(best, a.elapsed_time(b))
         return best
     assert us(torch.finfo(torch.float32).min) < 6 * us(-INF)
+
+
+def test_head_of_fp32_rows_in_blocks_of_what_they_are_split_into(dev):
+    """A short vocabulary and long rows: blocks of 682 rows by the split rows. Logits exact in fp32, as above."""
+    T, V, K = 700, 100, 65536
+    g = torch.Generator().manual_seed(1)
+    x, w = torch.zeros(T, K), (torch.rand(V, K, generator=g) < 0.5).float()
+    x[:, 5::1024] = 1 + torch.randint(0, 64, (T, 64), generator=g) * 2.0 ** -7 + 2.0 ** -8 + 2.0 ** -17
+    tok = torch.randint(0, V, (T,), generator=g, dtype=torch.int32)
+    r = ops.head_logprobs(x.to(dev), w.to(dev).bfloat16(), tok.to(dev), 4)
+    _check(x[:, 5::1024].double() @ w[:, 5::1024].double().t(), tok, 4, r)

@@ -263,3 +263,21 @@ def test_sizes_past_32_bits_are_refused(launches):
         with pytest.raises(ops.AegistError):
             call()
     assert not launches
+
+
+def test_head_workspace_of_fp32_rows():
+    """fp32 rows are split beside the logits, in blocks of 256 MiB however short the vocabulary is."""
+    L = _lib.lib()
+    def need(xd, wd, T, V=1000, K=8192, group=0):
+        return L.aegist_head_logprobs_workspace_bytes(xd, wd, T, V, K, group, 1)
+    for wd in (1, 2):
+        assert need(0, wd, 10 ** 6) < 1 << 30 and need(0, wd, 10 ** 6, V=5) < 1 << 30
+        assert need(0, wd, 100) >= need(1, wd, 100) + 6 * 100 * 8192
+        assert need(0, wd, 1) == need(1, wd, 1)
+        assert need(0, wd, 7, V=2 ** 27, K=2 ** 28) < 1 << 30   # a row at a time
+    assert need(0, 1, 2) == need(1, 1, 2) and need(0, 2, 2) > need(1, 2, 2)
+    sizes = [need(0, 1, T) for T in (1, 2, 3, 50, 1000, 5461, 5462, 20000, 10 ** 6)]
+    assert sizes == sorted(sizes)
+    def call(n, T=100):
+        return L.aegist_head_logprobs(256, 0, 8192, 256, 1, None, 64, 64, 64, 64, 64, T, 1000, 8192, 0, 1, 1 << 40, n, None)
+    assert call(need(0, 1, 100) - 1) == -2 and "head_logprobs" in _lib.last_error()
