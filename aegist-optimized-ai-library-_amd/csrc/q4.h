@@ -73,6 +73,8 @@ template <> struct X8<uint16_t> {
 
 // AEGIST_OK, or the error of sizes that no Q4 weight has.
 int check_q4(const char* who, int N, int K, int G);
+// The kernel that M rows (of more than 2^19, the first block) take: 0 the stream, else tiles of 2, 4 or 8 x 16 rows.
+int linear_q4_form(int x_dtype, int M, int N, int K, int G);
 size_t linear_q4_workspace(int x_dtype, int M, int N, int K, int G);
 int launch_linear_q4(const void* X, int x_dtype, long long ldx, const void* W, float* Y, long long ldy, int M, int N,
                      int K, int G, int accumulate, void* ws, size_t ws_bytes, hipStream_t st);

@@ -684,13 +684,15 @@ int run_gemm(int form, Q4Args a, int x_dtype, void* ws, hipStream_t st) {
 
 namespace aegist {
 
+int linear_q4_form(int x_dtype, int M, int N, int K, int G) { return q4_form(x_dtype, std::min(M, kMaxRows), Q4Dims{N, K, G}); }
+
 size_t linear_q4_workspace(int x_dtype, int M, int N, int K, int G) {
     const Q4Dims d{N, K, G};
     if (N == 0) return 0;
     M = std::min(M, kMaxRows);
     // (what the choice of any smaller M needs is enough for it)
     for (int m = 32; m < M + 16; m += 16)
-        if (q4_form(x_dtype, std::min(m, M), d)) return XOps(M, x_dtype == AEGIST_F32 ? 2 : 1, d).bytes();
+        if (linear_q4_form(x_dtype, std::min(m, M), N, K, G)) return XOps(M, x_dtype == AEGIST_F32 ? 2 : 1, d).bytes();
     return 0;
 }
 
@@ -717,7 +719,7 @@ int launch_linear_q4(const void* X, int x_dtype, long long ldx, const void* W, f
     for (int m = 0; m < M && !rc; m += std::min(kMaxRows, M - m)) {
         const Q4Args a{(const char*)X + (size_t)m * ldx * xs, ldx, (const unsigned char*)W, Y + (size_t)m * ldy, ldy,
                        std::min(kMaxRows, M - m), accumulate, d, 0};
-        const int form = q4_form(x_dtype, a.M, d);
+        const int form = linear_q4_form(x_dtype, a.M, N, K, G);
         if (!form) rc = run_stream(a, x_dtype, st);
         else if (!(rc = check_workspace(ws, ws_bytes, XOps(a.M, x_dtype == AEGIST_F32 ? 2 : 1, d).bytes(), "linear_q4")))
             rc = run_gemm(form, a, x_dtype, ws, st);
