@@ -477,7 +477,8 @@ def _rows(x, what: str):
     ld, one = x.stride()
     if one != 1 and shape[1] > 1:
         raise AegistError("layout", -1, f"{what} rows must be contiguous")
-    _int_sizes(*shape)
+    if (shape[0] | shape[1]) >> 31:
+        _int_sizes(*shape)
     return x, ld if shape[0] > 1 else -(-shape[1] // 8) * 8
 
 

@@ -521,20 +521,39 @@ __global__ void __launch_bounds__(NT) logprobs_join_kernel(const Part* __restric
 // fp32 rows [rows, K] (K a multiple of 16) as A + R, A the first 16 bits of each value and R the other 8, which bf16 holds:
 // the projections of several rows count an fp32 value with 16 bits, so A's product is one of all its bits and R's adds the
 // rest. (An infinity leaves a NaN in R.)
+template <typename TR>
 __global__ void __launch_bounds__(256) split_rows_kernel(const float* __restrict__ X, long long ldx, int rows, int K,
-                                                         float* __restrict__ A, uint16_t* __restrict__ R) {
+                                                         float* __restrict__ A, TR* __restrict__ R) {
     const int k4 = K / 4;
     for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < (size_t)rows * k4; i += (size_t)gridDim.x * 256) {
         const f32x4 x = *(const f32x4*)(X + (i / k4) * ldx + i % k4 * 4);
-        f32x4 a;
-        uint32_t r[4];
+        f32x4 a, r;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             a[e] = __uint_as_float(__float_as_uint(x[e]) & 0xffffff00u);
-            r[e] = __float_as_uint(x[e] - a[e]) >> 16;  // (exact)
+            r[e] = x[e] - a[e];  // (exact)
         }
         *(f32x4*)(A + i * 4) = a;
-        *(uint2*)(R + i * 4) = uint2{r[0] | r[1] << 16, r[2] | r[3] << 16};
+        if constexpr (sizeof(TR) == 4) {
+            *(f32x4*)(R + i * 4) = r;
+        } else {
+            uint32_t h[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) h[e] = __float_as_uint(r[e]) >> 16;
+            *(uint2*)(R + i * 4) = uint2{h[0] | h[1] << 16, h[2] | h[3] << 16};
+        }
+    }
+}
+
+// Y += Z over n values
+__global__ void __launch_bounds__(256) add_logits_kernel(float* __restrict__ Y, const float* __restrict__ Z, size_t n) {
+    typedef L4<float>::v v4;
+    for (size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (size_t)gridDim.x * 1024) {
+        if (i + 4 <= n) {
+            *(v4*)(Y + i) += *(const v4*)(Z + i);
+        } else {
+            for (size_t j = i; j < n; j++) Y[j] += Z[j];
+        }
     }
 }
 
@@ -608,18 +627,26 @@ int run_logprobs(const void* L, int dtype, long long ld, int T, int V, void* ws,
     return rc || f.splits == 1 ? rc : run_join(parts, tops, T, V, f.splits, o, st);
 }
 
-size_t head_logits_bytes(int rows, int V) { return ((size_t)rows * V * 4 + 255) / 256 * 256; }
-
 // Whether `rows` rows go to the product as A + R: fp32 ones on int8 or bf16 weights, where the projection does not take all
 // their bits as it is (it does for one row, and for two on bf16 weights).
 bool head_splits(int x_dtype, int w_dtype, int rows) {
     return x_dtype == AEGIST_F32 && w_dtype != AEGIST_Q4 && rows > (w_dtype == AEGIST_BF16 ? 2 : 1);
 }
-size_t head_a_bytes(int rows, int K) { return ((size_t)rows * K * 4 + 255) / 256 * 256; }
-size_t head_split_bytes(int x_dtype, int w_dtype, int rows, int K) {
-    return head_splits(x_dtype, w_dtype, rows) ? head_a_bytes(rows, K) + ((size_t)rows * K * 2 + 255) / 256 * 256 : 0;
+// Up to so many rows A and R are the rows of one product, so that it reads the weight once, and their logits are added; more
+// rows take two products. Us, of the products alone, one (two), 131072 x 2048: bf16 16 rows 129 (228), 64 191 (301), 128 332 (368),
+// 300 752 (689); int8 16 rows 65 (118), 64 138 (160), 128 262 (252). 32768 x 2048: bf16 64 rows 46 (60), int8 44 (53).
+constexpr int kStackedRows = 64;
+size_t round256(size_t n) { return (n + 255) / 256 * 256; }
+// (a last block of fewer rows may be stacked where the others are not)
+size_t head_logits_bytes(int x_dtype, int w_dtype, int rows, int V) {
+    const int n = head_splits(x_dtype, w_dtype, rows) ? std::max(rows, 2 * std::min(rows, kStackedRows)) : rows;
+    return round256((size_t)n * V * 4);
 }
-
+size_t head_a_bytes(int rows, int K) { return round256((size_t)rows * K * 4); }
+size_t head_split_bytes(int x_dtype, int w_dtype, int rows, int K) {
+    if (!head_splits(x_dtype, w_dtype, rows)) return 0;
+    return std::max(head_a_bytes(rows, K) + round256((size_t)rows * K * 2), head_a_bytes(2 * std::min(rows, kStackedRows), K));
+}
 // Rows of a block: 256 MiB of logits, and no more of split rows.
 int head_rows(int x_dtype, int w_dtype, int T, int V, int K) {
     long long rows = (256LL << 20) / (4LL * V);
@@ -654,7 +681,7 @@ extern "C" int aegist_token_logprobs(const void* logits, int dtype, long long ld
 extern "C" size_t aegist_head_logprobs_workspace_bytes(int x_dtype, int w_dtype, int T, int V, int K, int group, int top) {
     if (T < 1 || V < 1 || V > MAX_V || K < 1) return 0;
     const int rows = head_rows(x_dtype, w_dtype, T, V, K);
-    return head_logits_bytes(rows, V) + aegist_token_logprobs_workspace_bytes(rows, V, top) +
+    return head_logits_bytes(x_dtype, w_dtype, rows, V) + aegist_token_logprobs_workspace_bytes(rows, V, top) +
            head_split_bytes(x_dtype, w_dtype, rows, K) +
            (w_dtype == AEGIST_Q4 ? aegist_linear_q4_workspace_bytes(x_dtype, rows, V, K, group) : 0);
 }
@@ -677,7 +704,7 @@ extern "C" int aegist_head_logprobs(const void* X, int x_dtype, long long ldx, c
         return fail(AEGIST_ERR_SHAPE, "head_logprobs: X needs 16-byte aligned rows (ldx >= K), K a multiple of 16");
     const hipStream_t st = AEG_STREAM(stream);
     const int block = head_rows(x_dtype, w_dtype, T, V, K), xs = x_dtype == AEGIST_F32 ? 4 : 2;
-    const size_t lb = head_logits_bytes(block, V), pb = aegist_token_logprobs_workspace_bytes(block, V, top);
+    const size_t lb = head_logits_bytes(x_dtype, w_dtype, block, V), pb = aegist_token_logprobs_workspace_bytes(block, V, top);
     rc = check_workspace(ws, ws_bytes, lb + pb + head_split_bytes(x_dtype, w_dtype, block, K), "head_logprobs");
     if (rc) return rc;  // (what a 4-bit product needs behind them linear_q4 checks)
     float* logits = (float*)ws;
@@ -702,11 +729,20 @@ extern "C" int aegist_head_logprobs(const void* X, int x_dtype, long long ldx, c
             continue;
         }
         if (head_splits(x_dtype, w_dtype, m)) {
-            const size_t n = ((size_t)m * K / 4 + 255) / 256;
-            split_rows_kernel<<<(unsigned)std::min<size_t>(n, 1 << 16), 256, 0, st>>>((const float*)x, ldx, m, K, xa, xr);
+            const bool stacked = m <= kStackedRows;
+            const int grid = (int)std::min<size_t>(((size_t)m * K / 4 + 255) / 256, 1 << 16);
+            if (stacked) split_rows_kernel<float><<<grid, 256, 0, st>>>((const float*)x, ldx, m, K, xa, xa + (size_t)m * K);
+            else split_rows_kernel<uint16_t><<<grid, 256, 0, st>>>((const float*)x, ldx, m, K, xa, xr);
             if ((rc = after_launch("head_logprobs"))) return rc;
-            rc = launch_proj(xr, AEGIST_BF16, K, W, w_dtype, scale, logits, V, m, V, K, 0, st);
-            if (!rc) rc = launch_proj(xa, AEGIST_F32, K, W, w_dtype, scale, logits, V, m, V, K, 1, st);
+            if (stacked) {
+                const size_t n = (size_t)m * V;
+                if ((rc = launch_proj(xa, AEGIST_F32, K, W, w_dtype, scale, logits, V, 2 * m, V, K, 0, st))) return rc;
+                add_logits_kernel<<<(int)std::min<size_t>((n + 1023) / 1024, 1 << 16), 256, 0, st>>>(logits, logits + n, n);
+                rc = after_launch("head_logprobs");
+            } else {
+                rc = launch_proj(xr, AEGIST_BF16, K, W, w_dtype, scale, logits, V, m, V, K, 0, st);
+                if (!rc) rc = launch_proj(xa, AEGIST_F32, K, W, w_dtype, scale, logits, V, m, V, K, 1, st);
+            }
         } else
             rc = w_dtype == AEGIST_Q4 ? launch_linear_q4(x, x_dtype, ldx, W, logits, V, m, V, K, group, 0, lws, ws_bytes - lb - pb, st)
                                       : launch_proj(x, x_dtype, ldx, W, w_dtype, scale, logits, V, m, V, K, 0, st);

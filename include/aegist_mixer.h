@@ -461,7 +461,7 @@ int aegist_token_logprobs(const void* logits, int dtype, long long ld, const int
  * or per row; group is ignored) as in aegist_linear, or AEGIST_Q4 (scale is ignored). The logits are made
  * in blocks of rows in the workspace, or (bf16 operands, many rows, at most one alternative) not at all.
  * Rows of X count with all their bits (on a 4-bit head with those of aegist_linear_q4), however many there are: fp32 rows
- * on the other heads are two products, of 16 bits and of the rest. X needs 16-byte aligned rows, K % 16 == 0. */
+ * on the other heads are taken as two, of 16 bits of each value and of the rest. X needs 16-byte aligned rows, K % 16 == 0. */
 size_t aegist_head_logprobs_workspace_bytes(int x_dtype, int w_dtype, int T, int V, int K, int group, int top);
 int aegist_head_logprobs(const void* X, int x_dtype, long long ldx, const void* W, int w_dtype, const uint16_t* scale,
                          const int* tokens, float* logprob, float* entropy, int* top_ids, float* top_logprobs, int T,

@@ -552,3 +552,18 @@ def test_head_of_fp32_rows_in_blocks_of_what_they_are_split_into(dev):
     tok = torch.randint(0, V, (T,), generator=g, dtype=torch.int32)
     r = ops.head_logprobs(x.to(dev), w.to(dev).bfloat16(), tok.to(dev), 4)
     _check(x[:, 5::1024].double() @ w[:, 5::1024].double().t(), tok, 4, r)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+@pytest.mark.parametrize("T,V", [(64, 3001), (65, 3001), (129, 1001), (127 + 30, 2 ** 19 + 3), (2 * 127 + 65, 2 ** 19 + 3)])
+def test_head_where_the_split_rows_stop_being_stacked(dev, kind, T, V):
+    """64 rows and more, and last blocks of 30 and 65 rows behind ones of 127. Logits exact in fp32, as above."""
+    K, top = 64, 3
+    g = torch.Generator().manual_seed(T)
+    x = 1 + torch.randint(0, 64, (T, K), generator=g) * 2.0 ** -7 + 2.0 ** -8 + 2.0 ** -17
+    w = (torch.arange(K) < torch.randint(0, K + 1, (V, 1), generator=g)).to(dev)
+    tok = torch.randint(0, V, (T,), generator=g, dtype=torch.int32)
+    args = (w.bfloat16(), None) if kind == "bf16" else (w.to(torch.int8), torch.ones(V, device=dev).bfloat16())
+    r = ops.head_logprobs(x.to(dev), args[0], tok.to(dev), top, scale=args[1])
+    rows = torch.tensor([0, 1, 63, T - 31, T - 30, T - 29, T - 1])
+    _check(x[rows].double() @ w.cpu().double().t(), tok[rows], top, type(r)(*(f[rows.to(dev)] for f in r)))
