@@ -624,7 +624,8 @@ def token_logprobs(logits, tokens, top: int = 0) -> TokenLogprobs:
 
 
 def head_logprobs(x, weight, tokens, top: int = 0, scale=None) -> TokenLogprobs:
-    """token_logprobs of the logits x weight^T of an output head, which are never whole in memory.
+    """token_logprobs of the logits x weight^T of an output head, which are made in blocks of at most 256 MiB (or a row):
+    with bf16 x and weight, some hundred rows and more and at most one alternative not at all.
 
     x [..., K] fp32 or bf16 (rows contiguous, 16-byte aligned), K a multiple of 16; weight [V, K]: a Q4Weight, int8
     with scale bf16 [V], or bf16 (scale None or bf16 [V]); tokens int32 [...]. Rows count with all their bits

@@ -13,9 +13,10 @@
 // selection of the alternatives read it from there. Segments of a row are joined by their maxima in fixed order; few
 // long rows are cut into splits, which a second launch joins.
 //
-// Bound by HBM for many rows (2000 x 131072 fp32, 8 alternatives: 160 us, 6.5 TB/s with part of it in the last-level
-// cache; without alternatives 154), by the latency of a launch or two for few: 61 rows of 100003 in bf16 take 9.8 us, with
-// 5 alternatives 14.2.
+// Bound by HBM for many rows of fp32 (2000 x 131072, 8 alternatives: 163 to 170 us, 6.2 to 6.4 TB/s with part of it in the
+// last-level cache; without alternatives 165), by a segment's arithmetic, with nothing requested beside it, for as
+// many of bf16 (the same size 125 to 130, without alternatives 103), by the latency of a launch or two for few: 61 rows of
+// 100003 in bf16 take 10.6 us, with 5 alternatives 15.2.
 #include "logprobs.h"
 #include "q4.h"
 
@@ -212,7 +213,7 @@ __device__ __forceinline__ int lanes_below(u64 b) {
 
 // The candidates among a segment's logits: those at or above thr. Few lanes hold any. Up to HITS of those
 // at a time lay all their logits down in LDS, and the wave looks at 64 of them at once: a test and a branch per
-// register would be paid by every wave that holds a single one. (1703 rows of 38708 bf16, 20 alternatives: 57 us with
+// register would be paid by every wave that holds a single one. (1703 rows of 38708 bf16, 20 alternatives: 57 us (60 on other cards) with
 // 4 lanes of 64 logits at a time, 64 with 2, 63 with 8.)
 template <int VPT>
 struct alignas(16) Hits {
@@ -681,6 +682,8 @@ extern "C" int aegist_token_logprobs(const void* logits, int dtype, long long ld
 extern "C" size_t aegist_head_logprobs_workspace_bytes(int x_dtype, int w_dtype, int T, int V, int K, int group, int top) {
     if (T < 1 || V < 1 || V > MAX_V || K < 1) return 0;
     const int rows = head_rows(x_dtype, w_dtype, T, V, K);
+    // (the logits also where the product could leave statistics in their place: that takes an alignment, a stride and a weight
+    // without scales, which are not known here)
     return head_logits_bytes(x_dtype, w_dtype, rows, V) + aegist_token_logprobs_workspace_bytes(rows, V, top) +
            head_split_bytes(x_dtype, w_dtype, rows, K) +
            (w_dtype == AEGIST_Q4 ? aegist_linear_q4_workspace_bytes(x_dtype, rows, V, K, group) : 0);
@@ -721,7 +724,7 @@ extern "C" int aegist_head_logprobs(const void* X, int x_dtype, long long ldx, c
                               top_logprobs ? top_logprobs + (size_t)t * top : nullptr, top};
         // At most one alternative, on the tiles of gemm_bf16: the product leaves the rows' statistics in the place of the
         // logits (40 bytes per 128 columns), which a lane has nearly to itself: it holds 32 columns of a row (1000 rows of
-        // 32768 x 2048: 119 us, 112 without alternatives, by way of the logits 159; their product alone takes 130).
+        // 32768 x 2048: 114 us, 110 without alternatives, by way of the logits 155; their product alone takes 127).
         if (top <= 1 && V >= 256 && proj_is_gemm_bf16(x, x_dtype, ldx, W, w_dtype, scale, m, V, K)) {
             rc = launch_gemm_bf16_stats((const uint16_t*)x, ldx, (const uint16_t*)W, m, V, K,
                                         RowStats{part.tokens, parts, top ? keys : nullptr, splits}, st);

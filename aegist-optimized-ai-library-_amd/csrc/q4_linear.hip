@@ -10,8 +10,10 @@
 //     more of them cost as many bits, 3.5e-6 instead of 2e-7 of the output's 2-norm at 8192 x 2048);
 //   - a row of X is scaled by a power of two so that its largest value lies in [2^14, 2^15). A bf16 value is then
 //     exact in fp16, an fp32 one the sum of two (hi rounded, lo the remainder): 22 bits, where the products
-//     of the codes are exact. Values below 2^-28 of the row's largest lose bits to fp16's subnormals, at
-//     most 2^-39 of that largest;
+//     of the codes are exact (error of the product against 64 bits beside a plain fp32 product's, of the 2-norm: at K = 32
+//     1.26e-7 and 1.02e-7, from K = 64 on the smaller). What fp16's subnormals cut off, an fp32 value below about 2^-17 of
+//     its row's largest to fewer than 22 bits and a bf16 one below about 2^-31 to fewer than 8, is at most 2^-39 of
+//     that largest;
 //   - the sums of a group's X (fp32, rounded to 22 bits in two fp16 parts) against the minima are one more product
 //     with K / G in the place of K.
 // A group's products are summed apart and then join the row's sum with the group's scale, in fp32.
