@@ -484,25 +484,35 @@ def _rows(x, what: str):
 
 class Q4Weight:
     """A weight matrix [N, K] in 4 bits, packed for linear_q4 (the q4 block of include/aegist_mixer.h):
-    w = code * scale + min per `group` consecutive inputs. Made by q4_quantize or q4_pack."""
+    w = code * scale + min per `group` consecutive inputs. Made by q4_quantize or q4_pack, or of the bytes (`data`, uint8)
+    that one of them made for this shape and group."""
 
     __slots__ = ("data", "shape", "group")
 
     def __init__(self, data, shape, group: int):
-        self.data, self.shape, self.group = data, tuple(shape), group
+        N, K = shape
+        if data.dtype != torch.uint8 or not data.is_contiguous() or data.numel() < _q4_bytes(N, K, group):
+            raise AegistError("q4", -1, f"packed [{N}, {K}] in groups of {group}: {_q4_bytes(N, K, group)} contiguous bytes "
+                                        f"expected, got {data.numel()} of {data.dtype}")
+        self.data, self.shape, self.group = data, (N, K), group
 
     @property
     def device(self):
         return self.data.device
 
 
-def _q4_empty(N: int, K: int, group: int, device):
+@functools.lru_cache(maxsize=4096)
+def _q4_bytes(N: int, K: int, group: int) -> int:
     _int_sizes(N, K, group)
     nbytes = lib().aegist_q4_bytes(N, K, group)
-    if nbytes == 0 and N > 0:
+    if nbytes == 0 and N != 0:
         raise AegistError("q4", -1, f"no 4-bit form of [{N}, {K}] in groups of {group}: groups of 32, 64 or 128, "
-                                    "K a positive multiple of the group")
-    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+                                    "K a positive multiple of the group, N and K at most 2^28")
+    return nbytes
+
+
+def _q4_empty(N: int, K: int, group: int, device):
+    return torch.empty(_q4_bytes(N, K, group), dtype=torch.uint8, device=device)
 
 
 def q4_quantize(weight, group: int = 64) -> Q4Weight:

@@ -250,10 +250,10 @@ def test_sizes_past_32_bits_are_refused(launches):
     def m(*shape, dtype=torch.float32):
         return torch.empty(*shape, dtype=dtype, device="meta").as_subclass(_OnGpu)
     big, u8, i32, f16, bf = 2 ** 32, torch.uint8, torch.int32, torch.float16, torch.bfloat16
-    w4 = ops.Q4Weight(m(1, dtype=u8), (16, 64), 64)
+    w4 = ops.Q4Weight(m(2048, dtype=u8), (16, 64), 64)
     for call in (lambda: ops.q4_pack(m(big + 16, 32, dtype=u8), m(big + 16, 1, dtype=f16)),
                  lambda: ops.q4_quantize(m(big + 16, 64)), lambda: ops.q4_quantize(m(16, big + 64)),
-                 lambda: ops.q4_quantize(m(16, 64), big + 64), lambda: ops.linear_q4(m(big + 2, 64), w4),
+                 lambda: ops.q4_quantize(m(16, 64), big + 64), lambda: ops.Q4Weight(m(2048, dtype=u8), (big + 16, 64), 64), lambda: ops.linear_q4(m(big + 2, 64), w4),
                  lambda: ops.linear_q4(m(2, big // 4, 1, 64), w4),
                  lambda: ops.token_logprobs(m(1, big + 5), m(1, dtype=i32)),
                  lambda: ops.token_logprobs(m(big + 3, 5), m(big + 3, dtype=i32)),
@@ -281,3 +281,15 @@ def test_head_workspace_of_fp32_rows():
     def call(n, T=100):
         return L.aegist_head_logprobs(256, 0, 8192, 256, 1, None, 64, 64, 64, 64, 64, T, 1000, 8192, 0, 1, 1 << 40, n, None)
     assert call(need(0, 1, 100) - 1) == -2 and "head_logprobs" in _lib.last_error()
+
+
+def test_packed_weight_of_other_bytes_is_refused():
+    """A block that is shorter than its shape's would be read past its end."""
+    u8, need = torch.uint8, _lib.lib().aegist_q4_bytes(40, 192, 32)
+    w = ops.Q4Weight(_t(need, dtype=u8), [40, 192], 32)
+    assert w.shape == (40, 192) and w.group == 32
+    for data, shape, group in ((_t(need - 1, dtype=u8), (40, 192), 32), (_t(need, dtype=u8), (49, 192), 32), (_t(need, dtype=u8), (40, 320), 32),
+                               (_t(need), (40, 192), 32), (_t(2 * need, dtype=u8)[::2], (40, 192), 32), (_t(need, dtype=u8), (40, 192), 128),
+                               (_t(need, dtype=u8), (40, 192), 48), (_t(need, dtype=u8), (-40, 192), 32)):
+        with pytest.raises(ops.AegistError):
+            ops.Q4Weight(data, shape, group)
